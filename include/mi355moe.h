@@ -22,6 +22,8 @@
  *   mlp_partial over int8 leaves (shared expert, dense MLP) model.py:125-127,855  -> mi_int8_mlp
  *   mlp_partial / x @ W over bf16 leaves (int8_nonexpert off) model.py:125-127,855, engine.py:281 -> mi_bf16_mlp,
  *                                                                                   mi_bf16_project
+ *   fp8 checkpoint weights (dequant_fp8_device)            checkpoint.py:202     -> mi_fp8_project, mi_fp8_mlp, mi_fp8_moe
+ *   gather and combine around the ragged products          resident.py:153-165   -> mi_moe_dispatch, mi_moe_combine
  */
 #ifndef MI355MOE_H
 #define MI355MOE_H
@@ -404,6 +406,86 @@ int mi_mlp_many(const uint16_t *x_bf16, int32_t B, int32_t D, int32_t I, const v
                 int32_t down_form, float limit, uint16_t *y_bf16, float *y_f32, void *workspace,
                 size_t workspace_bytes, void *stream);
 size_t mi_mlp_many_workspace(int32_t B, int32_t D, int32_t I);
+
+/*
+ * Block-scaled fp8.  Activations: e4m3 values (OCP: largest 448, NaN but no infinity) with one f32 scale per row and
+ * group of 128 columns; weights: e4m3 with one f32 scale per 128 x 128 block, the layout of fp8 checkpoints
+ * (checkpoint.py:202), which the reference dequantises:
+ *   wq [E, R, K] row-major, ws f32 [E, ceil(R / 128), ceil(K / 128)];  xq [rows, K], xs f32 [rows, ceil(K / 128)]
+ *   y[b, o] = sum_c xs[b, c] ws[o / 128, c] sum_{i in group c} xq[b, i] wq[o, i]     exact products, f32 sums
+ * The last group and block may be partial.  K (n_in, D, I) % 16 == 0 and R, K <= 2^17; x and the weights 16-byte
+ * aligned; rows * K < 2^31, at most 2^22 rows.
+ *
+ * mi_fp8_quantize: n rows of K bf16 or f32 values, row stride x_stride elements (a multiple of 8) -> q, s:
+ *   a = max |x| of the group's finite values, s = 2^e with the least e >= -100 such that a <= 448 * 2^e,
+ *   q = e4m3(x / s) rounded to nearest even; infinities and NaN become NaN.
+ *   The scale is a power of two: x / s is exact, each value is rounded once.
+ */
+#define MI_X_FP8 2       /* activations quantised already: e4m3 values, with their scales xs */
+int mi_fp8_quantize(const void *x, int32_t x_dtype, int32_t n, int32_t K, int64_t x_stride, uint8_t *q, float *s,
+                    void *stream);
+
+/*
+ * Dense block-scaled product, 1 <= B tokens: x bf16 or f32 [B, n_in] (quantised as by mi_fp8_quantize; xs NULL) or
+ * MI_X_FP8 values with their scales xs.  y_bf16 (one rounding of the f32 sum) and/or y_f32 [B, n_out], any n_out.
+ * Workspace: mi_fp8_project_workspace bytes, 16-byte aligned, no initialisation; its size serves every smaller B.
+ */
+int mi_fp8_project(const void *x, int32_t x_dtype, const float *xs, int32_t B, const uint8_t *wq, const float *ws,
+                   int32_t n_in, int32_t n_out, uint16_t *y_bf16, float *y_f32, void *workspace,
+                   size_t workspace_bytes, void *stream);
+size_t mi_fp8_project_workspace(int32_t B, int32_t n_in, int32_t n_out);
+
+/*
+ * mlp_partial (model.py:125-127) over block-scaled leaves: g, u = x Wg^T, x Wu^T (f32, not rounded),
+ * h = silu(min(g, L)) * clip(u, -L, L) in f32, quantised as by mi_fp8_quantize, y = h Wd^T.  gate, up [I, D], down [D, I].
+ * x and the workspace as for mi_fp8_project.
+ */
+int mi_fp8_mlp(const void *x, int32_t x_dtype, const float *xs, int32_t B, int32_t D, int32_t I,
+               const uint8_t *gate_q, const float *gate_s, const uint8_t *up_q, const float *up_s,
+               const uint8_t *down_q, const float *down_s, float limit, uint16_t *y_bf16, float *y_f32,
+               void *workspace, size_t workspace_bytes, void *stream);
+size_t mi_fp8_mlp_workspace(int32_t B, int32_t D, int32_t I);
+
+/*
+ * The rows of a ragged_plan times their experts' matrices (moe_ragged_down's product, pallas_moe.py:693-755):
+ * n_blk blocks of tm rows (tm 16, 32, 64 or 128), block g's rows times expert blk_expert[g] of E; x (as for
+ * mi_fp8_project) and y have n_blk * tm rows.  Blocks from *n_blocks on, and blocks of an expert outside [0, E), get
+ * zeros.
+ */
+int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, int32_t n_blk, int32_t tm,
+                   const int32_t *blk_expert, const int32_t *n_blocks, const uint8_t *wq, const float *ws, int32_t E,
+                   int32_t K, int32_t R, uint16_t *y_bf16, float *y_f32, void *workspace, size_t workspace_bytes,
+                   void *stream);
+size_t mi_fp8_grouped_workspace(int32_t rows, int32_t K, int32_t R);
+
+/*
+ * The routed experts of one layer (ResidentFetch.apply's composition, resident.py:100-120) over block-scaled weights:
+ *   out[t] = sum_j w[t, j] MLP_{idx[t, j]}(x[t])      MLP as mi_fp8_mlp, its y and the sum in f32, columns in order
+ * x bf16 or f32 [T, D], idx int32 [T, k], w f32 [T, k]; out_f32 and/or out_bf16 [T, D].  A slot whose expert id is
+ * outside [0, E) adds nothing.  E <= 1024, T * k <= 2^22.  Workspace as for mi_fp8_project.
+ */
+int mi_fp8_moe(const uint8_t *gate_q, const float *gate_s, const uint8_t *up_q, const float *up_s,
+               const uint8_t *down_q, const float *down_s, int32_t E, int32_t D, int32_t I, const void *x,
+               int32_t x_dtype, int32_t T, int32_t k, const int32_t *idx, const float *w, float limit,
+               float *out_f32, uint16_t *out_bf16, void *workspace, size_t workspace_bytes, void *stream);
+size_t mi_fp8_moe_workspace(int32_t T, int32_t k, int32_t E, int32_t D, int32_t I);
+
+/*
+ * Tokens into expert order and back over mi_ragged_plan's layout (the gather and combine of _apply_ragged_kernel,
+ * resident.py:153-165), and their gradients; dtype MI_X_BF16 or MI_X_F32 for every row buffer, D % 8 == 0, rows
+ * 16-byte aligned, sums in f32 and in column order, one rounding:
+ *   mi_moe_dispatch      xs[r] = x[tok_row[r]], zeros on padding rows (tok_row -1), r < rows
+ *   mi_moe_combine       out[t] = sum_j w[t, j] y[row_slot[t, j]]; w NULL: weights 1 (dispatch's gradient)
+ *   mi_moe_combine_grad  dy[row_slot[t, j]] = w[t, j] dout[t], zeros on padding rows; dw[t, j] = <dout[t], y[row_slot[t, j]]>
+ * A slot without a row (row_slot -1) adds nothing and gets dw 0.
+ */
+int mi_moe_dispatch(const void *x, int32_t dtype, int32_t T, int32_t k, int32_t D, const int32_t *row_slot,
+                    const int32_t *tok_row, int32_t rows, void *xs, void *stream);
+int mi_moe_combine(const void *y, int32_t dtype, int32_t T, int32_t k, int32_t D, const int32_t *row_slot,
+                   const float *w, int32_t rows, void *out, void *stream);
+int mi_moe_combine_grad(const void *dout, const void *y, int32_t dtype, int32_t T, int32_t k, int32_t D,
+                        const int32_t *row_slot, const int32_t *tok_row, const float *w, int32_t rows, void *dy,
+                        float *dw, void *stream);
 
 /*
  * Launch-plan overrides, for tests and measurement runs only (no counterpart in the reference).  The library reads

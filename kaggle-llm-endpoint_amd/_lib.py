@@ -17,6 +17,7 @@ MI_QT_Q2_K = 5
 MI_QT_Q3_K = 6
 MI_X_BF16 = 0
 MI_X_F32 = 1
+MI_X_FP8 = 2                 # fp8 products: e4m3 values with their scales
 MI_MAX_SLOTS = 128
 MAX_DECODE_TOKENS = 16
 MI_I8_ROW_SCALES = 0         # s [n_in]: the reference's per-row scales [in, 1]
@@ -48,8 +49,9 @@ EXPORTS = ("mi_matvec", "mi_matvec_workspace", "mi_moe_decode", "mi_moe_decode_f
            "mi_moe_prefill_form_workspace", "mi_dequant", "mi_int8_project", "mi_int8_project_workspace", "mi_int8_project_many",
            "mi_int8_project_many_workspace", "mi_int8_mlp", "mi_int8_mlp_workspace", "mi_moe_route", "mi_moe_route_workspace", "mi_pack_planes", "mi_int8_tile", "mi_bf16_project", "mi_bf16_project_workspace",
            "mi_bf16_mlp", "mi_mlp_many", "mi_mlp_many_workspace", "mi_bf16_mlp_workspace", "mi_tuning_set", "mi_tuning_reset",
-           "mi_strerror",
-           "mi_version")
+           "mi_fp8_quantize", "mi_fp8_project", "mi_fp8_project_workspace", "mi_fp8_mlp", "mi_fp8_mlp_workspace",
+           "mi_fp8_grouped", "mi_fp8_grouped_workspace", "mi_fp8_moe", "mi_fp8_moe_workspace", "mi_moe_dispatch",
+           "mi_moe_combine", "mi_moe_combine_grad", "mi_strerror", "mi_version")
 
 
 class MiTable(ctypes.Structure):
@@ -114,6 +116,18 @@ def lib():
         "mi_moe_route": (I, [P, P, P, I, I, I, I, I, F, P, P, P, Z, P]),
         "mi_moe_route_workspace": (Z, [I, I, I]),
         "mi_pack_planes": (I, [I, P, I, I, I, ctypes.POINTER(ctypes.c_void_p), P]),
+        "mi_fp8_quantize": (I, [P, I, I, I, ctypes.c_int64, P, P, P]),
+        "mi_fp8_project": (I, [P, I, P, I, P, P, I, I, P, P, P, Z, P]),
+        "mi_fp8_project_workspace": (Z, [I, I, I]),
+        "mi_fp8_mlp": (I, [P, I, P, I, I, I, P, P, P, P, P, P, F, P, P, P, Z, P]),
+        "mi_fp8_mlp_workspace": (Z, [I, I, I]),
+        "mi_fp8_grouped": (I, [P, I, P, I, I, P, P, P, P, I, I, I, P, P, P, Z, P]),
+        "mi_fp8_grouped_workspace": (Z, [I, I, I]),
+        "mi_fp8_moe": (I, [P, P, P, P, P, P, I, I, I, P, I, I, I, P, P, F, P, P, P, Z, P]),
+        "mi_fp8_moe_workspace": (Z, [I, I, I, I, I]),
+        "mi_moe_dispatch": (I, [P, I, I, I, I, P, P, I, P, P]),
+        "mi_moe_combine": (I, [P, I, I, I, I, P, P, I, P, P]),
+        "mi_moe_combine_grad": (I, [P, P, I, I, I, I, P, P, P, I, P, P, P]),
         "mi_tuning_set": (I, [ctypes.c_char_p, I]),
         "mi_tuning_reset": (None, []),
         "mi_strerror": (ctypes.c_char_p, [I]),

@@ -1,0 +1,171 @@
+// Tokens into expert order and back, and the gradients of both, over the layout of ragged_plan_kernel
+// (pallas_moe.py:564-592): S = T k slots, slot (t, j) has sorted row row_slot[t, j] (-1: none), padding rows have
+// tok_row -1.
+//   dispatch        xs[row] = x[tok_row[row]], 0 on padding rows             its gradient is combine with weights 1
+//   combine         out[t] = sum_j w[t, j] y[row_slot[t, j]]                 f32, in column order, rounded once
+//   combine_grad    dy[row_slot[t, j]] = w[t, j] dout[t], 0 on padding rows;  dw[t, j] = <dout[t], y[row_slot[t, j]]>
+// No atomics: every output element has one writer and a fixed order of summation.  Rows and tokens outside the
+// buffers count as none.
+#include "common.h"
+
+namespace mi {
+
+constexpr int kMoeRowsMax = 1 << 22;
+
+// Eight consecutive elements of a row.
+template <int XD>
+struct Row8 {
+    float v[8];
+    __device__ __forceinline__ void load(const void *p, size_t at) {
+        if constexpr (XD == MI_X_BF16) {
+            const uint4 u = *(const uint4 *)((const uint16_t *)p + at);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            }
+        } else {
+            const float4 a = *(const float4 *)((const float *)p + at), b = *(const float4 *)((const float *)p + at + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        }
+    }
+    __device__ __forceinline__ void store(void *p, size_t at) const {
+        if constexpr (XD == MI_X_BF16) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16_rne(v[2 * j]) | (f32_to_bf16_rne(v[2 * j + 1]) << 16);
+            *(uint4 *)((uint16_t *)p + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            *(float4 *)((float *)p + at) = make_float4(v[0], v[1], v[2], v[3]);
+            *(float4 *)((float *)p + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    }
+};
+
+template <int XD>
+__global__ void __launch_bounds__(256) moe_dispatch_kernel(const void *__restrict__ x, const int32_t *__restrict__ tok_row,
+                                                           int T, int D, void *__restrict__ xs) {
+    const int row = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 8;
+    if (c >= D) return;
+    const int t = tok_row[row];
+    Row8<XD> r = {};
+    if (t >= 0 && t < T) r.load(x, (size_t)t * D + c);
+    r.store(xs, (size_t)row * D + c);
+}
+
+template <int XD>
+__global__ void __launch_bounds__(256) moe_combine_kernel(const void *__restrict__ y, const int32_t *__restrict__ row_slot,
+                                                          const float *__restrict__ w, int k, int D, int rows,
+                                                          void *__restrict__ out) {
+    const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 8;
+    if (c >= D) return;
+    Row8<XD> acc = {};
+    for (int j = 0; j < k; ++j) {
+        const int r = row_slot[(size_t)t * k + j];
+        if (r < 0 || r >= rows) continue;
+        const float wt = w ? w[(size_t)t * k + j] : 1.0f;
+        Row8<XD> v;
+        v.load(y, (size_t)r * D + c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc.v[i] = fmaf(wt, v.v[i], acc.v[i]);
+    }
+    acc.store(out, (size_t)t * D + c);
+}
+
+// Workgroups 0 .. T - 1: one token each; the others zero the padding rows.
+template <int XD>
+__global__ void __launch_bounds__(256) moe_combine_grad_kernel(const void *__restrict__ dout, const void *__restrict__ y,
+                                                               const int32_t *__restrict__ row_slot,
+                                                               const int32_t *__restrict__ tok_row,
+                                                               const float *__restrict__ w, int T, int k, int D,
+                                                               int rows, void *__restrict__ dy, float *__restrict__ dw) {
+    __shared__ float part[4];
+    if ((int)blockIdx.x >= T) {
+        const int row = blockIdx.x - T;
+        const int t = tok_row[row];
+        if (t >= 0 && t < T) return;
+        const Row8<XD> zero = {};
+        for (int c = threadIdx.x * 8; c < D; c += 2048) zero.store(dy, (size_t)row * D + c);
+        return;
+    }
+    const int t = blockIdx.x;
+    for (int j = 0; j < k; ++j) {
+        const int r = row_slot[(size_t)t * k + j];
+        float dot = 0.0f;
+        if (r >= 0 && r < rows) {
+            const float wt = w[(size_t)t * k + j];
+            for (int c = threadIdx.x * 8; c < D; c += 2048) {
+                Row8<XD> g, v;
+                g.load(dout, (size_t)t * D + c);
+                v.load(y, (size_t)r * D + c);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    dot = fmaf(g.v[i], v.v[i], dot);
+                    g.v[i] *= wt;
+                }
+                g.store(dy, (size_t)r * D + c);
+            }
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) dot += __shfl_xor(dot, m, 64);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
+        __syncthreads();
+        if (threadIdx.x == 0) dw[(size_t)t * k + j] = part[0] + part[1] + part[2] + part[3];
+        __syncthreads();
+    }
+}
+
+static int moe_rows_check(int dtype, int T, int k, int D, int rows) {
+    if (dtype != MI_X_BF16 && dtype != MI_X_F32) return MI_ERR_ARG;
+    if (T <= 0 || k <= 0 || (long long)T * k > kMoeRowsMax || rows <= 0 || rows > 2 * kMoeRowsMax) return MI_ERR_TOKENS;
+    if (D <= 0 || D % 8 || D > (1 << 17)) return MI_ERR_SHAPE;
+    return MI_OK;
+}
+static bool moe_rows_aligned(const void *a, const void *b, const void *c = nullptr) {
+    return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15) == 0;
+}
+static bool words_aligned(const void *a, const void *b = nullptr, const void *c = nullptr) {
+    return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 3) == 0;
+}
+
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" int mi_moe_dispatch(const void *x, int32_t dtype, int32_t T, int32_t k, int32_t D, const int32_t *row_slot,
+                               const int32_t *tok_row, int32_t rows, void *xs, void *stream) {
+    if (!x || !row_slot || !tok_row || !xs) return MI_ERR_NULL;
+    const int rc = moe_rows_check(dtype, T, k, D, rows);
+    if (rc != MI_OK) return rc;
+    if (!moe_rows_aligned(x, xs) || !words_aligned(row_slot, tok_row)) return MI_ERR_ARG;
+    auto kern = dtype == MI_X_BF16 ? moe_dispatch_kernel<MI_X_BF16> : moe_dispatch_kernel<MI_X_F32>;
+    hipLaunchKernelGGL(kern, dim3(rows, (D + 2047) / 2048), dim3(256), 0, (hipStream_t)stream, x, tok_row, T, D, xs);
+    return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
+}
+
+extern "C" int mi_moe_combine(const void *y, int32_t dtype, int32_t T, int32_t k, int32_t D, const int32_t *row_slot,
+                              const float *w, int32_t rows, void *out, void *stream) {
+    if (!y || !row_slot || !out) return MI_ERR_NULL;
+    const int rc = moe_rows_check(dtype, T, k, D, rows);
+    if (rc != MI_OK) return rc;
+    if (!moe_rows_aligned(y, out) || !words_aligned(row_slot, w)) return MI_ERR_ARG;
+    auto kern = dtype == MI_X_BF16 ? moe_combine_kernel<MI_X_BF16> : moe_combine_kernel<MI_X_F32>;
+    hipLaunchKernelGGL(kern, dim3(T, (D + 2047) / 2048), dim3(256), 0, (hipStream_t)stream, y, row_slot, w, k, D, rows,
+                       out);
+    return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
+}
+
+extern "C" int mi_moe_combine_grad(const void *dout, const void *y, int32_t dtype, int32_t T, int32_t k, int32_t D,
+                                   const int32_t *row_slot, const int32_t *tok_row, const float *w, int32_t rows,
+                                   void *dy, float *dw, void *stream) {
+    if (!dout || !y || !row_slot || !tok_row || !w || !dy || !dw) return MI_ERR_NULL;
+    const int rc = moe_rows_check(dtype, T, k, D, rows);
+    if (rc != MI_OK) return rc;
+    if (!moe_rows_aligned(dout, y, dy) || !words_aligned(row_slot, tok_row, w) || !words_aligned(dw)) return MI_ERR_ARG;
+    auto kern = dtype == MI_X_BF16 ? moe_combine_grad_kernel<MI_X_BF16> : moe_combine_grad_kernel<MI_X_F32>;
+    hipLaunchKernelGGL(kern, dim3(T + rows), dim3(256), 0, (hipStream_t)stream, dout, y, row_slot, tok_row, w, T, k, D,
+                       rows, dy, dw);
+    return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
+}

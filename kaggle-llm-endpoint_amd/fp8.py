@@ -1,0 +1,253 @@
+"""Products over block-scaled fp8 weights: the layout of fp8 checkpoints (checkpoint.py:202), e4m3 values with one f32
+scale per 128 x 128 block, contracted as fp8 on the matrix cores with activations quantised per row and 128 columns.
+
+    q, s = fp8_quantize(x)                              rows of activations, once for several products
+    y    = fp8_project(x, leaf)                         a dense projection
+    y    = fp8_mlp(x, gate, up, down, limit)            mlp_partial's products (mlp_partial calls it for such leaves)
+    y    = fp8_grouped(xs, plan, leaf)                  the sorted rows of a ragged_plan, each times its expert's matrix
+    o, _ = fp8_moe(gate, up, down, x, idx, w, limit)    the routed experts of a layer
+
+Everything runs on the current torch (HIP) stream of the current device.  The weights are a checkpoint's and the
+products have no gradient: an input that requires one is refused while gradients are recorded.
+"""
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .resident import _as, _ptr, _stream
+
+BLOCK = 128                     # columns per activation scale; rows and columns per weight scale
+FP8 = torch.float8_e4m3fn
+
+
+def _blocks(n):
+    return -(-n // BLOCK)
+
+
+class Fp8Leaf(NamedTuple):
+    """Block-scaled weights on the device: q e4m3 [n_out, n_in] (or [E, n_out, n_in] of E experts), s f32
+    [..., ceil(n_out / 128), ceil(n_in / 128)]; a weight is f32(q) * s of its block."""
+    q: torch.Tensor
+    s: torch.Tensor
+
+
+def fp8_leaf(leaf, device="cuda"):
+    """{"q": float8_e4m3fn [..., n_out, n_in], "s": [..., ceil(n_out / 128), ceil(n_in / 128)]}, as a checkpoint stores
+    a matrix (or E of them) and its scales -> Fp8Leaf on the device."""
+    q, s = (leaf["q"], leaf["s"]) if isinstance(leaf, dict) else leaf
+    leaf = Fp8Leaf(q.to(device).contiguous(), s.to(device=device, dtype=torch.float32).contiguous())
+    _leaf_dims(leaf, "fp8_leaf")
+    return leaf
+
+
+def _leaf_dims(leaf, who):
+    """(E, n_out, n_in) of an Fp8Leaf, its types and shapes checked."""
+    q, s = leaf
+    if q.dtype != FP8 or s.dtype != torch.float32:
+        raise TypeError("%s: weights are float8_e4m3fn with float32 scales (got %s, %s)" % (who, q.dtype, s.dtype))
+    if q.dim() not in (2, 3) or s.dim() != q.dim():
+        raise ValueError("%s: weights are [n_out, n_in] or [E, n_out, n_in], scales likewise" % who)
+    R, K = q.shape[-2:]
+    if tuple(s.shape) != tuple(q.shape[:-2]) + (_blocks(R), _blocks(K)):
+        raise ValueError("%s: scales %s do not fit weights %s: one per 128 x 128 block" % (who, tuple(s.shape),
+                                                                                           tuple(q.shape)))
+    if not (q.is_contiguous() and s.is_contiguous()):
+        raise ValueError("%s: weights and scales must be contiguous (fp8_leaf makes them so)" % who)
+    return (q.shape[0] if q.dim() == 3 else 1), R, K
+
+
+def _one_device(who, *tensors):
+    """Every tensor on the current device: the call runs on that device's stream."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError("%s: every tensor must be on the current device (cuda:%d), got one on %s" % (who, dev,
+                                                                                                       t.device))
+
+
+def _no_grad(who, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("%s has no gradient: detach its inputs or call it under torch.no_grad()" % who)
+
+
+def _aligned(t):
+    """t contiguous, at a 16-byte address (a copy when it is not)."""
+    t = t if t.is_contiguous() else t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _out(t, shape, dtype, who, device):
+    """A caller's output checked, or a new one."""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError("%s: an output must be a contiguous %s tensor of shape %s" % (who, dtype, tuple(shape)))
+    return t
+
+
+def _workspace(workspace, need, who, device):
+    # without one, the call's own: a kept buffer would be shared by two captured calls
+    if need == 0:
+        raise ValueError("%s: unsupported shape" % who)
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace
+
+
+class _Rows(NamedTuple):
+    x: torch.Tensor
+    xs: object
+    dtype: int
+
+
+def _rows_of(x, K, who):
+    """Activations of a product: bf16 or f32 [B, K], or the pair (q, s) of fp8_quantize."""
+    if isinstance(x, (tuple, list)):
+        q, s = x
+        if q.dtype != FP8 or s.dtype != torch.float32:
+            raise TypeError("%s: quantised activations are (float8_e4m3fn, float32 scales)" % who)
+        if q.dim() != 2 or tuple(s.shape) != (q.shape[0], _blocks(q.shape[1])):
+            raise ValueError("%s: quantised activations are q [B, n_in] with s [B, ceil(n_in / 128)]" % who)
+        r = _Rows(_aligned(q), s.contiguous(), _lib.MI_X_FP8)
+    else:
+        if x.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError("%s: activations are bf16 or f32 (or fp8_quantize's pair), got %s" % (who, x.dtype))
+        if x.dim() != 2:
+            raise ValueError("%s: activations are [B, n_in]" % who)
+        _no_grad(who, x)
+        r = _Rows(_aligned(x), None, _lib.MI_X_BF16 if x.dtype == torch.bfloat16 else _lib.MI_X_F32)
+    if r.x.shape[1] != K:
+        raise ValueError("%s: activations have %d columns, the weight %d" % (who, r.x.shape[1], K))
+    return r
+
+
+def fp8_quantize(x, q=None, s=None):
+    """x bf16 or f32 [..., K], K a multiple of 16 -> (q float8_e4m3fn [..., K], s f32 [..., ceil(K / 128)]): per row and
+    group of 128 columns s = 2^e, the least e >= -100 with max |x| <= 448 * 2^e over the group's finite values, and
+    q = x / s to nearest even; infinities and NaN become NaN.  A power of two, so that x / s is exact and each value is
+    rounded once.  Rows may be strided.  ``q`` and ``s``: outputs to write into."""
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("fp8_quantize: x must be bf16 or f32, got %s" % x.dtype)
+    if x.dim() < 1:
+        raise ValueError("fp8_quantize: x must have at least one dimension")
+    _no_grad("fp8_quantize", x)
+    K = x.shape[-1]
+    q = _out(q, x.shape, FP8, "fp8_quantize", x.device)
+    s = _out(s, x.shape[:-1] + (_blocks(K),), torch.float32, "fp8_quantize", x.device)
+    if x.numel() == 0:
+        return q, s
+    _one_device("fp8_quantize", x, q, s)
+    n = x.numel() // K
+    x2 = x if x.dim() == 2 else x.reshape(n, K)
+    if x2.stride(1) != 1 or x2.stride(0) < K or x2.stride(0) % 8 or x2.data_ptr() % 16:
+        x2 = _aligned(x2)
+    check("mi_fp8_quantize", lib().mi_fp8_quantize(_ptr(x2), _lib.MI_X_BF16 if x.dtype == torch.bfloat16
+                                                   else _lib.MI_X_F32, n, K, x2.stride(0) if n > 1 else -(-K // 8) * 8,
+                                                   _ptr(q), _ptr(s), _stream()))
+    return q, s
+
+
+def fp8_project(x, leaf, want_f32=False, y_bf16=None, y_f32=None, workspace=None):
+    """y = x W^T over a block-scaled leaf (Fp8Leaf, [n_out, n_in], any n_out, n_in a multiple of 16): x bf16 or f32
+    [B, n_in], quantised as by fp8_quantize, or that function's pair.  Sums in f32, rounded once.  -> y bf16 [B, n_out]
+    (and y f32 with want_f32).  Preallocated outputs and ``workspace`` (uint8, mi_fp8_project_workspace bytes, needs no
+    initialisation) make the call allocation-free."""
+    E, R, K = _leaf_dims(leaf, "fp8_project")
+    if leaf.q.dim() != 2:
+        raise ValueError("fp8_project: the weight must be one matrix [n_out, n_in]")
+    r = _rows_of(x, K, "fp8_project")
+    B = r.x.shape[0]
+    yb = _out(y_bf16, (B, R), torch.bfloat16, "fp8_project", r.x.device)
+    yf = _out(y_f32, (B, R), torch.float32, "fp8_project", r.x.device) if want_f32 or y_f32 is not None else None
+    if B:
+        _one_device("fp8_project", r.x, r.xs, leaf.q, leaf.s, yb, yf, workspace)
+        ws = _workspace(workspace, lib().mi_fp8_project_workspace(B, K, R), "fp8_project", r.x.device)
+        check("mi_fp8_project", lib().mi_fp8_project(_ptr(r.x), r.dtype, _ptr(r.xs), B, _ptr(leaf.q), _ptr(leaf.s), K, R,
+                                                     _ptr(yb), _ptr(yf), _ptr(ws), ws.numel(), _stream()))
+    return (yb, yf) if want_f32 else yb
+
+
+def _mlp_dims(gate, up, down, who):
+    E, I, D = _leaf_dims(gate, who)
+    if _leaf_dims(up, who) != (E, I, D) or _leaf_dims(down, who) != (E, D, I):
+        raise ValueError("%s: gate and up must be [.., I, D] and down [.., D, I], got %s, %s, %s"
+                         % (who, tuple(gate.q.shape), tuple(up.q.shape), tuple(down.q.shape)))
+    return E, I, D
+
+
+def fp8_mlp(x, gate, up, down, limit, want_f32=False, y_bf16=None, y_f32=None, workspace=None):
+    """mlp_partial over block-scaled leaves (model.py:125-127): g, u = x Wg^T, x Wu^T in f32,
+    h = silu(min(g, limit)) * clip(u, -limit, limit), quantised as by fp8_quantize, y = h Wd^T.  x as for fp8_project;
+    gate, up [I, D], down [D, I].  -> y bf16 [B, D] (and y f32 with want_f32).  Preallocated outputs and ``workspace``
+    (mi_fp8_mlp_workspace bytes) make the call allocation-free."""
+    E, I, D = _mlp_dims(gate, up, down, "fp8_mlp")
+    if gate.q.dim() != 2:
+        raise ValueError("fp8_mlp: gate, up and down are one matrix each")
+    r = _rows_of(x, D, "fp8_mlp")
+    B = r.x.shape[0]
+    yb = _out(y_bf16, (B, D), torch.bfloat16, "fp8_mlp", r.x.device)
+    yf = _out(y_f32, (B, D), torch.float32, "fp8_mlp", r.x.device) if want_f32 or y_f32 is not None else None
+    if B:
+        _one_device("fp8_mlp", r.x, r.xs, *gate, *up, *down, yb, yf, workspace)
+        ws = _workspace(workspace, lib().mi_fp8_mlp_workspace(B, D, I), "fp8_mlp", r.x.device)
+        check("mi_fp8_mlp", lib().mi_fp8_mlp(_ptr(r.x), r.dtype, _ptr(r.xs), B, D, I, _ptr(gate.q), _ptr(gate.s),
+                                             _ptr(up.q), _ptr(up.s), _ptr(down.q), _ptr(down.s), float(limit), _ptr(yb),
+                                             _ptr(yf), _ptr(ws), ws.numel(), _stream()))
+    return (yb, yf) if want_f32 else yb
+
+
+def fp8_grouped(xs, plan, leaf, want_f32=False, y_bf16=None, y_f32=None, workspace=None):
+    """The sorted rows of a ragged_plan (tm 16, 32, 64 or 128), each times its expert's matrix of ``leaf`` [E, R, K]: xs
+    bf16 or f32 [Rp, K] (moe_dispatch's rows) or fp8_quantize's pair -> y bf16 [Rp, R] (and y f32 with want_f32), ready
+    for moe_combine.  Rows of blocks that the plan does not use are zero."""
+    E, R, K = _leaf_dims(leaf, "fp8_grouped")
+    if leaf.q.dim() != 3:
+        raise ValueError("fp8_grouped: the weights must be [E, R, K]")
+    r = _rows_of(xs, K, "fp8_grouped")
+    blk, nb = _as(plan["blk_expert"], torch.int32), _as(plan["n_blocks"], torch.int32)
+    rows, G = r.x.shape[0], blk.numel()
+    if rows != plan["tok_row"].numel() or nb.numel() != 1 or G == 0 or rows % G:
+        raise ValueError("fp8_grouped: %d rows do not fit the plan's %d rows in %d blocks" % (rows, plan["tok_row"].numel(),
+                                                                                             G))
+    yb = _out(y_bf16, (rows, R), torch.bfloat16, "fp8_grouped", r.x.device)
+    yf = _out(y_f32, (rows, R), torch.float32, "fp8_grouped", r.x.device) if want_f32 or y_f32 is not None else None
+    _one_device("fp8_grouped", r.x, r.xs, blk, nb, leaf.q, leaf.s, yb, yf, workspace)
+    ws = _workspace(workspace, lib().mi_fp8_grouped_workspace(rows, K, R), "fp8_grouped", r.x.device)
+    check("mi_fp8_grouped", lib().mi_fp8_grouped(_ptr(r.x), r.dtype, _ptr(r.xs), G, rows // G, _ptr(blk), _ptr(nb),
+                                                 _ptr(leaf.q), _ptr(leaf.s), E, K, R, _ptr(yb), _ptr(yf), _ptr(ws),
+                                                 ws.numel(), _stream()))
+    return (yb, yf) if want_f32 else yb
+
+
+def fp8_moe(gate, up, down, x, idx, w, limit, want_f32=True, want_bf16=False, out_f32=None, out_bf16=None,
+            workspace=None):
+    """The routed experts of one layer over block-scaled weights, for one token or a whole prompt piece: out[t] =
+    sum_j w[t, j] * MLP_{idx[t, j]}(x[t]) with the MLP of fp8_mlp, everything between its quantisations and the output in
+    f32.  gate, up [E, I, D], down [E, D, I] (Fp8Leaf); x bf16 or f32 [T, D]; idx int32 [T, k]; w f32 [T, k] ->
+    (out_f32 [T, D] or None, out_bf16 [T, D] or None).  A slot whose expert id is outside [0, E) adds nothing.
+    Preallocated outputs and ``workspace`` (mi_fp8_moe_workspace bytes) make the call allocation-free."""
+    E, I, D = _mlp_dims(gate, up, down, "fp8_moe")
+    if gate.q.dim() != 3:
+        raise ValueError("fp8_moe: gate, up and down must be [E, ..] experts")
+    if isinstance(x, (tuple, list)):
+        raise TypeError("fp8_moe: activations are bf16 or f32")
+    r = _rows_of(x, D, "fp8_moe")
+    if idx.dim() != 2 or w.shape != idx.shape or idx.shape[0] != r.x.shape[0]:
+        raise ValueError("fp8_moe: idx and w must be [T, k] for the %d tokens of x" % r.x.shape[0])
+    _no_grad("fp8_moe", w)
+    idx, w = _as(idx, torch.int32), _as(w, torch.float32)
+    T, k = idx.shape
+    of, ob = out_f32, out_bf16
+    if of is not None or want_f32:
+        of = _out(of, (T, D), torch.float32, "fp8_moe", r.x.device)
+    if ob is not None or want_bf16:
+        ob = _out(ob, (T, D), torch.bfloat16, "fp8_moe", r.x.device)
+    if T:
+        _one_device("fp8_moe", r.x, idx, w, *gate, *up, *down, of, ob, workspace)
+        ws = _workspace(workspace, lib().mi_fp8_moe_workspace(T, k, E, D, I), "fp8_moe", r.x.device)
+        check("mi_fp8_moe", lib().mi_fp8_moe(_ptr(gate.q), _ptr(gate.s), _ptr(up.q), _ptr(up.s), _ptr(down.q),
+                                             _ptr(down.s), E, D, I, _ptr(r.x), r.dtype, T, k, _ptr(idx), _ptr(w),
+                                             float(limit), _ptr(of), _ptr(ob), _ptr(ws), ws.numel(), _stream()))
+    return of, ob

@@ -765,8 +765,16 @@ def bf16_mlp(x, gate, up, down, limit, want_f32=False, y_bf16=None, y_f32=None, 
 def mlp_partial(p, x, limit):
     """The reference's mlp_partial(p, x, cfg) (model.py:125-127) for p = {"gate", "up", "down"}: int8 leaves
     {"q", "s"} (quant8.py:17-18, int8_nonexpert on) or int8_leaf triples go to int8_mlp; bf16 leaves (W [in, out]
-    torch.bfloat16, the engine's default, engine.py:281) or Bf16Leaf to bf16_mlp.  x bf16 [B, D] -> bf16 [B, D]
-    (cfg.swiglu_limit passed as ``limit``)."""
+    torch.bfloat16, the engine's default, engine.py:281) or Bf16Leaf to bf16_mlp; block-scaled fp8 leaves (fp8.Fp8Leaf,
+    or {"q", "s"} with q float8_e4m3fn [out, in]) to fp8_mlp.  x bf16 [B, D] -> bf16 [B, D] (cfg.swiglu_limit passed as
+    ``limit``)."""
+    leaves = [p[k] for k in ("gate", "up", "down")]
+    is_fp8 = [isinstance(l, fp8.Fp8Leaf) or (isinstance(l, dict) and getattr(l["q"], "dtype", None) == fp8.FP8)
+              for l in leaves]
+    if any(is_fp8):
+        if not all(is_fp8):
+            raise ValueError("mlp_partial: gate, up and down must be all int8, all bf16 or all fp8 leaves")
+        return fp8.fp8_mlp(x, *[l if isinstance(l, fp8.Fp8Leaf) else fp8.fp8_leaf(l, x.device) for l in leaves], limit)
     kinds = {"int8" if isinstance(p[k], (dict, tuple)) and not isinstance(p[k], Bf16Leaf) else "bf16"
              for k in ("gate", "up", "down")}
     if len(kinds) != 1:
@@ -875,3 +883,6 @@ class ResidentFetch:
         form = {"ragged": self.combine, "sweep": "sweep", "gather": "xla_gather", "sweep_xla": "xla_sweep"}[br]
         out, _ = moe_prefill(gate, up, down, x.to(torch.bfloat16), idx, w, limit, combine=form, chunk=self.chunk)
         return out
+
+
+from . import fp8  # noqa: E402  (mlp_partial's fp8 leaves; fp8 uses the helpers above)

@@ -1,0 +1,105 @@
+"""Tokens into expert order and back over the layout of ``ragged_plan`` (pallas_moe.py:564-592), the gather and the
+combine around the ragged products (resident.py:153-165), with their gradients:
+
+    plan = ragged_plan(idx, w, E, tm)
+    xs   = moe_dispatch(x, plan)            [Rp, D]; the experts' products of xs give y [Rp, D]
+    out  = moe_combine(y, plan, w)          [T, D]
+
+Both record gradients (x; y and w), first order only, and save no copies: the rows a backward pass reads are the
+forward's own inputs.  Deterministic: no atomics, sums in f32 in column order, one rounding.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import check, lib
+from .fp8 import _aligned, _one_device
+from .resident import _as, _ptr, _stream
+
+_DTYPES = {torch.bfloat16: _lib.MI_X_BF16, torch.float32: _lib.MI_X_F32}
+
+
+def _rows_dtype(t, who):
+    if t.dtype not in _DTYPES:
+        raise TypeError("%s: rows are bf16 or f32, got %s" % (who, t.dtype))
+    if t.dim() != 2:
+        raise ValueError("%s: rows are [n, D]" % who)
+    return _DTYPES[t.dtype]
+
+
+def _plan_rows(plan):
+    """(tok_row [Rp], row_slot [T, k]) of a plan, contiguous int32."""
+    tok, slot = _as(plan["tok_row"], torch.int32), _as(plan["row_slot"], torch.int32)
+    if tok.dim() != 1 or slot.dim() != 2:
+        raise ValueError("a plan holds tok_row [Rp] and row_slot [T, k]")
+    return tok, slot
+
+
+def _combine(y, slot, w, who):
+    T, k = slot.shape
+    out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
+    check("mi_moe_combine", lib().mi_moe_combine(_ptr(y), _DTYPES[y.dtype], T, k, y.shape[1], _ptr(slot), _ptr(w),
+                                                 y.shape[0], _ptr(out), _stream()))
+    return out
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, tok, slot):
+        ctx.save_for_backward(slot)
+        xs = torch.empty((tok.numel(), x.shape[1]), dtype=x.dtype, device=x.device)
+        T, k = slot.shape
+        check("mi_moe_dispatch", lib().mi_moe_dispatch(_ptr(x), _DTYPES[x.dtype], T, k, x.shape[1], _ptr(slot), _ptr(tok),
+                                                       tok.numel(), _ptr(xs), _stream()))
+        return xs
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gxs):
+        slot, = ctx.saved_tensors
+        return _combine(_aligned(gxs), slot, None, "moe_dispatch"), None, None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, w, tok, slot):
+        ctx.save_for_backward(y, w, tok, slot)
+        return _combine(y, slot, w, "moe_combine")
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gout):
+        y, w, tok, slot = ctx.saved_tensors
+        gout = _aligned(gout)
+        T, k = slot.shape
+        dy, dw = torch.empty_like(y), torch.empty_like(w)
+        check("mi_moe_combine_grad",
+              lib().mi_moe_combine_grad(_ptr(gout), _ptr(y), _DTYPES[y.dtype], T, k, y.shape[1], _ptr(slot), _ptr(tok),
+                                        _ptr(w), y.shape[0], _ptr(dy), _ptr(dw), _stream()))
+        return dy, dw, None, None
+
+
+def moe_dispatch(x, plan):
+    """Tokens into expert order: x bf16 or f32 [T, D] (D a multiple of 8), plan = ragged_plan(idx, w, E, tm) ->
+    xs [Rp, D] of x's dtype, xs[r] = x[tok_row[r]], zeros on padding rows.  Records the gradient of x: the sum over a
+    token's rows."""
+    _rows_dtype(x, "moe_dispatch")
+    tok, slot = _plan_rows(plan)
+    if slot.shape[0] != x.shape[0]:
+        raise ValueError("moe_dispatch: the plan is of %d tokens, x has %d" % (slot.shape[0], x.shape[0]))
+    _one_device("moe_dispatch", x, tok, slot)
+    return _Dispatch.apply(_aligned(x), tok, slot)
+
+
+def moe_combine(y, plan, w):
+    """The way back: y bf16 or f32 [Rp, D] in the plan's row order, w f32 [T, k] -> out [T, D] of y's dtype, out[t] =
+    sum_j w[t, j] * y[row_slot[t, j]] in f32, in column order, rounded once; a slot without a row (an expert id outside
+    [0, E)) adds nothing.  Records the gradients of y (zeros on padding rows) and w."""
+    _rows_dtype(y, "moe_combine")
+    tok, slot = _plan_rows(plan)
+    if tok.numel() != y.shape[0]:
+        raise ValueError("moe_combine: the plan has %d rows, y %d" % (tok.numel(), y.shape[0]))
+    if w.dtype != torch.float32 or w.shape != slot.shape:
+        raise ValueError("moe_combine: w must be float32 %s" % (tuple(slot.shape),))
+    _one_device("moe_combine", y, w, tok, slot)
+    return _Combine.apply(_aligned(y), w.contiguous(), tok, slot)
