@@ -2,7 +2,9 @@
 // over sorted rows and the whole routed layer.
 #include <algorithm>
 
-#include "fp8.h"
+#include "fp8_gemm.h"
+#include "fp8_stream.h"
+#include "tuning.h"
 
 namespace mi {
 
@@ -60,15 +62,22 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const void *__restric
     if ((threadIdx.x & 15) == 0) s[(size_t)row * KB + c] = exp2_int(e);
 }
 
-// h = silu(min(g, L)) * clip(u, -L, L) in f32, quantised as above: one wavefront per row and group, two values a lane.
-__global__ void __launch_bounds__(64) fp8_swiglu_kernel(const float *__restrict__ g, const float *__restrict__ u,
-                                                        int I, float limit, uint8_t *__restrict__ q,
+// The split sums of gate and up added in split order, then h = silu(min(g, L)) * clip(u, -L, L) in f32, quantised as
+// above: one wavefront per row and group, two values a lane.
+__global__ void __launch_bounds__(64) fp8_swiglu_kernel(const float *__restrict__ g, const float *__restrict__ u, int S,
+                                                        int rows, int I, float limit, uint8_t *__restrict__ q,
                                                         float *__restrict__ s) {
     const int row = blockIdx.x, c = blockIdx.y, lane = threadIdx.x;
     const int col = c * kFp8Group + 2 * lane;
     float h0 = 0.0f, h1 = 0.0f;
     if (col < I) {
-        const float2 gv = *(const float2 *)(g + (size_t)row * I + col), uv = *(const float2 *)(u + (size_t)row * I + col);
+        float2 gv = {0.f, 0.f}, uv = {0.f, 0.f};
+        for (int k = 0; k < S; ++k) {
+            const size_t at = ((size_t)k * rows + row) * I + col;
+            const float2 a = *(const float2 *)(g + at), b = *(const float2 *)(u + at);
+            gv.x += a.x, gv.y += a.y;
+            uv.x += b.x, uv.y += b.y;
+        }
         h0 = fp8_swiglu(gv.x, uv.x, limit);
         h1 = fp8_swiglu(gv.y, uv.y, limit);
     }
@@ -84,70 +93,42 @@ __global__ void __launch_bounds__(64) fp8_swiglu_kernel(const float *__restrict_
     if (lane == 0) s[(size_t)row * fp8_groups(I) + c] = exp2_int(e);
 }
 
-// ------------------------------------------------------------------------------------------------ the product
-// One wavefront per 16 output columns x 16 rows.
-__global__ void __launch_bounds__(64) fp8_tile_kernel(Fp8Gemm a) {
-    const int lane = threadIdx.x, i = lane & 15, q = lane >> 4;
-    const int o0 = blockIdx.y * 16, r0 = blockIdx.x * 16;
-    const int KB = fp8_groups(a.K), RB = fp8_groups(a.R);
-    int e = 0;
-    bool live = true;
-    if (a.blk_expert) {
-        const int blk = r0 / a.tm;
-        e = a.blk_expert[blk];
-        live = blk < *a.n_blocks && e >= 0 && e < a.E;
-        if (!live) e = 0;
-    }
-    const int row = r0 + i;
-    int tok = row < a.rows ? (a.tok_row ? a.tok_row[row] : row) : -1;
-    if (tok >= a.x_rows) tok = -1;
-    const int o = min(o0 + i, a.R - 1);
-    const uint8_t *w = a.wq[0] + ((size_t)e * a.R + o) * a.K;
-    const float *ws = a.ws[0] + ((size_t)e * RB + o0 / kFp8Group) * KB;
-    const uint8_t *x = a.xq + (size_t)max(tok, 0) * a.K;
-    const float *xs = a.xs + (size_t)max(tok, 0) * KB;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    if (live) {
-        for (int g = 0; g < KB; ++g) {
-            uint4 wf[2] = {}, xf[2] = {};
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int col = g * kFp8Group + 16 * (q + 4 * c);
-                if (col < a.K) {
-                    wf[c] = *(const uint4 *)(w + col);
-                    if (tok >= 0) xf[c] = *(const uint4 *)(x + col);
-                }
-            }
-            const i32x8 wv = {(int)wf[0].x, (int)wf[0].y, (int)wf[0].z, (int)wf[0].w,
-                              (int)wf[1].x, (int)wf[1].y, (int)wf[1].z, (int)wf[1].w};
-            const i32x8 xv = {(int)xf[0].x, (int)xf[0].y, (int)xf[0].z, (int)xf[0].w,
-                              (int)xf[1].x, (int)xf[1].y, (int)xf[1].z, (int)xf[1].w};
-            const f32x4 p = fp8_mfma(wv, xv);
-            const float sc = (tok >= 0 ? xs[g] : 0.0f) * ws[g];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j] = fmaf(p[j], sc, acc[j]);
-        }
-    }
-    if (row >= a.rows) return;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int oo = o0 + 4 * q + j;
-        if (oo >= a.R) break;
-        if (a.y_f32) a.y_f32[(size_t)row * a.R + oo] = acc[j];
-        if (a.y_bf16) a.y_bf16[(size_t)row * a.R + oo] = (uint16_t)f32_to_bf16_rne(acc[j]);
+// The split sums of a product, added in split order.
+__global__ void __launch_bounds__(256) fp8_reduce_kernel(const float *__restrict__ part, int S, long long n,
+                                                         uint16_t *y_bf16, float *y_f32) {
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= n) return;
+    float v = part[at];
+    for (int k = 1; k < S; ++k) v += part[k * n + at];
+    if (y_f32) y_f32[at] = v;
+    if (y_bf16) y_bf16[at] = (uint16_t)f32_to_bf16_rne(v);
+}
+
+// Zeros for the rows of blocks that have no product.
+__global__ void __launch_bounds__(256) fp8_zero_blocks_kernel(const int32_t *__restrict__ blk_expert,
+                                                              const int32_t *__restrict__ n_blocks, int E, int tm, int R,
+                                                              uint16_t *y_bf16, float *y_f32) {
+    const int g = blockIdx.x, e = blk_expert[g];
+    if (g < *n_blocks && e >= 0 && e < E) return;
+    const long long n = (long long)tm * R;
+    for (long long at = (long long)blockIdx.y * 256 + threadIdx.x; at < n; at += (long long)gridDim.y * 256) {
+        if (y_f32) y_f32[g * n + at] = 0.0f;
+        if (y_bf16) y_bf16[g * n + at] = 0;
     }
 }
 
-// out[t] = sum_j w[t, j] * y[row_slot[t, j]], f32, in column order.
+// out[t] = sum_j w[t, j] * y[r(t, j)], f32, in column order: r the slot's sorted row, or (row_slot NULL) the slot itself.
 __global__ void __launch_bounds__(256) fp8_combine_kernel(const float *__restrict__ y, const int32_t *__restrict__ row_slot,
-                                                          const float *__restrict__ w, int T, int k, int D,
-                                                          float *out_f32, uint16_t *out_bf16) {
+                                                          const int32_t *__restrict__ idx, int E,
+                                                          const float *__restrict__ w, int k, int D, float *out_f32,
+                                                          uint16_t *out_bf16) {
     const int t = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;
     if (c >= D) return;
     float acc = 0.0f;
     for (int j = 0; j < k; ++j) {
-        const int r = row_slot[(size_t)t * k + j];
-        if (r >= 0) acc = fmaf(w[(size_t)t * k + j], y[(size_t)r * D + c], acc);
+        const int s = t * k + j, e = idx[s];
+        const int r = e < 0 || e >= E ? -1 : row_slot ? row_slot[s] : s;
+        if (r >= 0) acc = fmaf(w[s], y[(size_t)r * D + c], acc);
     }
     if (out_f32) out_f32[(size_t)t * D + c] = acc;
     if (out_bf16) out_bf16[(size_t)t * D + c] = (uint16_t)f32_to_bf16_rne(acc);
@@ -156,7 +137,6 @@ __global__ void __launch_bounds__(256) fp8_combine_kernel(const float *__restric
 // ------------------------------------------------------------------------------------------------ host side
 constexpr int kFp8MaxCols = 1 << 17;             // K, R: 32-bit offsets within a tile of 256 rows
 constexpr int kFp8MaxRows = 1 << 22;             // rows of activations
-constexpr int kFp8MoeTm = 16;
 
 static bool fp8_cols_ok(int K) { return K > 0 && K % 16 == 0 && K <= kFp8MaxCols; }
 static bool fp8_rows_ok(int R) { return R > 0 && R <= kFp8MaxCols; }
@@ -179,15 +159,120 @@ static int fp8_launch_quantize(const void *x, int x_dtype, int n, int K, long lo
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }
 
-static int fp8_launch_gemm(const Fp8Gemm &a, hipStream_t st) {
-    hipLaunchKernelGGL(fp8_tile_kernel, dim3((a.rows + 15) / 16, (a.R + 15) / 16), dim3(64), 0, st, a);
+// ---- the tiled product.  Tiles: 256 weight rows (128 where a dense product has few tiles) x tt tokens.
+template <int TW, int TT, int WM, int WN, int NST, bool PAIR>
+static int fp8_launch_tiled(Fp8Tiled p, hipStream_t st) {
+    p.nw = (p.g.R + (PAIR ? TW / 2 : TW) - 1) / (PAIR ? TW / 2 : TW);
+    p.nb = (p.g.rows + TT - 1) / TT;
+    // ids equal modulo 8 share an XCD and a piece of at most ceil(total / 8) workgroups
+    const long long total = (long long)p.nb * p.nw * p.S, grid = (total + 7) / 8 * 8;
+    if (grid >= (1ll << 31) / (64 * WM * WN)) return MI_ERR_TOKENS;
+    hipLaunchKernelGGL((fp8_gemm_kernel<TW, TT, WM, WN, NST, PAIR>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, p);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }
 
-static int fp8_launch_swiglu(const float *g, const float *u, int rows, int I, float limit, uint8_t *q, float *s,
-                             hipStream_t st) {
-    hipLaunchKernelGGL(fp8_swiglu_kernel, dim3(rows, fp8_groups(I)), dim3(64), 0, st, g, u, I, limit, q, s);
+template <bool PAIR>
+static int fp8_tiled(const Fp8Tiled &p, int tw, int tt, hipStream_t st) {
+    if constexpr (!PAIR) {
+        if (tw == 128) return tt == 64 ? fp8_launch_tiled<128, 64, 2, 2, 4, false>(p, st)
+                                       : fp8_launch_tiled<128, 128, 2, 2, 4, false>(p, st);
+    }
+    switch (tt) {
+        case 16: return fp8_launch_tiled<256, 16, 4, 1, 4, PAIR>(p, st);
+        case 32: return fp8_launch_tiled<256, 32, 4, 1, 4, PAIR>(p, st);
+        case 64: return fp8_launch_tiled<256, 64, 4, 1, 3, PAIR>(p, st);
+        case 128: return fp8_launch_tiled<256, 128, 2, 2, 3, PAIR>(p, st);
+        default: return fp8_launch_tiled<256, 256, 2, 4, 2, PAIR>(p, st);
+    }
+}
+
+// The tiles and splits of a dense product of B rows: the largest tiles that still give every CU one, splits of K where
+// even the smallest leave CUs idle (each at least 4 groups of columns).
+struct Fp8Plan {
+    int tw, tt, S;
+};
+constexpr int kFp8Cus = 256;
+constexpr int kFp8SplitTiles = 512;              // tiles x splits at most
+
+// Floats of split sums that any B up to the given one may need: S * tiles <= kFp8SplitTiles, so S * B * R is within
+// kFp8SplitTiles tiles whatever B is.
+static size_t fp8_split_floats(int R, bool pair) {
+    const size_t n = (size_t)(R + 127) / 128;    // tiles of 128 outputs per token tile
+    return std::max<size_t>(kFp8SplitTiles / n, 1) * 64 * R * (pair ? 2 : 1);
+}
+
+// A token tile that the tiled kernels have.
+static int fp8_tile_of(int tt) { return tt <= 16 ? 16 : tt <= 32 ? 32 : tt <= 64 ? 64 : tt <= 128 ? 128 : 256; }
+
+static Fp8Plan fp8_plan(int B, int R, int K, bool pair) {
+    auto tiles = [&](int tw, int tt) {
+        const int w = pair ? tw / 2 : tw;
+        return (long long)((R + w - 1) / w) * ((B + tt - 1) / tt);
+    };
+    Fp8Plan p{256, 64, 1};
+    if (tiles(256, 256) >= kFp8Cus) p.tt = 256;
+    else if (tiles(256, 128) >= kFp8Cus) p.tt = 128;
+    else if (pair) p.tt = B <= 32 ? 32 : 64;
+    else p.tw = 128, p.tt = B > 64 && tiles(128, 128) >= kFp8Cus ? 128 : 64;
+    p.tw = !pair && tuning(kTuneF8Tw, p.tw) == 128 ? 128 : 256;
+    p.tt = fp8_tile_of(tuning(kTuneF8Tt, p.tt));
+    if (p.tw == 128) p.tt = std::min(std::max(p.tt, 64), 128);
+    const long long n = tiles(p.tw, p.tt);
+    if (n < kFp8Cus) p.S = (int)std::max(1ll, std::min<long long>(kFp8SplitTiles / n, fp8_groups(K) / 4));
+    p.S = std::max(1, std::min(tuning(kTuneF8S, p.S), fp8_groups(K)));
+    if ((size_t)p.S * B * R * (pair ? 2 : 1) > fp8_split_floats(R, pair)) p.S = 1;
+    return p;
+}
+
+static int fp8_launch_dense(Fp8Gemm a, float *part, hipStream_t st) {
+    const Fp8Plan pl = fp8_plan(a.rows, a.R, a.K, false);
+    Fp8Tiled p = {};
+    p.g = a;
+    p.S = pl.S;
+    p.part[0] = part;
+    int rc = fp8_tiled<false>(p, pl.tw, pl.tt, st);
+    if (rc != MI_OK || pl.S == 1) return rc;
+    const long long n = (long long)a.rows * a.R;
+    hipLaunchKernelGGL(fp8_reduce_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, pl.S, n, a.y_bf16,
+                       a.y_f32);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
+}
+
+// gate and up of a dense MLP -> h as e4m3 rows.
+static int fp8_launch_dense_pair(Fp8Gemm a, float limit, uint8_t *hq, float *hs, float *part, hipStream_t st) {
+    const Fp8Plan pl = fp8_plan(a.rows, a.R, a.K, true);
+    Fp8Tiled p = {};
+    p.g = a;
+    p.S = pl.S;
+    p.limit = limit, p.hq = hq, p.hs = hs;
+    p.part[0] = part, p.part[1] = part + (size_t)pl.S * a.rows * a.R;
+    int rc = fp8_tiled<true>(p, 256, pl.tt, st);
+    if (rc != MI_OK || pl.S == 1) return rc;
+    hipLaunchKernelGGL(fp8_swiglu_kernel, dim3(a.rows, fp8_groups(a.R)), dim3(64), 0, st, p.part[0], p.part[1], pl.S,
+                       a.rows, a.R, limit, hq, hs);
+    return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
+}
+
+// ---- the streaming product
+constexpr int kFp8StreamRows = 32;               // rows that the dense streaming kernels take
+
+template <int XD, int NT, int RW, bool PAIR, bool SLOTS, int U, int OCC>
+static int fp8_launch_stream_as(const Fp8Stream &a, hipStream_t st) {
+    const dim3 grid((a.R + 16 * RW - 1) / (16 * RW), SLOTS ? a.rows : 1);
+    hipLaunchKernelGGL((fp8_stream_kernel<XD, NT, RW, PAIR, SLOTS, U, OCC>), grid, dim3(64 * kFp8StreamWaves), 0, st, a);
+    return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
+}
+
+template <int XD, bool PAIR>
+static int fp8_stream_dense_as(const Fp8Stream &a, hipStream_t st) {
+    if (a.rows > 16) return fp8_launch_stream_as<XD, 2, 1, PAIR, false, 2, 2>(a, st);
+    return fp8_launch_stream_as<XD, 1, 1, PAIR, false, XD == MI_X_F32 ? 2 : 3, PAIR || XD == MI_X_F32 ? 2 : 4>(a, st);
+}
+
+template <bool PAIR>
+static int fp8_stream_dense(const Fp8Stream &a, int xd, hipStream_t st) {
+    return xd == MI_X_BF16 ? fp8_stream_dense_as<MI_X_BF16, PAIR>(a, st)
+         : xd == MI_X_F32 ? fp8_stream_dense_as<MI_X_F32, PAIR>(a, st) : fp8_stream_dense_as<MI_X_FP8, PAIR>(a, st);
 }
 
 // A workspace cut into pieces of whole 256 bytes.
@@ -254,7 +339,8 @@ extern "C" int mi_fp8_quantize(const void *x, int32_t x_dtype, int32_t n, int32_
 extern "C" size_t mi_fp8_project_workspace(int32_t B, int32_t n_in, int32_t n_out) {
     if (B <= 0 || B > kFp8MaxRows || !fp8_cols_ok(n_in) || !fp8_rows_ok(n_out) || (long long)B * n_in >= (1ll << 31))
         return 0;
-    return fp8_row_bytes(B, n_in);
+    // (the streaming kernels need none; 256 bytes keep an allocation from being empty)
+    return B <= kFp8StreamRows ? 256 : fp8_row_bytes(B, n_in) + up256(fp8_split_floats(n_out, false) * sizeof(float));
 }
 
 extern "C" int mi_fp8_project(const void *x, int32_t x_dtype, const float *xs, int32_t B, const uint8_t *wq,
@@ -268,6 +354,15 @@ extern "C" int mi_fp8_project(const void *x, int32_t x_dtype, const float *xs, i
     if (!workspace || workspace_bytes < mi_fp8_project_workspace(B, n_in, n_out)) return MI_ERR_WORKSPACE;
     if (!aligned16(workspace)) return MI_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
+    if (B <= kFp8StreamRows) {
+        Fp8Stream f = {};
+        f.x = x, f.xs = xs;
+        f.wq[0] = wq, f.ws[0] = ws;
+        f.rows = B;
+        f.E = 1, f.R = n_out, f.K = n_in;
+        f.y_bf16 = y_bf16, f.y_f32 = y_f32;
+        return fp8_stream_dense<false>(f, x_dtype, st);
+    }
     Fp8Cut c{(uint8_t *)workspace};
     Fp8Gemm a = {};
     rc = fp8_rows_of(x, x_dtype, xs, B, n_in, c, a, st);
@@ -276,13 +371,16 @@ extern "C" int mi_fp8_project(const void *x, int32_t x_dtype, const float *xs, i
     a.x_rows = a.rows = B;
     a.E = 1, a.R = n_out, a.K = n_in;
     a.y_bf16 = y_bf16, a.y_f32 = y_f32;
-    return fp8_launch_gemm(a, st);
+    return fp8_launch_dense(a, c.take<float>(fp8_split_floats(n_out, false)), st);
 }
 
 extern "C" size_t mi_fp8_mlp_workspace(int32_t B, int32_t D, int32_t I) {
     if (B <= 0 || B > kFp8MaxRows || !fp8_cols_ok(D) || !fp8_cols_ok(I) || (long long)B * std::max(D, I) >= (1ll << 31))
         return 0;
-    return fp8_row_bytes(B, D) + fp8_row_bytes(B, I) + 2 * up256((size_t)B * I * sizeof(float));
+    const size_t few = up256((size_t)std::min(B, kFp8StreamRows) * I * sizeof(float));
+    if (B <= kFp8StreamRows) return few;
+    return std::max(few, fp8_row_bytes(B, D) + fp8_row_bytes(B, I) +
+                             up256(std::max(fp8_split_floats(I, true), fp8_split_floats(D, false)) * sizeof(float)));
 }
 
 extern "C" int mi_fp8_mlp(const void *x, int32_t x_dtype, const float *xs, int32_t B, int32_t D, int32_t I,
@@ -301,23 +399,36 @@ extern "C" int mi_fp8_mlp(const void *x, int32_t x_dtype, const float *xs, int32
     if (!aligned16(workspace)) return MI_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
     Fp8Cut c{(uint8_t *)workspace};
+    if (B <= kFp8StreamRows) {
+        float *h = c.take<float>((size_t)B * I);
+        Fp8Stream f = {};
+        f.x = x, f.xs = xs;
+        f.wq[0] = gate_q, f.ws[0] = gate_s, f.wq[1] = up_q, f.ws[1] = up_s;
+        f.rows = B;
+        f.E = 1, f.R = I, f.K = D;
+        f.limit = limit;
+        f.y_f32 = h;
+        if ((rc = fp8_stream_dense<true>(f, x_dtype, st)) != MI_OK) return rc;
+        f.x = h, f.xs = nullptr;
+        f.wq[0] = down_q, f.ws[0] = down_s;
+        f.R = D, f.K = I;
+        f.y_bf16 = y_bf16, f.y_f32 = y_f32;
+        return fp8_stream_dense<false>(f, MI_X_F32, st);
+    }
     Fp8Gemm a = {};
     rc = fp8_rows_of(x, x_dtype, xs, B, D, c, a, st);
     if (rc != MI_OK) return rc;
-    float *g = c.take<float>((size_t)B * I), *u = c.take<float>((size_t)B * I);
     uint8_t *hq = c.take<uint8_t>((size_t)B * I);
     float *hs = c.take<float>((size_t)B * fp8_groups(I));
+    float *part = c.take<float>(std::max(fp8_split_floats(I, true), fp8_split_floats(D, false)));
     a.x_rows = a.rows = B;
     a.E = 1, a.R = I, a.K = D;
-    a.wq[0] = gate_q, a.ws[0] = gate_s, a.y_f32 = g;
-    if ((rc = fp8_launch_gemm(a, st)) != MI_OK) return rc;
-    a.wq[0] = up_q, a.ws[0] = up_s, a.y_f32 = u;
-    if ((rc = fp8_launch_gemm(a, st)) != MI_OK) return rc;
-    if ((rc = fp8_launch_swiglu(g, u, B, I, limit, hq, hs, st)) != MI_OK) return rc;
+    a.wq[0] = gate_q, a.ws[0] = gate_s, a.wq[1] = up_q, a.ws[1] = up_s;
+    if ((rc = fp8_launch_dense_pair(a, limit, hq, hs, part, st)) != MI_OK) return rc;
     a.xq = hq, a.xs = hs;
     a.R = D, a.K = I;
     a.wq[0] = down_q, a.ws[0] = down_s, a.y_bf16 = y_bf16, a.y_f32 = y_f32;
-    return fp8_launch_gemm(a, st);
+    return fp8_launch_dense(a, part, st);
 }
 
 extern "C" size_t mi_fp8_grouped_workspace(int32_t rows, int32_t K, int32_t R) {
@@ -351,24 +462,48 @@ extern "C" int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, i
     a.tm = tm;
     a.E = E, a.R = R, a.K = K;
     a.y_bf16 = y_bf16, a.y_f32 = y_f32;
-    return fp8_launch_gemm(a, st);
+    Fp8Tiled p = {};
+    p.g = a;
+    p.S = 1;
+    if ((rc = fp8_tiled<false>(p, 256, tm, st)) != MI_OK) return rc;
+    hipLaunchKernelGGL(fp8_zero_blocks_kernel, dim3(n_blk, 8), dim3(256), 0, st, blk_expert, n_blocks, E, tm, R, y_bf16,
+                       y_f32);
+    return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }
 
 namespace mi {
 
+// A call of at most MI_MAX_SLOTS slots whose experts are mostly distinct streams the experts' weights per slot; a larger
+// one sorts its slots by expert and takes the tiled product, its token tile the smaller the fewer rows an expert has.
+static bool fp8_moe_streams(int S) { return S <= std::min(tuning(kTuneF8Stream, MI_MAX_SLOTS), MI_MAX_SLOTS); }
+static int fp8_moe_tile(int S, int E) {
+    const int per = S / E;
+    return fp8_tile_of(tuning(kTuneF8Tm, per <= 8 ? 16 : per <= 24 ? 32 : per <= 48 ? 64 : per <= 160 ? 128 : 256));
+}
+
 struct Fp8MoeCut {
-    int rows, blocks;
+    int rows, blocks, tm;
     uint8_t *xq, *hq;
-    float *xs, *hs, *g, *u, *y, *w_row;
+    float *xs, *hs, *h, *y, *w_row;
     int32_t *blk_expert, *n_blocks, *tok_row, *row_slot;
     size_t bytes;
 };
 
+static Fp8MoeCut fp8_moe_cut_stream(uint8_t *base, int S, int D, int I) {
+    Fp8MoeCut m = {};
+    Fp8Cut c{base};
+    m.h = c.take<float>((size_t)S * I);
+    m.y = c.take<float>((size_t)S * D);
+    m.bytes = c.used;
+    return m;
+}
+
 static Fp8MoeCut fp8_moe_cut(uint8_t *base, int T, int k, int E, int D, int I) {
-    Fp8MoeCut m;
-    const int S = T * k, tm = kFp8MoeTm;
-    m.blocks = (S + tm - 1) / tm + E;
-    m.rows = m.blocks * tm;
+    Fp8MoeCut m = {};
+    const int S = T * k;
+    m.tm = fp8_moe_tile(S, E);
+    m.blocks = (S + m.tm - 1) / m.tm + E;
+    m.rows = m.blocks * m.tm;
     Fp8Cut c{base};
     m.xq = c.take<uint8_t>((size_t)T * D);
     m.xs = c.take<float>((size_t)T * fp8_groups(D));
@@ -377,8 +512,6 @@ static Fp8MoeCut fp8_moe_cut(uint8_t *base, int T, int k, int E, int D, int I) {
     m.tok_row = c.take<int32_t>(m.rows);
     m.w_row = c.take<float>(m.rows);
     m.row_slot = c.take<int32_t>(S);
-    m.g = c.take<float>((size_t)m.rows * I);
-    m.u = c.take<float>((size_t)m.rows * I);
     m.hq = c.take<uint8_t>((size_t)m.rows * I);
     m.hs = c.take<float>((size_t)m.rows * fp8_groups(I));
     m.y = c.take<float>((size_t)m.rows * D);
@@ -389,14 +522,21 @@ static Fp8MoeCut fp8_moe_cut(uint8_t *base, int T, int k, int E, int D, int I) {
 static int fp8_moe_check(int T, int k, int E, int D, int I) {
     if (T <= 0 || k <= 0 || (long long)T * k > kFp8MaxRows || (long long)T * D >= (1ll << 31)) return MI_ERR_TOKENS;
     if (E <= 0 || E > kMaxExperts || !fp8_cols_ok(D) || !fp8_cols_ok(I)) return MI_ERR_SHAPE;
-    const long long rows = (((long long)T * k + kFp8MoeTm - 1) / kFp8MoeTm + E) * kFp8MoeTm;
+    const long long rows = ((long long)T * k / 256 + 1 + E) * 256;
     return rows * I < (1ll << 31) ? MI_OK : MI_ERR_TOKENS;
+}
+
+// Enough for every smaller T too: the streaming form's slots besides the tiled form's rows, which grow with T.
+static size_t fp8_moe_bytes(int T, int k, int E, int D, int I) {
+    const int S = T * k;
+    const size_t few = fp8_moe_cut_stream(nullptr, std::min(S, MI_MAX_SLOTS), D, I).bytes;
+    return fp8_moe_streams(S) ? few : std::max(few, fp8_moe_cut(nullptr, T, k, E, D, I).bytes);
 }
 
 }  // namespace mi
 
 extern "C" size_t mi_fp8_moe_workspace(int32_t T, int32_t k, int32_t E, int32_t D, int32_t I) {
-    return fp8_moe_check(T, k, E, D, I) == MI_OK ? fp8_moe_cut(nullptr, T, k, E, D, I).bytes : 0;
+    return fp8_moe_check(T, k, E, D, I) == MI_OK ? fp8_moe_bytes(T, k, E, D, I) : 0;
 }
 
 extern "C" int mi_fp8_moe(const uint8_t *gate_q, const float *gate_s, const uint8_t *up_q, const float *up_s,
@@ -411,29 +551,52 @@ extern "C" int mi_fp8_moe(const uint8_t *gate_q, const float *gate_s, const uint
     if (rc == MI_OK) rc = fp8_check_w(down_q, down_s, E, D, I);
     if (rc != MI_OK) return rc;
     if (!(limit > 0.0f) || !aligned16(x) || !aligned4(idx) || !aligned4(w) || !fp8_y_ok(out_bf16, out_f32)) return MI_ERR_ARG;
-    const Fp8MoeCut m = fp8_moe_cut((uint8_t *)workspace, T, k, E, D, I);
-    if (!workspace || workspace_bytes < m.bytes) return MI_ERR_WORKSPACE;
+    if (!workspace || workspace_bytes < fp8_moe_bytes(T, k, E, D, I)) return MI_ERR_WORKSPACE;
     if (!aligned16(workspace)) return MI_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
-    if ((rc = fp8_launch_quantize(x, x_dtype, T, D, D, m.xq, m.xs, st)) != MI_OK) return rc;
-    rc = mi_ragged_plan(idx, w, T, k, E, kFp8MoeTm, m.blk_expert, m.n_blocks, m.tok_row, m.w_row, m.row_slot, stream);
-    if (rc != MI_OK) return rc;
-    Fp8Gemm a = {};
-    a.xq = m.xq, a.xs = m.xs;
-    a.tok_row = m.tok_row, a.blk_expert = m.blk_expert, a.n_blocks = m.n_blocks;
-    a.x_rows = T, a.rows = m.rows, a.tm = kFp8MoeTm;
-    a.E = E, a.R = I, a.K = D;
-    a.wq[0] = gate_q, a.ws[0] = gate_s, a.y_f32 = m.g;
-    if ((rc = fp8_launch_gemm(a, st)) != MI_OK) return rc;
-    a.wq[0] = up_q, a.ws[0] = up_s, a.y_f32 = m.u;
-    if ((rc = fp8_launch_gemm(a, st)) != MI_OK) return rc;
-    if ((rc = fp8_launch_swiglu(m.g, m.u, m.rows, I, limit, m.hq, m.hs, st)) != MI_OK) return rc;
-    a.xq = m.hq, a.xs = m.hs;
-    a.tok_row = nullptr, a.x_rows = m.rows;
-    a.R = D, a.K = I;
-    a.wq[0] = down_q, a.ws[0] = down_s, a.y_f32 = m.y;
-    if ((rc = fp8_launch_gemm(a, st)) != MI_OK) return rc;
-    hipLaunchKernelGGL(fp8_combine_kernel, dim3(T, (D + 255) / 256), dim3(256), 0, st, m.y, m.row_slot, w, T, k, D,
+    const int S = T * k;
+    Fp8MoeCut m;
+    if (fp8_moe_streams(S)) {
+        m = fp8_moe_cut_stream((uint8_t *)workspace, S, D, I);
+        Fp8Stream f = {};
+        f.x = x;
+        f.wq[0] = gate_q, f.ws[0] = gate_s, f.wq[1] = up_q, f.ws[1] = up_s;
+        f.idx = idx;
+        f.rows = S, f.div = k;
+        f.E = E, f.R = I, f.K = D;
+        f.limit = limit;
+        f.y_f32 = m.h;
+        rc = x_dtype == MI_X_BF16 ? fp8_launch_stream_as<MI_X_BF16, 1, 1, true, true, 3, 2>(f, st)
+                                  : fp8_launch_stream_as<MI_X_F32, 1, 1, true, true, 2, 2>(f, st);
+        if (rc != MI_OK) return rc;
+        f.x = m.h;
+        f.wq[0] = down_q, f.ws[0] = down_s;
+        f.div = 1;
+        f.R = D, f.K = I;
+        f.y_f32 = m.y;
+        if ((rc = fp8_launch_stream_as<MI_X_F32, 1, 2, false, true, 2, 2>(f, st)) != MI_OK) return rc;
+    } else {
+        m = fp8_moe_cut((uint8_t *)workspace, T, k, E, D, I);
+        if ((rc = fp8_launch_quantize(x, x_dtype, T, D, D, m.xq, m.xs, st)) != MI_OK) return rc;
+        rc = mi_ragged_plan(idx, w, T, k, E, m.tm, m.blk_expert, m.n_blocks, m.tok_row, m.w_row, m.row_slot, stream);
+        if (rc != MI_OK) return rc;
+        Fp8Tiled p = {};
+        Fp8Gemm &a = p.g;
+        a.xq = m.xq, a.xs = m.xs;
+        a.tok_row = m.tok_row, a.blk_expert = m.blk_expert, a.n_blocks = m.n_blocks;
+        a.x_rows = T, a.rows = m.rows, a.tm = m.tm;
+        a.E = E, a.R = I, a.K = D;
+        a.wq[0] = gate_q, a.ws[0] = gate_s, a.wq[1] = up_q, a.ws[1] = up_s;
+        p.S = 1;
+        p.limit = limit, p.hq = m.hq, p.hs = m.hs;
+        if ((rc = fp8_tiled<true>(p, 256, m.tm, st)) != MI_OK) return rc;
+        a.xq = m.hq, a.xs = m.hs;
+        a.tok_row = nullptr, a.x_rows = m.rows;
+        a.R = D, a.K = I;
+        a.wq[0] = down_q, a.ws[0] = down_s, a.y_f32 = m.y;
+        if ((rc = fp8_tiled<false>(p, 256, m.tm, st)) != MI_OK) return rc;
+    }
+    hipLaunchKernelGGL(fp8_combine_kernel, dim3(T, (D + 255) / 256), dim3(256), 0, st, m.y, m.row_slot, idx, E, w, k, D,
                        out_f32, out_bf16);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }

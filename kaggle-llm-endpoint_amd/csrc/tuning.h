@@ -18,6 +18,8 @@ enum Knob : int {
     kTuneI8S, kTuneI8Waves, kTuneI8Fuse,
     kTuneDgS1, kTuneDgS2, kTuneDgNt,         // many-token MLP: gate/up and down splits, token tiles per wavefront
     kTunePfWide,                             // prefill: 1 wide blocks, 0 narrow ones
+    kTuneF8Tw, kTuneF8Tt, kTuneF8S,          // dense fp8 product: weight rows and tokens per tile, splits of K
+    kTuneF8Stream, kTuneF8Tm,                // fp8 routed layer: most slots that stream, rows per block
     kTuneCount
 };
 

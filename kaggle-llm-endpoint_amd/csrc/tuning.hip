@@ -32,6 +32,7 @@ const Entry kNames[] = {
     {"I8S", kTuneI8S}, {"I8_WAVES", kTuneI8Waves}, {"I8_FUSE", kTuneI8Fuse},
     {"DG_S1", kTuneDgS1}, {"DG_S2", kTuneDgS2}, {"DG_NT", kTuneDgNt},
     {"PF_WIDE", kTunePfWide},
+    {"F8_TW", kTuneF8Tw}, {"F8_TT", kTuneF8Tt}, {"F8_S", kTuneF8S}, {"F8_STREAM", kTuneF8Stream}, {"F8_TM", kTuneF8Tm},
 };
 static_assert(sizeof(kNames) / sizeof(kNames[0]) == kTuneCount, "every knob has a name");
 
