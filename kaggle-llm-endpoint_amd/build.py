@@ -34,7 +34,9 @@ FLAGS = [
 # (source, extra defines, object name)
 UNITS = [("moe_decode.hip", [], "moe_decode"), ("int8_project.hip", [], "int8_project"),
          ("prefill.hip", [], "prefill"), ("route.hip", [], "route"),
-         ("pack.hip", [], "pack"), ("tuning.hip", [], "tuning"), ("fp8.hip", [], "fp8"),
+         ("pack.hip", [], "pack"), ("tuning.hip", [], "tuning"),
+         # matrix results straight into vector registers, where they are scaled, instead of by way of accumulation ones
+         ("fp8.hip", ["-mllvm", "-amdgpu-mfma-vgpr-form=1"], "fp8"),
          ("moe_rows.hip", [], "moe_rows")]
 UNITS += [("k_grouped.hip", ["-DMI_KMODE=%d" % m, "-DMI_KQT=%d" % q], "k_grouped_%d_%d" % (m, q))
           for m in (0, 1, 2) for q in (1, 2, 3, 4, 5, 6)]

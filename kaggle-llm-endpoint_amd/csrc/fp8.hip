@@ -118,20 +118,54 @@ __global__ void __launch_bounds__(256) fp8_zero_blocks_kernel(const int32_t *__r
 }
 
 // out[t] = sum_j w[t, j] * y[r(t, j)], f32, in column order: r the slot's sorted row, or (row_slot NULL) the slot itself.
+// Four outputs a thread, the rows of eight slots loaded before the first is added (D % 16 == 0).
 __global__ void __launch_bounds__(256) fp8_combine_kernel(const float *__restrict__ y, const int32_t *__restrict__ row_slot,
                                                           const int32_t *__restrict__ idx, int E,
                                                           const float *__restrict__ w, int k, int D, float *out_f32,
                                                           uint16_t *out_bf16) {
-    const int t = blockIdx.x, c = blockIdx.y * 256 + threadIdx.x;
+    const int t = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * 4;
     if (c >= D) return;
-    float acc = 0.0f;
-    for (int j = 0; j < k; ++j) {
-        const int s = t * k + j, e = idx[s];
-        const int r = e < 0 || e >= E ? -1 : row_slot ? row_slot[s] : s;
-        if (r >= 0) acc = fmaf(w[s], y[(size_t)r * D + c], acc);
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < k; j0 += 8) {
+        float4 v[8];
+        float wt[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int s = t * k + min(j0 + j, k - 1), e = idx[s];
+            const int r = j0 + j >= k || e < 0 || e >= E ? -1 : row_slot ? row_slot[s] : s;
+            wt[j] = w[s];
+            v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r >= 0) v[j] = *(const float4 *)(y + (size_t)r * D + c);
+            else wt[j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            acc[0] = fmaf(wt[j], v[j].x, acc[0]);
+            acc[1] = fmaf(wt[j], v[j].y, acc[1]);
+            acc[2] = fmaf(wt[j], v[j].z, acc[2]);
+            acc[3] = fmaf(wt[j], v[j].w, acc[3]);
+        }
     }
-    if (out_f32) out_f32[(size_t)t * D + c] = acc;
-    if (out_bf16) out_bf16[(size_t)t * D + c] = (uint16_t)f32_to_bf16_rne(acc);
+    const size_t at = (size_t)t * D + c;
+    if (out_f32) {
+        if (((uintptr_t)out_f32 & 15) == 0) {
+            *(float4 *)(out_f32 + at) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out_f32[at + j] = acc[j];
+        }
+    }
+    if (out_bf16) {
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = f32_to_bf16_rne(acc[j]);
+        if (((uintptr_t)out_bf16 & 7) == 0) {
+            *(uint2 *)(out_bf16 + at) = make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out_bf16[at + j] = (uint16_t)h[j];
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -181,7 +215,7 @@ static int fp8_tiled(const Fp8Tiled &p, int tw, int tt, hipStream_t st) {
         case 16: return fp8_launch_tiled<256, 16, 4, 1, 4, PAIR>(p, st);
         case 32: return fp8_launch_tiled<256, 32, 4, 1, 4, PAIR>(p, st);
         case 64: return fp8_launch_tiled<256, 64, 4, 1, 3, PAIR>(p, st);
-        case 128: return fp8_launch_tiled<256, 128, 2, 2, 3, PAIR>(p, st);
+        case 128: return fp8_launch_tiled<256, 128, 4, 2, 3, PAIR>(p, st);
         default: return fp8_launch_tiled<256, 256, 2, 4, 2, PAIR>(p, st);
     }
 }
@@ -475,7 +509,8 @@ namespace mi {
 
 // A call of at most MI_MAX_SLOTS slots whose experts are mostly distinct streams the experts' weights per slot; a larger
 // one sorts its slots by expert and takes the tiled product, its token tile the smaller the fewer rows an expert has.
-static bool fp8_moe_streams(int S) { return S <= std::min(tuning(kTuneF8Stream, MI_MAX_SLOTS), MI_MAX_SLOTS); }
+constexpr int kFp8StreamSlots = 16;
+static bool fp8_moe_streams(int S) { return S <= std::min(tuning(kTuneF8Stream, kFp8StreamSlots), MI_MAX_SLOTS); }
 static int fp8_moe_tile(int S, int E) {
     const int per = S / E;
     return fp8_tile_of(tuning(kTuneF8Tm, per <= 8 ? 16 : per <= 24 ? 32 : per <= 48 ? 64 : per <= 160 ? 128 : 256));
@@ -596,7 +631,7 @@ extern "C" int mi_fp8_moe(const uint8_t *gate_q, const float *gate_s, const uint
         a.wq[0] = down_q, a.ws[0] = down_s, a.y_f32 = m.y;
         if ((rc = fp8_tiled<false>(p, 256, m.tm, st)) != MI_OK) return rc;
     }
-    hipLaunchKernelGGL(fp8_combine_kernel, dim3(T, (D + 255) / 256), dim3(256), 0, st, m.y, m.row_slot, idx, E, w, k, D,
+    hipLaunchKernelGGL(fp8_combine_kernel, dim3(T, (D + 1023) / 1024), dim3(256), 0, st, m.y, m.row_slot, idx, E, w, k, D,
                        out_f32, out_bf16);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }

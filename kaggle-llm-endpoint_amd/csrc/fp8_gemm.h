@@ -4,6 +4,10 @@
 
 namespace mi {
 
+#ifndef NEAR
+#define NEAR 8
+#endif
+constexpr int kFp8Near = NEAR;                      // token tiles of a weight tile that run next to each other
 constexpr int kFp8MaxGroups = 1024;              // K / 128: the weight scales of a tile's blocks are kept in LDS
 
 // Memory to LDS without registers: lane l's 16 (4) bytes to dst + 16 l (4 l).
@@ -33,24 +37,25 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     static_assert(TW % (8 * W) == 0 && CT >= 1 && CT <= 4 && (!PAIR || (TW == 256 && RT % 2 == 0 && 16 % W == 0)), "");
     __shared__ uint4 buf0[ROWS * 8], buf1[ROWS * 8], buf2[NST > 2 ? ROWS * 8 : 1], buf3[NST > 3 ? ROWS * 8 : 1];
     __shared__ float sx0[W * 64], sx1[W * 64], sx2[NST > 2 ? W * 64 : 1], sx3[NST > 3 ? W * 64 : 1];
-    __shared__ float sw[2][kFp8MaxGroups];
+    __shared__ float sw[2][kFp8MaxGroups + 1];     // (a step reads one group ahead)
     const Fp8Gemm &a = p.g;
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
     const int KB = fp8_groups(a.K), RB = fp8_groups(a.R);
 
-    // an XCD's workgroups (ids equal modulo 8) take one contiguous piece of the work, two token tiles of a weight tile
-    // next to each other: they meet its weights in that XCD's L2
+    // An XCD's workgroups (ids equal modulo 8) take one contiguous piece of the work: kFp8Near token tiles of a weight tile,
+    // then of the next.  Its 32 CUs then work on about 8 token tiles x 4 weight tiles at a time and meet each other's
+    // loads in that XCD's L2; the blocks of one expert are next to each other and share its weights.
     const int nb = a.n_blocks ? min(max(*a.n_blocks, 0), p.nb) : p.nb;
     const long long total = (long long)nb * p.nw * p.S;
     const int xcd = blockIdx.x & 7, li = blockIdx.x >> 3;
     const long long first = total * xcd / 8, at = first + li;
     if (at >= total * (xcd + 1) / 8) return;
-    const int per2 = 2 * p.nw * p.S;
-    const int pr = (int)(at / per2), in2 = (int)(at - (long long)pr * per2);
-    const int width = min(2, nb - 2 * pr);
-    const int tb = 2 * pr + in2 % width, ws = in2 / width, wt = ws % p.nw, split = ws / p.nw;
+    const int per = kFp8Near * p.nw * p.S;
+    const int pr = (int)(at / per), in = (int)(at - (long long)pr * per);
+    const int width = min(kFp8Near, nb - kFp8Near * pr);
+    const int tb = kFp8Near * pr + in % width, ws = in / width, wt = ws % p.nw, split = ws / p.nw;
 
     const int row0 = tb * TT;                    // first row of the token tile
     const int o0 = wt * (PAIR ? TW / 2 : TW);    // first output of the weight tile
@@ -98,15 +103,17 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     }
     __syncthreads();
 
-    auto load = [&](uint4 *buf, float *sx, int g) __attribute__((always_inline)) {
-        const uint32_t past = g >= t1 || g * kFp8Group + col >= a.K ? kFp8Out : 0u;
-        const int so = g * kFp8Group;
-#pragma unroll
-        for (int j = 0; j < WL; ++j) lds_load16(rw[PAIR ? (j * W) / 16 : 0], buf + 64 * (j * W + wave), voff[j] | past, so);
-#pragma unroll
-        for (int j = 0; j < TL; ++j)
-            lds_load16(rx, buf + 8 * TW + 64 * ((j * W + wave) % (TT / 8)), voff[WL + j] | past, so);
-        lds_load4(rs, sx + 64 * wave, g >= t1 ? kFp8Out : soff, 4 * g);
+    constexpr int PER = WL + TL + 1;             // loads per wavefront and stage
+    auto past = [&](int g) __attribute__((always_inline)) {
+        return g >= t1 || g * kFp8Group + col >= a.K ? kFp8Out : 0u;
+    };
+    auto load_piece = [&](uint4 *buf, float *sx, int g, uint32_t pst, int j) __attribute__((always_inline)) {
+        if (j < WL)
+            lds_load16(rw[PAIR ? (j * W) / 16 : 0], buf + 64 * (j * W + wave), voff[j] | pst, g * kFp8Group);
+        else if (j < WL + TL)
+            lds_load16(rx, buf + 8 * TW + 64 * (((j - WL) * W + wave) % (TT / 8)), voff[j] | pst, g * kFp8Group);
+        else
+            lds_load4(rs, sx + 64 * wave, g >= t1 ? kFp8Out : soff, 4 * g);
     };
 
     f32x4 acc[RT][CT];
@@ -122,46 +129,92 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
         const uint4 u = buf[(row + i) * 8 + c0], v = buf[(row + i) * 8 + c1];
         return (i32x8){(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w};
     };
-    auto compute = [&](const uint4 *buf, const float *sx, int g) __attribute__((always_inline)) {
-        i32x8 b[CT];
-        float s[2][CT];
-        const int m0 = PAIR ? 0 : TW == 128 ? 0 : wm * 2 / WM;
-        const float w0 = sw[m0][g], w1 = PAIR ? sw[1][g] : 0.0f;
+    // One matrix instruction after the other, n = r CT + t, each followed by the scaling of the result two instructions
+    // older, which is done by then; weights are read from LDS two row tiles ahead, the next stage's tokens where this
+    // stage's are used last.  The order below is the order of the instructions: left alone the compiler puts each
+    // result's use right behind its instruction and waits for it.
+    //
+    // The only barrier of a stage is where its last fragment has been read: then the next stage must have landed (the
+    // later ones stay in flight), and this one's buffer may be overwritten.
+    constexpr int N = RT * CT, LAG = 2, BAR = RT - 2;
+    static_assert(RT % 4 == 0, "the rings w and v start every step at 0");
+    i32x8 b[CT], w[4];
+    f32x4 v[4];
+    float x[CT], w0, w1, s[PAIR ? 2 : 1][CT], last[LAG];
+    auto add = [&](int n, float sc) __attribute__((always_inline)) {
 #pragma unroll
-        for (int t = 0; t < CT; ++t) {
-            b[t] = frag(buf, TW + wn * CT * 16 + 16 * t);
-            const float x = sx[64 * wave + 16 * t + i];
-            s[0][t] = x * w0;
-            s[1][t] = PAIR ? x * w1 : 0.0f;
-        }
+        for (int j = 0; j < 4; ++j) acc[n / CT][n % CT][j] = fmaf(v[n & 3][j], sc, acc[n / CT][n % CT][j]);
+    };
+    auto read_x = [&](const uint4 *buf, const float *sx, int t) __attribute__((always_inline)) {
+        b[t] = frag(buf, TW + wn * CT * 16 + 16 * t);
+        x[t] = sx[64 * wave + 16 * t + i];
+    };
+    auto read_sw = [&](int g) __attribute__((always_inline)) {
+        w0 = sw[PAIR || TW == 128 ? 0 : wm * 2 / WM][g];
+        if (PAIR) w1 = sw[1][g];
+    };
+    // stage g in buf; the next stage in nbuf; buf takes stage g + NST
+    auto step = [&](uint4 *buf, float *sx, const uint4 *nbuf, const float *nsx, int g) __attribute__((always_inline)) {
+        const uint32_t pst = past(g + NST);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            const i32x8 w = frag(buf, wrow(r));
+            if (r == BAR) {
+                vm_wait<(NST - 2) * PER>();
+                lds_barrier();
+            }
+            w[(r + 2) & 3] = r + 2 < RT ? frag(buf, wrow(r + 2)) : frag(nbuf, wrow(r + 2 - RT));
+            if (r >= BAR) {
+#pragma unroll
+                for (int j = (r - BAR) * PER / (RT - BAR); j < (r - BAR + 1) * PER / (RT - BAR); ++j)
+                    load_piece(buf, sx, g + NST, pst, j);
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
-                const f32x4 v = fp8_mfma(w, b[t]);
-                const float sc = s[PAIR ? r / (RT / 2) : 0][t];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[r][t][j] = fmaf(v[j], sc, acc[r][t][j]);
+                const int n = r * CT + t;
+                if (r == 0) {
+                    s[0][t] = x[t] * w0;
+                    if (PAIR) s[PAIR ? 1 : 0][t] = x[t] * w1;
+                }
+                v[n & 3] = fp8_mfma(w[r & 3], b[t]);
+                if (n < LAG) add(N - LAG + n, last[n]);
+                else add(n - LAG, s[PAIR ? (n - LAG) / CT / (RT / 2) : 0][(n - LAG) % CT]);
+                if (r == RT - 1) read_x(nbuf, nsx, t);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
+        read_sw(g + 1);
+#pragma unroll
+        for (int k = 0; k < LAG; ++k) last[k] = s[PAIR ? 1 : 0][(N - LAG + k) % CT];
     };
-    constexpr int PER = WL + TL + 1;             // loads per wavefront and stage
     uint4 *const bufs[4] = {buf0, buf1, buf2, buf3};
     float *const sxs[4] = {sx0, sx1, sx2, sx3};
 #pragma unroll
-    for (int s = 0; s < NST - 1; ++s) load(bufs[s], sxs[s], t0 + s);
-    for (int t = t0; t < t1; t += NST) {
+    for (int st = 0; st < NST; ++st)
 #pragma unroll
-        for (int s = 0; s < NST; ++s) {
-            // stage t + s has landed (the later ones stay in flight) for every wavefront, and every wavefront is done
-            // with the buffer that the next loads overwrite
-            vm_wait<(NST - 2) * PER>();
-            lds_barrier();
-            load(bufs[(s + NST - 1) % NST], sxs[(s + NST - 1) % NST], t + s + NST - 1);
-            if (t + s < t1) compute(bufs[s], sxs[s], t + s);
-        }
+        for (int j = 0; j < PER; ++j) load_piece(bufs[st], sxs[st], t0 + st, past(t0 + st), j);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < LAG; ++k) last[k] = 0.0f;
+    vm_wait<(NST - 1) * PER>();
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < CT; ++t) read_x(buf0, sx0, t);
+    read_sw(t0);
+    w[0] = frag(buf0, wrow(0));
+    w[1] = frag(buf0, wrow(1));
+    int g = t0;
+    for (; g + NST <= t1; g += NST) {            // no branch between the steps
+#pragma unroll
+        for (int st = 0; st < NST; ++st)
+            step(bufs[st], sxs[st], bufs[(st + 1) % NST], sxs[(st + 1) % NST], g + st);
     }
+#pragma unroll
+    for (int st = 0; st < NST - 1; ++st)
+        if (g + st < t1) step(bufs[st], sxs[st], bufs[(st + 1) % NST], sxs[(st + 1) % NST], g + st);
+#pragma unroll
+    for (int k = 0; k < LAG; ++k) add(N - LAG + k, last[k]);
     vm_wait<0>();
 
     // ---- lane (i, q) holds outputs 4 q .. 4 q + 3 of each row tile for row 16 t + i
