@@ -449,13 +449,13 @@ size_t mi_fp8_mlp_workspace(int32_t B, int32_t D, int32_t I);
 /*
  * The rows of a ragged_plan times their experts' matrices (moe_ragged_down's product, pallas_moe.py:693-755):
  * n_blk blocks of tm rows (tm 16, 32, 64 or 128), block g's rows times expert blk_expert[g] of E; x (as for
- * mi_fp8_project) and y have n_blk * tm rows.  Blocks from *n_blocks on, and blocks of an expert outside [0, E), get
- * zeros.
+ * mi_fp8_project) and y have n_blk * tm rows.  Blocks from *n_blocks on, blocks of an expert outside [0, E), and with
+ * tok_row (may be NULL) the rows at the end of a block that it marks as padding (-1), get zeros whatever x holds there.
  */
 int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, int32_t n_blk, int32_t tm,
-                   const int32_t *blk_expert, const int32_t *n_blocks, const uint8_t *wq, const float *ws, int32_t E,
-                   int32_t K, int32_t R, uint16_t *y_bf16, float *y_f32, void *workspace, size_t workspace_bytes,
-                   void *stream);
+                   const int32_t *blk_expert, const int32_t *n_blocks, const int32_t *tok_row, const uint8_t *wq,
+                   const float *ws, int32_t E, int32_t K, int32_t R, uint16_t *y_bf16, float *y_f32, void *workspace,
+                   size_t workspace_bytes, void *stream);
 size_t mi_fp8_grouped_workspace(int32_t rows, int32_t K, int32_t R);
 
 /*

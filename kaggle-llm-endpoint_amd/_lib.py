@@ -121,7 +121,7 @@ def lib():
         "mi_fp8_project_workspace": (Z, [I, I, I]),
         "mi_fp8_mlp": (I, [P, I, P, I, I, I, P, P, P, P, P, P, F, P, P, P, Z, P]),
         "mi_fp8_mlp_workspace": (Z, [I, I, I]),
-        "mi_fp8_grouped": (I, [P, I, P, I, I, P, P, P, P, I, I, I, P, P, P, Z, P]),
+        "mi_fp8_grouped": (I, [P, I, P, I, I, P, P, P, P, P, I, I, I, P, P, P, Z, P]),
         "mi_fp8_grouped_workspace": (Z, [I, I, I]),
         "mi_fp8_moe": (I, [P, P, P, P, P, P, I, I, I, P, I, I, I, P, P, F, P, P, P, Z, P]),
         "mi_fp8_moe_workspace": (Z, [I, I, I, I, I]),

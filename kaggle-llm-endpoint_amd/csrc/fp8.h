@@ -72,6 +72,7 @@ struct Fp8Gemm {
     const uint8_t *wq[2];       // e4m3 [E, R, K]
     const float *ws[2];         // f32 [E, R / 128, K / 128]
     const int32_t *tok_row;     // [rows] or NULL
+    const int32_t *live;        // [rows] or NULL: < 0 marks rows without a token, the last ones of their block
     const int32_t *blk_expert;  // [rows / tm] or NULL
     const int32_t *n_blocks;    // [1] (with blk_expert)
     int x_rows;                 // rows of xq (bounds tok_row)

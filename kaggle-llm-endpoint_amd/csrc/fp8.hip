@@ -31,11 +31,13 @@ __device__ __forceinline__ void load8(const void *x, size_t at, float v[8]) {
 // Whole groups of lanes run or return together (the grid's tail), so the exchanges stay within live lanes.
 template <int XD>
 __global__ void __launch_bounds__(256) fp8_quantize_kernel(const void *__restrict__ x, int n, int K, long long stride,
-                                                           uint8_t *__restrict__ q, float *__restrict__ s) {
+                                                           const int32_t *__restrict__ live, uint8_t *__restrict__ q,
+                                                           float *__restrict__ s) {
     const int KB = fp8_groups(K);
     const long long gi = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
     if (gi >= (long long)n * KB) return;
     const int row = (int)(gi / KB), c = (int)(gi - (long long)row * KB);
+    if (live && live[row] < 0) return;           // (the same for the group's 16 lanes)
     const int col = c * kFp8Group + (threadIdx.x & 15) * 8;
     const bool in = col < K;                     // K % 16 == 0: a lane's values are all inside or all past the row
     float v[8];
@@ -182,14 +184,14 @@ static bool fp8_x_dtype_ok(int d) { return d == MI_X_BF16 || d == MI_X_F32 || d 
 // Bytes of n quantised rows of K columns: values, then scales.
 static size_t fp8_row_bytes(size_t n, int K) { return up256(n * K) + up256(n * fp8_groups(K) * sizeof(float)); }
 
-static int fp8_launch_quantize(const void *x, int x_dtype, int n, int K, long long stride, uint8_t *q, float *s,
-                               hipStream_t st) {
+static int fp8_launch_quantize(const void *x, int x_dtype, int n, int K, long long stride, const int32_t *live,
+                               uint8_t *q, float *s, hipStream_t st) {
     const long long threads = (long long)n * fp8_groups(K) * 16;
     const dim3 grid((unsigned)((threads + 255) / 256));
     if (x_dtype == MI_X_BF16)
-        hipLaunchKernelGGL(fp8_quantize_kernel<MI_X_BF16>, grid, dim3(256), 0, st, x, n, K, stride, q, s);
+        hipLaunchKernelGGL(fp8_quantize_kernel<MI_X_BF16>, grid, dim3(256), 0, st, x, n, K, stride, live, q, s);
     else
-        hipLaunchKernelGGL(fp8_quantize_kernel<MI_X_F32>, grid, dim3(256), 0, st, x, n, K, stride, q, s);
+        hipLaunchKernelGGL(fp8_quantize_kernel<MI_X_F32>, grid, dim3(256), 0, st, x, n, K, stride, live, q, s);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }
 
@@ -290,17 +292,24 @@ static int fp8_launch_dense_pair(Fp8Gemm a, float limit, uint8_t *hq, float *hs,
 // ---- the streaming product
 constexpr int kFp8StreamRows = 32;               // rows that the dense streaming kernels take
 
-template <int XD, int NT, int RW, bool PAIR, bool SLOTS, int U, int OCC>
+template <int XD, int NT, int RW, bool PAIR, bool SLOTS, int W, int U, int OCC>
 static int fp8_launch_stream_as(const Fp8Stream &a, hipStream_t st) {
     const dim3 grid((a.R + 16 * RW - 1) / (16 * RW), SLOTS ? a.rows : 1);
-    hipLaunchKernelGGL((fp8_stream_kernel<XD, NT, RW, PAIR, SLOTS, U, OCC>), grid, dim3(64 * kFp8StreamWaves), 0, st, a);
+    hipLaunchKernelGGL((fp8_stream_kernel<XD, NT, RW, PAIR, SLOTS, W, U, OCC>), grid, dim3(64 * W), 0, st, a);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }
 
+// Two row tiles a wavefront halve the reads of x, one gives twice the workgroups: two where that leaves half the CUs a
+// workgroup each (6144 x 6144: 1 / 16 / 32 rows take 12.6 / 19.9 / 30.9 us with one, 11.5 / 14.3 / 19.8 with two; 2048
+// x 6144: 16 / 32 rows 11.3 / 16.4 with one, 13.5 / 19.4 with two).
 template <int XD, bool PAIR>
 static int fp8_stream_dense_as(const Fp8Stream &a, hipStream_t st) {
-    if (a.rows > 16) return fp8_launch_stream_as<XD, 2, 1, PAIR, false, 2, 2>(a, st);
-    return fp8_launch_stream_as<XD, 1, 1, PAIR, false, XD == MI_X_F32 ? 2 : 3, PAIR || XD == MI_X_F32 ? 2 : 4>(a, st);
+    constexpr int U = XD == MI_X_F32 ? 1 : 2;
+    if (a.R / 32 >= kFp8Cus / 2)
+        return a.rows > 16 ? fp8_launch_stream_as<XD, 2, 2, PAIR, false, 4, U, 2>(a, st)
+                           : fp8_launch_stream_as<XD, 1, 2, PAIR, false, 4, 2, PAIR ? 2 : 3>(a, st);
+    return a.rows > 16 ? fp8_launch_stream_as<XD, 2, 1, PAIR, false, 4, U, 2>(a, st)
+                       : fp8_launch_stream_as<XD, 1, 1, PAIR, false, 4, XD == MI_X_F32 ? 2 : 3, 3>(a, st);
 }
 
 template <bool PAIR>
@@ -333,7 +342,7 @@ static int fp8_rows_of(const void *x, int x_dtype, const float *xs, int n, int K
     float *s = c.take<float>((size_t)n * fp8_groups(K));
     a.xq = q;
     a.xs = s;
-    return fp8_launch_quantize(x, x_dtype, n, K, K, q, s, st);
+    return fp8_launch_quantize(x, x_dtype, n, K, K, a.live, q, s, st);
 }
 
 static int fp8_check_x(const void *x, int x_dtype, const float *xs, int rows, int K) {
@@ -367,7 +376,7 @@ extern "C" int mi_fp8_quantize(const void *x, int32_t x_dtype, int32_t n, int32_
     if (!fp8_cols_ok(K)) return MI_ERR_SHAPE;
     if (x_stride < K || x_stride % 8 || x_stride > (1ll << 40)) return MI_ERR_ARG;
     if (!aligned16(x) || !aligned16(q) || !aligned4(s)) return MI_ERR_ARG;
-    return fp8_launch_quantize(x, x_dtype, n, K, x_stride, q, s, (hipStream_t)stream);
+    return fp8_launch_quantize(x, x_dtype, n, K, x_stride, nullptr, q, s, (hipStream_t)stream);
 }
 
 extern "C" size_t mi_fp8_project_workspace(int32_t B, int32_t n_in, int32_t n_out) {
@@ -472,8 +481,8 @@ extern "C" size_t mi_fp8_grouped_workspace(int32_t rows, int32_t K, int32_t R) {
 }
 
 extern "C" int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, int32_t n_blk, int32_t tm,
-                              const int32_t *blk_expert, const int32_t *n_blocks, const uint8_t *wq, const float *ws,
-                              int32_t E, int32_t K, int32_t R, uint16_t *y_bf16, float *y_f32, void *workspace,
+                              const int32_t *blk_expert, const int32_t *n_blocks, const int32_t *tok_row,
+                              const uint8_t *wq, const float *ws, int32_t E, int32_t K, int32_t R, uint16_t *y_bf16, float *y_f32, void *workspace,
                               size_t workspace_bytes, void *stream) {
     if (tm != 16 && tm != 32 && tm != 64 && tm != 128) return MI_ERR_ARG;
     if (n_blk <= 0 || n_blk > kFp8MaxRows / tm) return MI_ERR_TOKENS;
@@ -482,12 +491,13 @@ extern "C" int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, i
     if (rc == MI_OK) rc = fp8_check_w(wq, ws, E, R, K);
     if (rc != MI_OK) return rc;
     if (!blk_expert || !n_blocks || (!y_bf16 && !y_f32)) return MI_ERR_NULL;
-    if (!aligned4(blk_expert) || !aligned4(n_blocks) || !fp8_y_ok(y_bf16, y_f32)) return MI_ERR_ARG;
+    if (!aligned4(blk_expert) || !aligned4(n_blocks) || !aligned4(tok_row) || !fp8_y_ok(y_bf16, y_f32)) return MI_ERR_ARG;
     if (!workspace || workspace_bytes < mi_fp8_grouped_workspace(rows, K, R)) return MI_ERR_WORKSPACE;
     if (!aligned16(workspace)) return MI_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
     Fp8Cut c{(uint8_t *)workspace};
     Fp8Gemm a = {};
+    a.live = tok_row;
     rc = fp8_rows_of(x, x_dtype, xs, rows, K, c, a, st);
     if (rc != MI_OK) return rc;
     a.wq[0] = wq, a.ws[0] = ws;
@@ -513,7 +523,7 @@ constexpr int kFp8StreamSlots = 16;
 static bool fp8_moe_streams(int S) { return S <= std::min(tuning(kTuneF8Stream, kFp8StreamSlots), MI_MAX_SLOTS); }
 static int fp8_moe_tile(int S, int E) {
     const int per = S / E;
-    return fp8_tile_of(tuning(kTuneF8Tm, per <= 8 ? 16 : per <= 24 ? 32 : per <= 48 ? 64 : per <= 160 ? 128 : 256));
+    return fp8_tile_of(tuning(kTuneF8Tm, per <= 8 ? 16 : per <= 18 ? 32 : per <= 40 ? 64 : per <= 96 ? 128 : 256));
 }
 
 struct Fp8MoeCut {
@@ -601,28 +611,29 @@ extern "C" int mi_fp8_moe(const uint8_t *gate_q, const float *gate_s, const uint
         f.E = E, f.R = I, f.K = D;
         f.limit = limit;
         f.y_f32 = m.h;
-        rc = x_dtype == MI_X_BF16 ? fp8_launch_stream_as<MI_X_BF16, 1, 1, true, true, 3, 2>(f, st)
-                                  : fp8_launch_stream_as<MI_X_F32, 1, 1, true, true, 2, 2>(f, st);
+        rc = x_dtype == MI_X_BF16 ? fp8_launch_stream_as<MI_X_BF16, 1, 1, true, true, 4, 3, 3>(f, st)
+                                  : fp8_launch_stream_as<MI_X_F32, 1, 1, true, true, 4, 2, 3>(f, st);
         if (rc != MI_OK) return rc;
         f.x = m.h;
         f.wq[0] = down_q, f.ws[0] = down_s;
         f.div = 1;
         f.R = D, f.K = I;
         f.y_f32 = m.y;
-        if ((rc = fp8_launch_stream_as<MI_X_F32, 1, 2, false, true, 2, 2>(f, st)) != MI_OK) return rc;
+        if ((rc = fp8_launch_stream_as<MI_X_F32, 1, 2, false, true, 4, 2, 3>(f, st)) != MI_OK) return rc;
     } else {
         m = fp8_moe_cut((uint8_t *)workspace, T, k, E, D, I);
-        if ((rc = fp8_launch_quantize(x, x_dtype, T, D, D, m.xq, m.xs, st)) != MI_OK) return rc;
+        if ((rc = fp8_launch_quantize(x, x_dtype, T, D, D, nullptr, m.xq, m.xs, st)) != MI_OK) return rc;
         rc = mi_ragged_plan(idx, w, T, k, E, m.tm, m.blk_expert, m.n_blocks, m.tok_row, m.w_row, m.row_slot, stream);
         if (rc != MI_OK) return rc;
         Fp8Tiled p = {};
         Fp8Gemm &a = p.g;
         a.xq = m.xq, a.xs = m.xs;
-        a.tok_row = m.tok_row, a.blk_expert = m.blk_expert, a.n_blocks = m.n_blocks;
+        a.tok_row = a.live = m.tok_row, a.blk_expert = m.blk_expert, a.n_blocks = m.n_blocks;
         a.x_rows = T, a.rows = m.rows, a.tm = m.tm;
         a.E = E, a.R = I, a.K = D;
         a.wq[0] = gate_q, a.ws[0] = gate_s, a.wq[1] = up_q, a.ws[1] = up_s;
         p.S = 1;
+        p.skip = 1;
         p.limit = limit, p.hq = m.hq, p.hs = m.hs;
         if ((rc = fp8_tiled<true>(p, 256, m.tm, st)) != MI_OK) return rc;
         a.xq = m.hq, a.xs = m.hs;

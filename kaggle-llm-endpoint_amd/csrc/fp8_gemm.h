@@ -1,13 +1,12 @@
 // Tiled block-scaled fp8 product (fp8.h) for many rows, dense or of sorted rows by expert.
 #pragma once
+#include <type_traits>
+
 #include "fp8.h"
 
 namespace mi {
 
-#ifndef NEAR
-#define NEAR 8
-#endif
-constexpr int kFp8Near = NEAR;                      // token tiles of a weight tile that run next to each other
+constexpr int kFp8Near = 8;                      // token tiles of a weight tile that run next to each other
 constexpr int kFp8MaxGroups = 1024;              // K / 128: the weight scales of a tile's blocks are kept in LDS
 
 // Memory to LDS without registers: lane l's 16 (4) bytes to dst + 16 l (4 l).
@@ -23,6 +22,7 @@ struct Fp8Tiled {
     int nw;                     // weight tiles
     int nb;                     // token tiles (grouped: at most; *g.n_blocks are used)
     int S;                      // splits of K
+    int skip;                   // rows without a token are not written (else: zeros)
     float limit;                // PAIR
     uint8_t *hq;                // PAIR: e4m3 [rows, R] and its scales
     float *hs;
@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     constexpr int W = WM * WN, RT = TW / WM / 16, CT = TT / WN / 16;
     constexpr int WL = TW / 8 / W, TL = TT / 8 >= W ? TT / 8 / W : 1;      // 1 KB loads per wavefront and stage
     constexpr int ROWS = TW + TT;
-    static_assert(TW % (8 * W) == 0 && CT >= 1 && CT <= 4 && (!PAIR || (TW == 256 && RT % 2 == 0 && 16 % W == 0)), "");
+    static_assert(TW % (8 * W) == 0 && (CT == 1 || CT == 2 || CT == 4) && (!PAIR || (TW == 256 && RT % 2 == 0 && 16 % W == 0)), "");
     __shared__ uint4 buf0[ROWS * 8], buf1[ROWS * 8], buf2[NST > 2 ? ROWS * 8 : 1], buf3[NST > 3 ? ROWS * 8 : 1];
     __shared__ float sx0[W * 64], sx1[W * 64], sx2[NST > 2 ? W * 64 : 1], sx3[NST > 3 ? W * 64 : 1];
     __shared__ float sw[2][kFp8MaxGroups + 1];     // (a step reads one group ahead)
@@ -66,6 +66,20 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     }
     const int t0 = split * KB / p.S, t1 = (split + 1) * KB / p.S;
 
+    // token tile t of wavefront column wn is rows 16 (t WN + wn) ..: dealt out in turn, so that a block with fewer rows
+    // takes as many steps less of every wavefront.  Rows are filled from the front (live says which are).
+    int used = min(TT, a.rows - row0);
+    if (a.live) {
+        int n = 0;
+        for (int r = lane; r < TT; r += 64)
+            if (row0 + r < a.rows && a.live[row0 + r] >= 0) n = r + 1;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) n = max(n, __shfl_xor(n, m, 64));
+        used = __builtin_amdgcn_readfirstlane(n);
+    }
+    const int ct = (used + 16 * WN - 1) / (16 * WN);
+    auto trow = [&](int t) { return 16 * (t * WN + wn); };
+
     // ---- loads: instruction j of a wavefront fills 8 LDS rows of 128 bytes; 16-byte slot c of row r holds chunk
     // c ^ (r & 7) of the row, so that the fragment reads below spread over the banks
     const int col = 16 * ((lane & 7) ^ (lane >> 3));
@@ -84,7 +98,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     rs = __builtin_amdgcn_make_buffer_rsrc((void *)a.xs, (short)0, 0x7fffffff, kFp8Word3);
     auto token = [&](int r) {                    // row r of the tile: its row of xq, -1 for none
         int tok = row0 + r;
-        if (tok >= a.rows) return -1;
+        if (tok >= a.rows || (a.live && a.live[tok] < 0)) return -1;
         if (a.tok_row) tok = a.tok_row[tok];
         return tok < a.x_rows ? tok : -1;
     };
@@ -93,7 +107,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
         const int tok = token(8 * ((j * W + wave) % (TT / 8)) + (lane >> 3));
         voff[WL + j] = tok < 0 ? kFp8Out : (uint32_t)tok * (uint32_t)a.K + col;
     }
-    const int stok = token(wn * CT * 16 + lane % (CT * 16));
+    const int stok = token(trow(lane / 16 % CT) + i);
     const uint32_t soff = stok < 0 ? kFp8Out : (uint32_t)stok * (uint32_t)KB * 4u;
     // weight scales of the tile's one or two blocks
 #pragma unroll
@@ -129,92 +143,98 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
         const uint4 u = buf[(row + i) * 8 + c0], v = buf[(row + i) * 8 + c1];
         return (i32x8){(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w};
     };
-    // One matrix instruction after the other, n = r CT + t, each followed by the scaling of the result two instructions
-    // older, which is done by then; weights are read from LDS two row tiles ahead, the next stage's tokens where this
+    // One matrix instruction after the other, n = r CU + t, each behind the scaling of the result two instructions
+    // older, which is done by then; weights are read from LDS WD row tiles ahead (one where registers are short), the next stage's tokens where this
     // stage's are used last.  The order below is the order of the instructions: left alone the compiler puts each
     // result's use right behind its instruction and waits for it.
     //
     // The only barrier of a stage is where its last fragment has been read: then the next stage must have landed (the
     // later ones stay in flight), and this one's buffer may be overwritten.
-    constexpr int N = RT * CT, LAG = 2, BAR = RT - 2;
-    static_assert(RT % 4 == 0, "the rings w and v start every step at 0");
-    i32x8 b[CT], w[4];
-    f32x4 v[4];
-    float x[CT], w0, w1, s[PAIR ? 2 : 1][CT], last[LAG];
-    auto add = [&](int n, float sc) __attribute__((always_inline)) {
+    auto main_loop = [&](auto cu) __attribute__((always_inline)) {
+        constexpr int CU = decltype(cu)::value, N = RT * CU, LAG = 2, WD = RT * CU > 16 ? 1 : 2, BAR = RT - WD;
+        static_assert(RT % 4 == 0, "the rings w and v start every step at 0");
+        i32x8 b[CU], w[4];
+        f32x4 v[4];
+        float x[CU], w0, w1, s[PAIR ? 2 : 1][CU], last[LAG];
+        auto add = [&](int n, float sc) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[n / CT][n % CT][j] = fmaf(v[n & 3][j], sc, acc[n / CT][n % CT][j]);
-    };
-    auto read_x = [&](const uint4 *buf, const float *sx, int t) __attribute__((always_inline)) {
-        b[t] = frag(buf, TW + wn * CT * 16 + 16 * t);
-        x[t] = sx[64 * wave + 16 * t + i];
-    };
-    auto read_sw = [&](int g) __attribute__((always_inline)) {
-        w0 = sw[PAIR || TW == 128 ? 0 : wm * 2 / WM][g];
-        if (PAIR) w1 = sw[1][g];
-    };
-    // stage g in buf; the next stage in nbuf; buf takes stage g + NST
-    auto step = [&](uint4 *buf, float *sx, const uint4 *nbuf, const float *nsx, int g) __attribute__((always_inline)) {
-        const uint32_t pst = past(g + NST);
+            for (int j = 0; j < 4; ++j) acc[n / CU][n % CU][j] = fmaf(v[n & 3][j], sc, acc[n / CU][n % CU][j]);
+        };
+        auto read_x = [&](const uint4 *buf, const float *sx, int t) __attribute__((always_inline)) {
+            b[t] = frag(buf, TW + trow(t));
+            x[t] = sx[64 * wave + 16 * t + i];
+        };
+        auto read_sw = [&](int g) __attribute__((always_inline)) {
+            w0 = sw[PAIR || TW == 128 ? 0 : wm * 2 / WM][g];
+            if (PAIR) w1 = sw[1][g];
+        };
+        // stage g in buf; the next stage in nbuf; buf takes stage g + NST
+        auto step = [&](uint4 *buf, float *sx, const uint4 *nbuf, const float *nsx, int g) __attribute__((always_inline)) {
+            const uint32_t pst = past(g + NST);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            if (r == BAR) {
-                vm_wait<(NST - 2) * PER>();
-                lds_barrier();
-            }
-            w[(r + 2) & 3] = r + 2 < RT ? frag(buf, wrow(r + 2)) : frag(nbuf, wrow(r + 2 - RT));
-            if (r >= BAR) {
-#pragma unroll
-                for (int j = (r - BAR) * PER / (RT - BAR); j < (r - BAR + 1) * PER / (RT - BAR); ++j)
-                    load_piece(buf, sx, g + NST, pst, j);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                const int n = r * CT + t;
-                if (r == 0) {
-                    s[0][t] = x[t] * w0;
-                    if (PAIR) s[PAIR ? 1 : 0][t] = x[t] * w1;
+            for (int r = 0; r < RT; ++r) {
+                if (r == BAR) {
+                    vm_wait<(NST - 2) * PER>();
+                    lds_barrier();
                 }
-                v[n & 3] = fp8_mfma(w[r & 3], b[t]);
-                if (n < LAG) add(N - LAG + n, last[n]);
-                else add(n - LAG, s[PAIR ? (n - LAG) / CT / (RT / 2) : 0][(n - LAG) % CT]);
-                if (r == RT - 1) read_x(nbuf, nsx, t);
+                w[(r + WD) & 3] = r + WD < RT ? frag(buf, wrow(r + WD)) : frag(nbuf, wrow(r + WD - RT));
+                if (r >= BAR) {
+#pragma unroll
+                    for (int j = (r - BAR) * PER / (RT - BAR); j < (r - BAR + 1) * PER / (RT - BAR); ++j)
+                        load_piece(buf, sx, g + NST, pst, j);
+                }
                 __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < CU; ++t) {
+                    const int n = r * CU + t;
+                    if (r == 0) {
+                        s[0][t] = x[t] * w0;
+                        if (PAIR) s[PAIR ? 1 : 0][t] = x[t] * w1;
+                    }
+                    if (n < LAG) add(N - LAG + n, last[n]);
+                    else add(n - LAG, s[PAIR ? (n - LAG) / CU / (RT / 2) : 0][(n - LAG) % CU]);
+                    v[n & 3] = fp8_mfma(w[r & 3], b[t]);
+                    if (r == RT - 1) read_x(nbuf, nsx, t);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
-        }
-        read_sw(g + 1);
+            read_sw(g + 1);
 #pragma unroll
-        for (int k = 0; k < LAG; ++k) last[k] = s[PAIR ? 1 : 0][(N - LAG + k) % CT];
-    };
-    uint4 *const bufs[4] = {buf0, buf1, buf2, buf3};
-    float *const sxs[4] = {sx0, sx1, sx2, sx3};
-#pragma unroll
-    for (int st = 0; st < NST; ++st)
-#pragma unroll
-        for (int j = 0; j < PER; ++j) load_piece(bufs[st], sxs[st], t0 + st, past(t0 + st), j);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < LAG; ++k) last[k] = 0.0f;
-    vm_wait<(NST - 1) * PER>();
-    lds_barrier();
-#pragma unroll
-    for (int t = 0; t < CT; ++t) read_x(buf0, sx0, t);
-    read_sw(t0);
-    w[0] = frag(buf0, wrow(0));
-    w[1] = frag(buf0, wrow(1));
-    int g = t0;
-    for (; g + NST <= t1; g += NST) {            // no branch between the steps
+            for (int k = 0; k < LAG; ++k) last[k] = s[PAIR ? 1 : 0][(N - LAG + k) % CU];
+        };
+        uint4 *const bufs[4] = {buf0, buf1, buf2, buf3};
+        float *const sxs[4] = {sx0, sx1, sx2, sx3};
 #pragma unroll
         for (int st = 0; st < NST; ++st)
-            step(bufs[st], sxs[st], bufs[(st + 1) % NST], sxs[(st + 1) % NST], g + st);
-    }
 #pragma unroll
-    for (int st = 0; st < NST - 1; ++st)
-        if (g + st < t1) step(bufs[st], sxs[st], bufs[(st + 1) % NST], sxs[(st + 1) % NST], g + st);
+            for (int j = 0; j < PER; ++j) load_piece(bufs[st], sxs[st], t0 + st, past(t0 + st), j);
 #pragma unroll
-    for (int k = 0; k < LAG; ++k) add(N - LAG + k, last[k]);
+        for (int k = 0; k < 4; ++k) v[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < LAG; ++k) last[k] = 0.0f;
+        vm_wait<(NST - 1) * PER>();
+        lds_barrier();
+#pragma unroll
+        for (int t = 0; t < CU; ++t) read_x(buf0, sx0, t);
+        read_sw(t0);
+        w[0] = frag(buf0, wrow(0));
+        if (WD > 1) w[1] = frag(buf0, wrow(1));
+        int g = t0;
+        for (; g + NST <= t1; g += NST) {            // no branch between the steps
+#pragma unroll
+            for (int st = 0; st < NST; ++st)
+                step(bufs[st], sxs[st], bufs[(st + 1) % NST], sxs[(st + 1) % NST], g + st);
+        }
+#pragma unroll
+        for (int st = 0; st < NST - 1; ++st)
+            if (g + st < t1) step(bufs[st], sxs[st], bufs[(st + 1) % NST], sxs[(st + 1) % NST], g + st);
+#pragma unroll
+        for (int k = 0; k < LAG; ++k) add(N - LAG + k, last[k]);
+    };
+    if (CT == 4 && ct >= 4) main_loop(std::integral_constant<int, CT >= 4 ? 4 : 1>{});
+    else if (CT == 4 && ct == 3) main_loop(std::integral_constant<int, CT >= 4 ? 3 : 1>{});
+    else if (CT >= 2 && ct >= 2) main_loop(std::integral_constant<int, CT >= 2 ? 2 : 1>{});
+    else main_loop(std::integral_constant<int, 1>{});
     vm_wait<0>();
 
     // ---- lane (i, q) holds outputs 4 q .. 4 q + 3 of each row tile for row 16 t + i
@@ -239,18 +259,18 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
                     }
                 am[t] = max(am[t], (uint32_t)__shfl_xor((int)am[t], 16, 64));
                 am[t] = max(am[t], (uint32_t)__shfl_xor((int)am[t], 32, 64));
-                if (q == 0) red[wm * TT + wn * CT * 16 + 16 * t + i] = __uint_as_float(am[t]);
+                if (q == 0) red[wm * TT + trow(t) + i] = __uint_as_float(am[t]);
             }
             __syncthreads();
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
-                const int c = wn * CT * 16 + 16 * t + i, row = row0 + c;
+                const int c = trow(t) + i, row = row0 + c;
                 uint32_t m = 0;
 #pragma unroll
                 for (int k = 0; k < WM; ++k) m = max(m, __float_as_uint(red[k * TT + c]));
                 const int ex = fp8_exponent(m);
                 const float inv = exp2_int(-ex);
-                if (row >= a.rows) continue;
+                if (row >= a.rows || (p.skip && a.live[row] < 0)) continue;
                 if (wm == 0 && q == 0) p.hs[(size_t)row * RB + o0 / kFp8Group] = exp2_int(ex);
 #pragma unroll
                 for (int r = 0; r < RT / 2; ++r) {
@@ -268,8 +288,8 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     const bool b8 = quads && ((uintptr_t)a.y_bf16 & 7) == 0, f16 = quads && ((uintptr_t)a.y_f32 & 15) == 0;
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
-        const int row = row0 + wn * CT * 16 + 16 * t + i;
-        if (row >= a.rows) continue;
+        const int row = row0 + trow(t) + i;
+        if (row >= a.rows || (p.skip && a.live[row] < 0)) continue;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int m = PAIR ? r / (RT / 2) : 0;

@@ -1,15 +1,13 @@
 // Block-scaled fp8 product (fp8.h) for few rows: the weights stream from memory into registers once.
 //
-// A workgroup owns 16 RW outputs (of each of two matrices, PAIR) for up to 16 NT rows; its 8 wavefronts split the groups of
+// A workgroup owns 16 RW outputs (of each of two matrices, PAIR) for up to 16 NT rows; its W wavefronts split the groups of
 // 128 columns, each holds U groups' weights in flight, quantises its own part of the activations in registers (a group of a
 // row is 32 values in each of 4 lanes: two exchanges give its maximum) and multiplies with one instruction per group and
-// tile; the 8 sums are added through LDS in wavefront order.
+// tile; the W sums are added through LDS in wavefront order.
 #pragma once
 #include "fp8.h"
 
 namespace mi {
-
-constexpr int kFp8StreamWaves = 8;
 
 struct Fp8Stream {
     const void *x;              // bf16, f32 or e4m3 [x_rows, K] (XD)
@@ -96,9 +94,9 @@ __device__ __forceinline__ i32x8 fp8_x_quantize(const Fp8X<XD> &f, float &scale)
     return o;
 }
 
-template <int XD, int NT, int RW, bool PAIR, bool SLOTS, int U, int OCC>
-__global__ void __launch_bounds__(64 * kFp8StreamWaves, OCC) fp8_stream_kernel(Fp8Stream a) {
-    constexpr int M = PAIR ? 2 : 1, W = kFp8StreamWaves, TILES = M * RW * NT;
+template <int XD, int NT, int RW, bool PAIR, bool SLOTS, int W, int U, int OCC>
+__global__ void __launch_bounds__(64 * W, OCC) fp8_stream_kernel(Fp8Stream a) {
+    constexpr int M = PAIR ? 2 : 1, TILES = M * RW * NT;
     static_assert(!SLOTS || NT == 1, "a slot tile is 16 slots");
     __shared__ f32x4 red[W][TILES][64];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;

@@ -201,22 +201,21 @@ def fp8_mlp(x, gate, up, down, limit, want_f32=False, y_bf16=None, y_f32=None, w
 def fp8_grouped(xs, plan, leaf, want_f32=False, y_bf16=None, y_f32=None, workspace=None):
     """The sorted rows of a ragged_plan (tm 16, 32, 64 or 128), each times its expert's matrix of ``leaf`` [E, R, K]: xs
     bf16 or f32 [Rp, K] (moe_dispatch's rows) or fp8_quantize's pair -> y bf16 [Rp, R] (and y f32 with want_f32), ready
-    for moe_combine.  Rows of blocks that the plan does not use are zero."""
+    for moe_combine.  Rows of blocks that the plan does not use, and padding rows, are zero."""
     E, R, K = _leaf_dims(leaf, "fp8_grouped")
     if leaf.q.dim() != 3:
         raise ValueError("fp8_grouped: the weights must be [E, R, K]")
     r = _rows_of(xs, K, "fp8_grouped")
-    blk, nb = _as(plan["blk_expert"], torch.int32), _as(plan["n_blocks"], torch.int32)
+    blk, nb, tok = [_as(plan[k], torch.int32) for k in ("blk_expert", "n_blocks", "tok_row")]
     rows, G = r.x.shape[0], blk.numel()
-    if rows != plan["tok_row"].numel() or nb.numel() != 1 or G == 0 or rows % G:
-        raise ValueError("fp8_grouped: %d rows do not fit the plan's %d rows in %d blocks" % (rows, plan["tok_row"].numel(),
-                                                                                             G))
+    if rows != tok.numel() or nb.numel() != 1 or G == 0 or rows % G:
+        raise ValueError("fp8_grouped: %d rows do not fit the plan's %d rows in %d blocks" % (rows, tok.numel(), G))
     yb = _out(y_bf16, (rows, R), torch.bfloat16, "fp8_grouped", r.x.device)
     yf = _out(y_f32, (rows, R), torch.float32, "fp8_grouped", r.x.device) if want_f32 or y_f32 is not None else None
-    _one_device("fp8_grouped", r.x, r.xs, blk, nb, leaf.q, leaf.s, yb, yf, workspace)
+    _one_device("fp8_grouped", r.x, r.xs, blk, nb, tok, leaf.q, leaf.s, yb, yf, workspace)
     ws = _workspace(workspace, lib().mi_fp8_grouped_workspace(rows, K, R), "fp8_grouped", r.x.device)
     check("mi_fp8_grouped", lib().mi_fp8_grouped(_ptr(r.x), r.dtype, _ptr(r.xs), G, rows // G, _ptr(blk), _ptr(nb),
-                                                 _ptr(leaf.q), _ptr(leaf.s), E, K, R, _ptr(yb), _ptr(yf), _ptr(ws),
+                                                 _ptr(tok), _ptr(leaf.q), _ptr(leaf.s), E, K, R, _ptr(yb), _ptr(yf), _ptr(ws),
                                                  ws.numel(), _stream()))
     return (yb, yf) if want_f32 else yb
 

@@ -269,9 +269,13 @@ def test_grouped_plan_out_of_range(pkg, gpu):
     leaf = _leaf(pkg, *of8.random_weights(rng, 100, 128, 0.05, 3))
     x = _acts(rng, 64, 128)
     plan = {"blk_expert": torch.tensor([0, -1, 3, 2], dtype=torch.int32, device="cuda"),
-            "n_blocks": torch.tensor([1000], dtype=torch.int32, device="cuda"), "tok_row": torch.zeros(64, dtype=torch.int32)}
+            "n_blocks": torch.tensor([1000], dtype=torch.int32, device="cuda"),
+            "tok_row": torch.zeros(64, dtype=torch.int32, device="cuda")}
     y = pkg.fp8_grouped(x, plan, leaf, want_f32=True)[1]
     assert (y[16:48] == 0).all() and (y[:16] != 0).any() and (y[48:] != 0).any()
+    plan["tok_row"][5:16] = -1                            # padding rows: zeros whatever x holds
+    z = pkg.fp8_grouped(x, plan, leaf, want_f32=True)[1]
+    assert (z[5:16] == 0).all() and torch.equal(z[:5], y[:5]) and torch.equal(z[48:], y[48:])
     plan["n_blocks"].fill_(-5)
     assert (pkg.fp8_grouped(x, plan, leaf) == 0).all()
 

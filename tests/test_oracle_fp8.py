@@ -112,7 +112,7 @@ def test_mlp_refusals(L):
 def test_grouped_refusals(L):
     need = L.mi_fp8_grouped_workspace(8 * 32, 256, 100)
     call = lambda x=X, n=8, tm=32, be=P(0x60000), nb=P(0x70000), E=4, K=256, R=100, y=Y, wb=BIG: L.mi_fp8_grouped(
-        x, 0, None, n, tm, be, nb, Q, S, E, K, R, y, None, WS, wb, None)
+        x, 0, None, n, tm, be, nb, P(0x80000), Q, S, E, K, R, y, None, WS, wb, None)
     assert call(tm=48) == 8 and call(tm=0) == 8 and call(tm=256) == 8
     assert call(n=0) == 4 and call(n=1 << 20) == 4
     assert call(E=0) == 3 and call(E=1025) == 3 and call(K=24) == 3
