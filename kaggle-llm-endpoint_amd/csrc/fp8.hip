@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(256) fp8_combine_kernel(const float *__restric
 }
 
 // ------------------------------------------------------------------------------------------------ host side
-constexpr int kFp8MaxCols = 1 << 17;             // K, R: 32-bit offsets within a tile of 256 rows
+constexpr int kFp8MaxCols = 1 << 16;             // K, R: a tile's weight scales in LDS
 constexpr int kFp8MaxRows = 1 << 22;             // rows of activations
 
 static bool fp8_cols_ok(int K) { return K > 0 && K % 16 == 0 && K <= kFp8MaxCols; }
@@ -210,7 +210,7 @@ static int fp8_launch_tiled(Fp8Tiled p, hipStream_t st) {
 template <bool PAIR>
 static int fp8_tiled(const Fp8Tiled &p, int tw, int tt, hipStream_t st) {
     if constexpr (!PAIR) {
-        if (tw == 128) return tt == 64 ? fp8_launch_tiled<128, 64, 2, 2, 4, false>(p, st)
+        if (tw == 128) return tt == 64 ? fp8_launch_tiled<128, 64, 2, 2, 3, false>(p, st)
                                        : fp8_launch_tiled<128, 128, 2, 2, 4, false>(p, st);
     }
     switch (tt) {
@@ -222,16 +222,18 @@ static int fp8_tiled(const Fp8Tiled &p, int tw, int tt, hipStream_t st) {
     }
 }
 
-// The tiles and splits of a dense product of B rows: the largest tiles that still give every CU one, splits of K where
-// even the smallest leave CUs idle (each at least 4 groups of columns).
+// The tile and the splits of K of a dense product of B rows: the pair of least estimated time.  A round of tiles (one per CU,
+// two of the smallest) takes `step` us per group of 128 columns -- measured with weights from memory, 144 to 576 tiles, 2048
+// and 6144 columns, within a tenth -- and a split adds a launch and a pass over its partial sums.  Splits only fill CUs of
+// the first round.  (6144 x 6144, 96 / 384 / 1536 rows: 22 us with 128 x 64 in two splits, 45 with 128 x 128, 97 with
+// 256 x 256; each of the others takes 1.1 to 3 times as long at two of the three sizes.)
 struct Fp8Plan {
     int tw, tt, S;
 };
 constexpr int kFp8Cus = 256;
 constexpr int kFp8SplitTiles = 512;              // tiles x splits at most
 
-// Floats of split sums that any B up to the given one may need: S * tiles <= kFp8SplitTiles, so S * B * R is within
-// kFp8SplitTiles tiles whatever B is.
+// Floats of split sums that any B up to the given one may need.
 static size_t fp8_split_floats(int R, bool pair) {
     const size_t n = (size_t)(R + 127) / 128;    // tiles of 128 outputs per token tile
     return std::max<size_t>(kFp8SplitTiles / n, 1) * 64 * R * (pair ? 2 : 1);
@@ -241,23 +243,34 @@ static size_t fp8_split_floats(int R, bool pair) {
 static int fp8_tile_of(int tt) { return tt <= 16 ? 16 : tt <= 32 ? 32 : tt <= 64 ? 64 : tt <= 128 ? 128 : 256; }
 
 static Fp8Plan fp8_plan(int B, int R, int K, bool pair) {
-    auto tiles = [&](int tw, int tt) {
-        const int w = pair ? tw / 2 : tw;
-        return (long long)((R + w - 1) / w) * ((B + tt - 1) / tt);
+    struct Tile {
+        int tw, tt, slots;
+        float step;
     };
-    Fp8Plan p{256, 64, 1};
-    if (tiles(256, 256) >= kFp8Cus) p.tt = 256;
-    else if (tiles(256, 128) >= kFp8Cus) p.tt = 128;
-    else if (pair) p.tt = B <= 32 ? 32 : 64;
-    else p.tw = 128, p.tt = B > 64 && tiles(128, 128) >= kFp8Cus ? 128 : 64;
-    p.tw = !pair && tuning(kTuneF8Tw, p.tw) == 128 ? 128 : 256;
-    p.tt = fp8_tile_of(tuning(kTuneF8Tt, p.tt));
-    if (p.tw == 128) p.tt = std::min(std::max(p.tt, 64), 128);
-    const long long n = tiles(p.tw, p.tt);
-    if (n < kFp8Cus) p.S = (int)std::max(1ll, std::min<long long>(kFp8SplitTiles / n, fp8_groups(K) / 4));
-    p.S = std::max(1, std::min(tuning(kTuneF8S, p.S), fp8_groups(K)));
-    if ((size_t)p.S * B * R * (pair ? 2 : 1) > fp8_split_floats(R, pair)) p.S = 1;
-    return p;
+    static const Tile dense[] = {{128, 64, 2 * kFp8Cus, 0.7f}, {128, 128, kFp8Cus, 0.85f}, {256, 64, kFp8Cus, 0.9f},
+                                 {256, 128, kFp8Cus, 1.35f}, {256, 256, kFp8Cus, 2.1f}};
+    static const Tile gate_up[] = {{256, 32, kFp8Cus, 0.75f}, {256, 64, kFp8Cus, 0.9f}, {256, 128, kFp8Cus, 1.35f},
+                                   {256, 256, kFp8Cus, 2.1f}};
+    const Tile *c = pair ? gate_up : dense;
+    const int n = pair ? 4 : 5, KB = fp8_groups(K);
+    const int tw = tuning(kTuneF8Tw, 0), tt = tuning(kTuneF8Tt, 0), fs = tuning(kTuneF8S, 0);
+    Fp8Plan best{c[0].tw, c[0].tt, 1};
+    float least = 1e30f;
+    for (int i = 0; i < n; ++i) {
+        if ((tw && !pair && c[i].tw != tw) || (tt && c[i].tt != tt)) continue;
+        const int w = pair ? c[i].tw / 2 : c[i].tw;
+        const long long tiles = (long long)((R + w - 1) / w) * ((B + c[i].tt - 1) / c[i].tt);
+        for (int S = 1; S <= std::min(8, KB); ++S) {
+            const double floats = (double)S * B * R * (pair ? 2 : 1);
+            if (S > 1 && (tiles * S > c[i].slots || floats > (double)fp8_split_floats(R, pair))) break;
+            if (fs && S != fs) continue;
+            const float rounds = (float)((tiles * S + c[i].slots - 1) / c[i].slots);
+            const float step = tiles * S <= c[i].slots / 2 ? 0.8f * c[i].step : c[i].step;
+            const float us = rounds * step * ((KB + S - 1) / S) + (S > 1 ? 2.0f + (float)(floats * 8 / 3.5e6) : 0.0f);
+            if (us < least) least = us, best = Fp8Plan{c[i].tw, c[i].tt, S};
+        }
+    }
+    return best;
 }
 
 static int fp8_launch_dense(Fp8Gemm a, float *part, hipStream_t st) {

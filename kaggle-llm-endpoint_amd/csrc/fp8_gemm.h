@@ -7,7 +7,7 @@
 namespace mi {
 
 constexpr int kFp8Near = 8;                      // token tiles of a weight tile that run next to each other
-constexpr int kFp8MaxGroups = 1024;              // K / 128: the weight scales of a tile's blocks are kept in LDS
+constexpr int kFp8MaxGroups = 512;              // K / 128: the weight scales of a tile's blocks are kept in LDS
 
 // Memory to LDS without registers: lane l's 16 (4) bytes to dst + 16 l (4 l).
 __device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint4 *dst, uint32_t voff, int soff) {

@@ -42,7 +42,7 @@ def _check(yb, yf, want, bound):
 
 # ------------------------------------------------------------------------------------------------ quantize
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("n,K", [(1, 16), (1, 128), (3, 144), (5, 6144), (67, 1360), (1000, 592), (2, 131072)])
+@pytest.mark.parametrize("n,K", [(1, 16), (1, 128), (3, 144), (5, 6144), (67, 1360), (1000, 592), (2, 65536)])
 def test_quantize(pkg, gpu, n, K, dtype):
     x = _acts(np.random.default_rng(n + K), n, K, dtype)
     q, s = pkg.fp8_quantize(x)

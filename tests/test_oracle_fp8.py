@@ -75,7 +75,7 @@ def test_quantize_refusals(L):
     assert call(x=None) == 1 and call(q=None) == 1 and call(s=None) == 1
     assert call(dt=2) == 8 and call(dt=7) == 8
     assert call(n=0) == 4 and call(n=(1 << 22) + 1) == 4
-    assert call(K=250) == 3 and call(K=0) == 3 and call(K=(1 << 17) + 16) == 3
+    assert call(K=250) == 3 and call(K=0) == 3 and call(K=(1 << 16) + 16) == 3
     assert call(st=240) == 8 and call(st=260) == 8                          # shorter than a row; not whole 8 elements
     assert call(x=P(0x10008)) == 8 and call(q=P(0x20004)) == 8 and call(s=P(0x30002)) == 8
 
@@ -89,7 +89,7 @@ def test_project_refusals(L):
     assert call(dt=2) == 1                                                     # quantised rows without their scales
     assert call(dt=3) == 8
     assert call(B=0) == 4 and call(B=-1) == 4 and call(B=1 << 22, K=4096) == 4
-    assert call(K=248) == 3 and call(R=0) == 3 and call(R=(1 << 17) + 1) == 3
+    assert call(K=248) == 3 and call(R=0) == 3 and call(R=(1 << 16) + 1) == 3
     assert call(x=P(0x10004)) == 8 and call(wq=P(0x20008)) == 8 and call(ws=P(0x30001)) == 8 and call(y=P(0x40001)) == 8
     assert call(w=None) == 5 and call(wb=need - 1) == 5 and call(w=P(0x50008)) == 8
     sizes = [L.mi_fp8_project_workspace(b, 6144, 6144) for b in (1, 2, 8, 16, 17, 32, 33, 64, 100, 128, 200, 512, 1000, 4096)]
