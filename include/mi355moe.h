@@ -474,7 +474,7 @@ size_t mi_fp8_moe_workspace(int32_t T, int32_t k, int32_t E, int32_t D, int32_t 
  * Tokens into expert order and back over mi_ragged_plan's layout (the gather and combine of _apply_ragged_kernel,
  * resident.py:153-165), and their gradients; dtype MI_X_BF16 or MI_X_F32 for every row buffer, D % 8 == 0, rows
  * 16-byte aligned, sums in f32 and in column order, one rounding:
- *   mi_moe_dispatch      xs[r] = x[tok_row[r]], zeros on padding rows (tok_row -1), r < rows
+ *   mi_moe_dispatch      xs[row_slot[t, j]] = x[t], zeros on padding rows (tok_row -1)
  *   mi_moe_combine       out[t] = sum_j w[t, j] y[row_slot[t, j]]; w NULL: weights 1 (dispatch's gradient)
  *   mi_moe_combine_grad  dy[row_slot[t, j]] = w[t, j] dout[t], zeros on padding rows; dw[t, j] = <dout[t], y[row_slot[t, j]]>
  * A slot without a row (row_slot -1) adds nothing and gets dw 0.

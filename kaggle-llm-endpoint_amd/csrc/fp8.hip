@@ -28,13 +28,13 @@ __device__ __forceinline__ void load8(const void *x, size_t at, float v[8]) {
 }
 
 // A group of 128 columns is 16 lanes of 8 values: its maximum is 4 exchanges, its loads and stores are contiguous.
-// Whole groups of lanes run or return together (the grid's tail), so the exchanges stay within live lanes.
+// Whole groups of lanes run or return together (the grid's tail), so the exchanges stay within live lanes.  gi: the
+// group of this lane, over all rows.
 template <int XD>
-__global__ void __launch_bounds__(256) fp8_quantize_kernel(const void *__restrict__ x, int n, int K, long long stride,
-                                                           const int32_t *__restrict__ live, uint8_t *__restrict__ q,
-                                                           float *__restrict__ s) {
+__device__ __forceinline__ void fp8_quantize_group(const void *__restrict__ x, long long gi, int n, int K,
+                                                   long long stride, const int32_t *__restrict__ live,
+                                                   uint8_t *__restrict__ q, float *__restrict__ s) {
     const int KB = fp8_groups(K);
-    const long long gi = ((long long)blockIdx.x * 256 + threadIdx.x) >> 4;
     if (gi >= (long long)n * KB) return;
     const int row = (int)(gi / KB), c = (int)(gi - (long long)row * KB);
     if (live && live[row] < 0) return;           // (the same for the group's 16 lanes)
@@ -63,6 +63,92 @@ __global__ void __launch_bounds__(256) fp8_quantize_kernel(const void *__restric
     }
     if ((threadIdx.x & 15) == 0) s[(size_t)row * KB + c] = exp2_int(e);
 }
+
+template <int XD>
+__global__ void __launch_bounds__(256) fp8_quantize_kernel(const void *__restrict__ x, int n, int K, long long stride,
+                                                           const int32_t *__restrict__ live, uint8_t *__restrict__ q,
+                                                           float *__restrict__ s) {
+    fp8_quantize_group<XD>(x, ((long long)blockIdx.x * 256 + threadIdx.x) >> 4, n, K, stride, live, q, s);
+}
+
+// What the tiled routed layer needs first, in one launch: workgroup 0 gives every slot a row (its expert's blocks of tm
+// rows; rows without a slot get token -1), the others quantise the tokens.  Within an expert the rows are dealt out by LDS
+// atomics: their order is the run's, but a row's result does not depend on its place, so the layer's bits do not either.
+struct Fp8Prepare {
+    const void *x;
+    uint8_t *xq;
+    float *xs;
+    const int32_t *idx;         // [T, k]
+    int32_t *blk_expert, *n_blocks, *tok_row, *row_slot;
+    int T, k, D, E, tm;
+};
+constexpr int kFp8PrepareThreads = 1024;
+
+template <int XD>
+__global__ void __launch_bounds__(kFp8PrepareThreads) fp8_prepare_kernel(Fp8Prepare p) {
+    __shared__ int cnt[kMaxExperts], base[kMaxExperts], wsum[kFp8PrepareThreads / 64], total;
+    const int tid = threadIdx.x;
+    if (blockIdx.x > 0) {
+        fp8_quantize_group<XD>(p.x, ((long long)(blockIdx.x - 1) * kFp8PrepareThreads + tid) >> 4, p.T, p.D, p.D, nullptr,
+                               p.xq, p.xs);
+        return;
+    }
+    const int S = p.T * p.k;
+    cnt[tid] = 0;                                // kMaxExperts == threads
+    __syncthreads();
+    // eight slots at a time, every load issued before its count; a slot's place in its expert waits in row_slot
+    for (int s0 = tid; s0 < S; s0 += 8 * kFp8PrepareThreads) {
+        int e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int s = s0 + j * kFp8PrepareThreads;
+            e[j] = s < S ? p.idx[s] : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int s = s0 + j * kFp8PrepareThreads;
+            if (s < S) p.row_slot[s] = e[j] >= 0 && e[j] < p.E ? atomicAdd(&cnt[e[j]], 1) : -1;
+        }
+    }
+    __syncthreads();
+    const int n = cnt[tid], nb = (n + p.tm - 1) / p.tm;
+    int incl = nb;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(incl, d, 64);
+        if ((tid & 63) >= d) incl += o;
+    }
+    if ((tid & 63) == 63) wsum[tid >> 6] = incl;
+    __syncthreads();
+    for (int w = 0; w < tid >> 6; ++w) incl += wsum[w];
+    base[tid] = (incl - nb) * p.tm;
+    if (tid == kFp8PrepareThreads - 1) *p.n_blocks = incl;
+    for (int b = incl - nb; b < incl; ++b) p.blk_expert[b] = tid;
+    if (tid == kFp8PrepareThreads - 1) total = incl;
+    __syncthreads();
+    for (int r = tid; r < total * p.tm; r += kFp8PrepareThreads) {      // rows behind an expert's last
+        const int e = p.blk_expert[r / p.tm];
+        if (r - base[e] >= cnt[e]) p.tok_row[r] = -1;
+    }
+    for (int s0 = tid; s0 < S; s0 += 8 * kFp8PrepareThreads) {
+        int e[8], at[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int s = s0 + j * kFp8PrepareThreads;
+            e[j] = s < S ? p.idx[s] : -1;
+            at[j] = s < S ? p.row_slot[s] : -1;  // this thread's own store above
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int s = s0 + j * kFp8PrepareThreads;
+            if (at[j] < 0) continue;
+            const int row = base[e[j]] + at[j];
+            p.row_slot[s] = row;
+            p.tok_row[row] = s / p.k;
+        }
+    }
+}
+static_assert(kMaxExperts == kFp8PrepareThreads, "one thread per expert");
 
 // The split sums of gate and up added in split order, then h = silu(min(g, L)) * clip(u, -L, L) in f32, quantised as
 // above: one wavefront per row and group, two values a lane.
@@ -106,19 +192,6 @@ __global__ void __launch_bounds__(256) fp8_reduce_kernel(const float *__restrict
     if (y_bf16) y_bf16[at] = (uint16_t)f32_to_bf16_rne(v);
 }
 
-// Zeros for the rows of blocks that have no product.
-__global__ void __launch_bounds__(256) fp8_zero_blocks_kernel(const int32_t *__restrict__ blk_expert,
-                                                              const int32_t *__restrict__ n_blocks, int E, int tm, int R,
-                                                              uint16_t *y_bf16, float *y_f32) {
-    const int g = blockIdx.x, e = blk_expert[g];
-    if (g < *n_blocks && e >= 0 && e < E) return;
-    const long long n = (long long)tm * R;
-    for (long long at = (long long)blockIdx.y * 256 + threadIdx.x; at < n; at += (long long)gridDim.y * 256) {
-        if (y_f32) y_f32[g * n + at] = 0.0f;
-        if (y_bf16) y_bf16[g * n + at] = 0;
-    }
-}
-
 // out[t] = sum_j w[t, j] * y[r(t, j)], f32, in column order: r the slot's sorted row, or (row_slot NULL) the slot itself.
 // Four outputs a thread, the rows of eight slots loaded before the first is added (D % 16 == 0).
 __global__ void __launch_bounds__(256) fp8_combine_kernel(const float *__restrict__ y, const int32_t *__restrict__ row_slot,
@@ -131,21 +204,22 @@ __global__ void __launch_bounds__(256) fp8_combine_kernel(const float *__restric
     for (int j0 = 0; j0 < k; j0 += 8) {
         float4 v[8];
         float wt[8];
+        bool in[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int s = t * k + min(j0 + j, k - 1), e = idx[s];
             const int r = j0 + j >= k || e < 0 || e >= E ? -1 : row_slot ? row_slot[s] : s;
+            // (no branch around the loads: a slot without a row loads row 0 and adds nothing, whatever that holds)
+            in[j] = r >= 0;
             wt[j] = w[s];
-            v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r >= 0) v[j] = *(const float4 *)(y + (size_t)r * D + c);
-            else wt[j] = 0.0f;
+            v[j] = *(const float4 *)(y + (size_t)max(r, 0) * D + c);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            acc[0] = fmaf(wt[j], v[j].x, acc[0]);
-            acc[1] = fmaf(wt[j], v[j].y, acc[1]);
-            acc[2] = fmaf(wt[j], v[j].z, acc[2]);
-            acc[3] = fmaf(wt[j], v[j].w, acc[3]);
+            acc[0] = in[j] ? fmaf(wt[j], v[j].x, acc[0]) : acc[0];
+            acc[1] = in[j] ? fmaf(wt[j], v[j].y, acc[1]) : acc[1];
+            acc[2] = in[j] ? fmaf(wt[j], v[j].z, acc[2]) : acc[2];
+            acc[3] = in[j] ? fmaf(wt[j], v[j].w, acc[3]) : acc[3];
         }
     }
     const size_t at = (size_t)t * D + c;
@@ -201,7 +275,8 @@ static int fp8_launch_tiled(Fp8Tiled p, hipStream_t st) {
     p.nw = (p.g.R + (PAIR ? TW / 2 : TW) - 1) / (PAIR ? TW / 2 : TW);
     p.nb = (p.g.rows + TT - 1) / TT;
     // ids equal modulo 8 share an XCD and a piece of at most ceil(total / 8) workgroups
-    const long long total = (long long)p.nb * p.nw * p.S, grid = (total + 7) / 8 * 8;
+    // (one more for each XCD where there may be blocks without a product, to write their zeros)
+    const long long total = (long long)p.nb * p.nw * p.S, grid = (total + 7) / 8 * 8 + (p.g.blk_expert && !p.skip ? 8 : 0);
     if (grid >= (1ll << 31) / (64 * WM * WN)) return MI_ERR_TOKENS;
     hipLaunchKernelGGL((fp8_gemm_kernel<TW, TT, WM, WN, NST, PAIR>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, p);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
@@ -522,10 +597,7 @@ extern "C" int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, i
     Fp8Tiled p = {};
     p.g = a;
     p.S = 1;
-    if ((rc = fp8_tiled<false>(p, 256, tm, st)) != MI_OK) return rc;
-    hipLaunchKernelGGL(fp8_zero_blocks_kernel, dim3(n_blk, 8), dim3(256), 0, st, blk_expert, n_blocks, E, tm, R, y_bf16,
-                       y_f32);
-    return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
+    return fp8_tiled<false>(p, 256, tm, st);
 }
 
 namespace mi {
@@ -542,7 +614,7 @@ static int fp8_moe_tile(int S, int E) {
 struct Fp8MoeCut {
     int rows, blocks, tm;
     uint8_t *xq, *hq;
-    float *xs, *hs, *h, *y, *w_row;
+    float *xs, *hs, *h, *y;
     int32_t *blk_expert, *n_blocks, *tok_row, *row_slot;
     size_t bytes;
 };
@@ -568,7 +640,6 @@ static Fp8MoeCut fp8_moe_cut(uint8_t *base, int T, int k, int E, int D, int I) {
     m.blk_expert = c.take<int32_t>(m.blocks);
     m.n_blocks = c.take<int32_t>(1);
     m.tok_row = c.take<int32_t>(m.rows);
-    m.w_row = c.take<float>(m.rows);
     m.row_slot = c.take<int32_t>(S);
     m.hq = c.take<uint8_t>((size_t)m.rows * I);
     m.hs = c.take<float>((size_t)m.rows * fp8_groups(I));
@@ -635,9 +706,13 @@ extern "C" int mi_fp8_moe(const uint8_t *gate_q, const float *gate_s, const uint
         if ((rc = fp8_launch_stream_as<MI_X_F32, 1, 2, false, true, 4, 2, 3>(f, st)) != MI_OK) return rc;
     } else {
         m = fp8_moe_cut((uint8_t *)workspace, T, k, E, D, I);
-        if ((rc = fp8_launch_quantize(x, x_dtype, T, D, D, nullptr, m.xq, m.xs, st)) != MI_OK) return rc;
-        rc = mi_ragged_plan(idx, w, T, k, E, m.tm, m.blk_expert, m.n_blocks, m.tok_row, m.w_row, m.row_slot, stream);
-        if (rc != MI_OK) return rc;
+        const Fp8Prepare f = {x, m.xq, m.xs, idx, m.blk_expert, m.n_blocks, m.tok_row, m.row_slot, T, k, D, E, m.tm};
+        const dim3 grid((unsigned)(1 + ((long long)T * fp8_groups(D) * 16 + kFp8PrepareThreads - 1) / kFp8PrepareThreads));
+        if (x_dtype == MI_X_BF16)
+            hipLaunchKernelGGL(fp8_prepare_kernel<MI_X_BF16>, grid, dim3(kFp8PrepareThreads), 0, st, f);
+        else
+            hipLaunchKernelGGL(fp8_prepare_kernel<MI_X_F32>, grid, dim3(kFp8PrepareThreads), 0, st, f);
+        if (hipGetLastError() != hipSuccess) return MI_ERR_LAUNCH;
         Fp8Tiled p = {};
         Fp8Gemm &a = p.g;
         a.xq = m.xq, a.xs = m.xs;

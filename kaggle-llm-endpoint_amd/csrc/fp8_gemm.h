@@ -50,8 +50,25 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     const int nb = a.n_blocks ? min(max(*a.n_blocks, 0), p.nb) : p.nb;
     const long long total = (long long)nb * p.nw * p.S;
     const int xcd = blockIdx.x & 7, li = blockIdx.x >> 3;
-    const long long first = total * xcd / 8, at = first + li;
-    if (at >= total * (xcd + 1) / 8) return;
+    const long long first = total * xcd / 8, at = first + li, end = total * (xcd + 1) / 8;
+    // the zeros of one 256-output piece of a block that has no product
+    auto zero = [&](int blk, int w) {
+        const int o1 = w * TW;
+        for (int r = wave; r < TT && blk * TT + r < a.rows; r += W)
+            for (int o = o1 + lane; o < min(o1 + TW, a.R); o += 64) {
+                const size_t n = (size_t)(blk * TT + r) * a.R + o;
+                if (a.y_f32) a.y_f32[n] = 0.0f;
+                if (a.y_bf16) a.y_bf16[n] = 0;
+            }
+    };
+    if (at >= end) {
+        // this workgroup has none: the blocks behind the last one in use are dealt out to those that every XCD has over
+        const int over = (int)(gridDim.x >> 3) - (int)((total + 7) / 8), z = (int)(at - end);
+        if (PAIR || p.skip || !a.blk_expert || z >= over) return;
+        const long long dead = (long long)(p.nb - nb) * p.nw;
+        for (long long d = z * 8 + xcd; d < dead; d += over * 8) zero(nb + (int)(d / p.nw), (int)(d % p.nw));
+        return;
+    }
     const int per = kFp8Near * p.nw * p.S;
     const int pr = (int)(at / per), in = (int)(at - (long long)pr * per);
     const int width = min(kFp8Near, nb - kFp8Near * pr);
@@ -62,7 +79,10 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     int e = 0;
     if (a.blk_expert) {
         e = a.blk_expert[tb];
-        if (e < 0 || e >= a.E) return;           // the whole workgroup
+        if (e < 0 || e >= a.E) {                 // the whole workgroup
+            if (!PAIR && !p.skip) zero(tb, wt);
+            return;
+        }
     }
     const int t0 = split * KB / p.S, t1 = (split + 1) * KB / p.S;
 
