@@ -428,7 +428,8 @@ int mi_fp8_quantize(const void *x, int32_t x_dtype, int32_t n, int32_t K, int64_
 /*
  * Dense block-scaled product, 1 <= B tokens: x bf16 or f32 [B, n_in] (quantised as by mi_fp8_quantize; xs NULL) or
  * MI_X_FP8 values with their scales xs.  y_bf16 (one rounding of the f32 sum) and/or y_f32 [B, n_out], any n_out.
- * Workspace: mi_fp8_project_workspace bytes, 16-byte aligned, no initialisation; its size serves every smaller B.
+ * Workspace: mi_fp8_project_workspace bytes, 16-byte aligned, no initialisation; its size serves every smaller B.  Up to
+ * 32 rows need none (the size is 0, as for a shape that the call refuses).
  */
 int mi_fp8_project(const void *x, int32_t x_dtype, const float *xs, int32_t B, const uint8_t *wq, const float *ws,
                    int32_t n_in, int32_t n_out, uint16_t *y_bf16, float *y_f32, void *workspace,

@@ -470,8 +470,7 @@ extern "C" int mi_fp8_quantize(const void *x, int32_t x_dtype, int32_t n, int32_
 extern "C" size_t mi_fp8_project_workspace(int32_t B, int32_t n_in, int32_t n_out) {
     if (B <= 0 || B > kFp8MaxRows || !fp8_cols_ok(n_in) || !fp8_rows_ok(n_out) || (long long)B * n_in >= (1ll << 31))
         return 0;
-    // (the streaming kernels need none; 256 bytes keep an allocation from being empty)
-    return B <= kFp8StreamRows ? 256 : fp8_row_bytes(B, n_in) + up256(fp8_split_floats(n_out, false) * sizeof(float));
+    return B <= kFp8StreamRows ? 0 : fp8_row_bytes(B, n_in) + up256(fp8_split_floats(n_out, false) * sizeof(float));
 }
 
 extern "C" int mi_fp8_project(const void *x, int32_t x_dtype, const float *xs, int32_t B, const uint8_t *wq,
@@ -482,7 +481,8 @@ extern "C" int mi_fp8_project(const void *x, int32_t x_dtype, const float *xs, i
     if (rc != MI_OK) return rc;
     if (!y_bf16 && !y_f32) return MI_ERR_NULL;
     if (!fp8_y_ok(y_bf16, y_f32)) return MI_ERR_ARG;
-    if (!workspace || workspace_bytes < mi_fp8_project_workspace(B, n_in, n_out)) return MI_ERR_WORKSPACE;
+    const size_t need = mi_fp8_project_workspace(B, n_in, n_out);
+    if (need && (!workspace || workspace_bytes < need)) return MI_ERR_WORKSPACE;
     if (!aligned16(workspace)) return MI_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
     if (B <= kFp8StreamRows) {

@@ -50,10 +50,12 @@ constexpr int kPadRows = 16;                     // rows that one of the padding
 template <int XD>
 __device__ __forceinline__ void zero_padding(const int32_t *__restrict__ tok_row, int blk, int T, int D, int rows, void *out) {
     const Row8<XD> zero = {};
-    for (int r = blk * kPadRows; r < min((blk + 1) * kPadRows, rows); ++r) {
-        const int t = tok_row[r];
-        if (t >= 0 && t < T) continue;
-        for (int c = threadIdx.x * 8; c < D; c += 2048) zero.store(out, (size_t)r * D + c);
+    const int r0 = blk * kPadRows, n = min(kPadRows, rows - r0);
+    const int t = tok_row[r0 + min((int)threadIdx.x % kPadRows, n - 1)];
+    const uint64_t none = __ballot(t < 0 || t >= T);               // bits 0 .. kPadRows - 1: this workgroup's rows
+    for (int j = 0; j < n; ++j) {
+        if (!((none >> j) & 1)) continue;
+        for (int c = threadIdx.x * 8; c < D; c += 2048) zero.store(out, (size_t)(r0 + j) * D + c);
     }
 }
 

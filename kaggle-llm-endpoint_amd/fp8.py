@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .resident import _as, _ptr, _stream
+from .resident import _as, _ptr
 
 BLOCK = 128                     # columns per activation scale; rows and columns per weight scale
 FP8 = torch.float8_e4m3fn
@@ -43,32 +43,35 @@ def fp8_leaf(leaf, device="cuda"):
 
 
 def _leaf_dims(leaf, who):
-    """(E, n_out, n_in) of an Fp8Leaf, its types and shapes checked."""
+    """(E, n_out, n_in) of an Fp8Leaf, its types and shapes checked; E is 0 for one matrix."""
     q, s = leaf
-    if q.dtype != FP8 or s.dtype != torch.float32:
+    qs, ss = q.shape, s.shape
+    n = len(qs)
+    if q.dtype is not FP8 or s.dtype is not torch.float32:
         raise TypeError("%s: weights are float8_e4m3fn with float32 scales (got %s, %s)" % (who, q.dtype, s.dtype))
-    if q.dim() not in (2, 3) or s.dim() != q.dim():
+    if n not in (2, 3) or len(ss) != n:
         raise ValueError("%s: weights are [n_out, n_in] or [E, n_out, n_in], scales likewise" % who)
-    R, K = q.shape[-2:]
-    if tuple(s.shape) != tuple(q.shape[:-2]) + (_blocks(R), _blocks(K)):
-        raise ValueError("%s: scales %s do not fit weights %s: one per 128 x 128 block" % (who, tuple(s.shape),
-                                                                                           tuple(q.shape)))
+    R, K = qs[n - 2], qs[n - 1]
+    E = qs[0] if n == 3 else 0
+    if ss[n - 2] != -(-R // BLOCK) or ss[n - 1] != -(-K // BLOCK) or (E and ss[0] != E):
+        raise ValueError("%s: scales %s do not fit weights %s: one per 128 x 128 block" % (who, tuple(ss), tuple(qs)))
     if not (q.is_contiguous() and s.is_contiguous()):
         raise ValueError("%s: weights and scales must be contiguous (fp8_leaf makes them so)" % who)
-    return (q.shape[0] if q.dim() == 3 else 1), R, K
+    return E, R, K
 
 
-def _one_device(who, *tensors):
-    """Every tensor on the current device: the call runs on that device's stream."""
+def _stream_of(who, *tensors):
+    """The current stream; every tensor has to be on the current device, whose stream the call runs on."""
     dev = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError("%s: every tensor must be on the current device (cuda:%d), got one on %s" % (who, dev,
                                                                                                        t.device))
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _no_grad(who, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_grad(who, t):
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("%s has no gradient: detach its inputs or call it under torch.no_grad()" % who)
 
 
@@ -87,40 +90,40 @@ def _out(t, shape, dtype, who, device):
     return t
 
 
-def _workspace(workspace, need, who, device):
-    # without one, the call's own: a kept buffer would be shared by two captured calls
-    if need == 0:
-        raise ValueError("%s: unsupported shape" % who)
+def _workspace(workspace, need, device):
+    """(tensor, address, bytes) of a call's workspace: the caller's, or the call's own, since two captured calls would
+    share a kept one (the caller of this holds the tensor until its launches are queued).  need 0: none (or a shape that
+    the call refuses)."""
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device)
-    return workspace
+        if need == 0:
+            return None, None, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
-class _Rows(NamedTuple):
-    x: torch.Tensor
-    xs: object
-    dtype: int
+_DTYPES = {torch.bfloat16: _lib.MI_X_BF16, torch.float32: _lib.MI_X_F32}
 
 
 def _rows_of(x, K, who):
-    """Activations of a product: bf16 or f32 [B, K], or the pair (q, s) of fp8_quantize."""
+    """(rows, scales or None, dtype code) of a product's activations: bf16 or f32 [B, K], or fp8_quantize's pair."""
     if isinstance(x, (tuple, list)):
         q, s = x
         if q.dtype != FP8 or s.dtype != torch.float32:
             raise TypeError("%s: quantised activations are (float8_e4m3fn, float32 scales)" % who)
         if q.dim() != 2 or tuple(s.shape) != (q.shape[0], _blocks(q.shape[1])):
             raise ValueError("%s: quantised activations are q [B, n_in] with s [B, ceil(n_in / 128)]" % who)
-        r = _Rows(_aligned(q), s.contiguous(), _lib.MI_X_FP8)
+        x, xs, dtype = _aligned(q), s.contiguous(), _lib.MI_X_FP8
     else:
-        if x.dtype not in (torch.bfloat16, torch.float32):
+        xs, dtype = None, _DTYPES.get(x.dtype)
+        if dtype is None:
             raise TypeError("%s: activations are bf16 or f32 (or fp8_quantize's pair), got %s" % (who, x.dtype))
         if x.dim() != 2:
             raise ValueError("%s: activations are [B, n_in]" % who)
         _no_grad(who, x)
-        r = _Rows(_aligned(x), None, _lib.MI_X_BF16 if x.dtype == torch.bfloat16 else _lib.MI_X_F32)
-    if r.x.shape[1] != K:
-        raise ValueError("%s: activations have %d columns, the weight %d" % (who, r.x.shape[1], K))
-    return r
+        x = _aligned(x)
+    if x.shape[1] != K:
+        raise ValueError("%s: activations have %d columns, the weight %d" % (who, x.shape[1], K))
+    return x, xs, dtype
 
 
 def fp8_quantize(x, q=None, s=None):
@@ -128,24 +131,29 @@ def fp8_quantize(x, q=None, s=None):
     group of 128 columns s = 2^e, the least e >= -100 with max |x| <= 448 * 2^e over the group's finite values, and
     q = x / s to nearest even; infinities and NaN become NaN.  A power of two, so that x / s is exact and each value is
     rounded once.  Rows may be strided.  ``q`` and ``s``: outputs to write into."""
-    if x.dtype not in (torch.bfloat16, torch.float32):
+    dtype, shape = _DTYPES.get(x.dtype), x.shape
+    if dtype is None:
         raise TypeError("fp8_quantize: x must be bf16 or f32, got %s" % x.dtype)
-    if x.dim() < 1:
+    if not shape:
         raise ValueError("fp8_quantize: x must have at least one dimension")
     _no_grad("fp8_quantize", x)
-    K = x.shape[-1]
-    q = _out(q, x.shape, FP8, "fp8_quantize", x.device)
-    s = _out(s, x.shape[:-1] + (_blocks(K),), torch.float32, "fp8_quantize", x.device)
-    if x.numel() == 0:
+    K = shape[-1]
+    q = _out(q, shape, FP8, "fp8_quantize", x.device)
+    s = _out(s, shape[:-1] + (_blocks(K),), torch.float32, "fp8_quantize", x.device)
+    size = x.numel()
+    if size == 0:
         return q, s
-    _one_device("fp8_quantize", x, q, s)
-    n = x.numel() // K
-    x2 = x if x.dim() == 2 else x.reshape(n, K)
-    if x2.stride(1) != 1 or x2.stride(0) < K or x2.stride(0) % 8 or x2.data_ptr() % 16:
+    stream = _stream_of("fp8_quantize", x, q, s)
+    n = size // K
+    x2 = x if len(shape) == 2 else x.reshape(n, K)
+    if x2.is_contiguous():
+        stride = -(-K // 8) * 8 if n == 1 else K
         x2 = _aligned(x2)
-    check("mi_fp8_quantize", lib().mi_fp8_quantize(_ptr(x2), _lib.MI_X_BF16 if x.dtype == torch.bfloat16
-                                                   else _lib.MI_X_F32, n, K, x2.stride(0) if n > 1 else -(-K // 8) * 8,
-                                                   _ptr(q), _ptr(s), _stream()))
+    else:
+        stride = x2.stride(0)
+        if x2.stride(1) != 1 or stride < K or stride % 8 or x2.data_ptr() % 16:
+            x2, stride = _aligned(x2), K
+    check("mi_fp8_quantize", lib().mi_fp8_quantize(x2.data_ptr(), dtype, n, K, stride, q.data_ptr(), s.data_ptr(), stream))
     return q, s
 
 
@@ -155,17 +163,17 @@ def fp8_project(x, leaf, want_f32=False, y_bf16=None, y_f32=None, workspace=None
     (and y f32 with want_f32).  Preallocated outputs and ``workspace`` (uint8, mi_fp8_project_workspace bytes, needs no
     initialisation) make the call allocation-free."""
     E, R, K = _leaf_dims(leaf, "fp8_project")
-    if leaf.q.dim() != 2:
+    if E:
         raise ValueError("fp8_project: the weight must be one matrix [n_out, n_in]")
-    r = _rows_of(x, K, "fp8_project")
-    B = r.x.shape[0]
-    yb = _out(y_bf16, (B, R), torch.bfloat16, "fp8_project", r.x.device)
-    yf = _out(y_f32, (B, R), torch.float32, "fp8_project", r.x.device) if want_f32 or y_f32 is not None else None
+    x, xs, dtype = _rows_of(x, K, "fp8_project")
+    B = x.shape[0]
+    yb = _out(y_bf16, (B, R), torch.bfloat16, "fp8_project", x.device)
+    yf = _out(y_f32, (B, R), torch.float32, "fp8_project", x.device) if want_f32 or y_f32 is not None else None
     if B:
-        _one_device("fp8_project", r.x, r.xs, leaf.q, leaf.s, yb, yf, workspace)
-        ws = _workspace(workspace, lib().mi_fp8_project_workspace(B, K, R), "fp8_project", r.x.device)
-        check("mi_fp8_project", lib().mi_fp8_project(_ptr(r.x), r.dtype, _ptr(r.xs), B, _ptr(leaf.q), _ptr(leaf.s), K, R,
-                                                     _ptr(yb), _ptr(yf), _ptr(ws), ws.numel(), _stream()))
+        stream = _stream_of("fp8_project", x, xs, leaf.q, leaf.s, yb, yf, workspace)
+        held, ws, nbytes = _workspace(workspace, lib().mi_fp8_project_workspace(B, K, R), x.device)
+        check("mi_fp8_project", lib().mi_fp8_project(x.data_ptr(), dtype, _ptr(xs), B, _ptr(leaf.q), _ptr(leaf.s), K, R,
+                                                     _ptr(yb), _ptr(yf), ws, nbytes, stream))
     return (yb, yf) if want_f32 else yb
 
 
@@ -183,18 +191,18 @@ def fp8_mlp(x, gate, up, down, limit, want_f32=False, y_bf16=None, y_f32=None, w
     gate, up [I, D], down [D, I].  -> y bf16 [B, D] (and y f32 with want_f32).  Preallocated outputs and ``workspace``
     (mi_fp8_mlp_workspace bytes) make the call allocation-free."""
     E, I, D = _mlp_dims(gate, up, down, "fp8_mlp")
-    if gate.q.dim() != 2:
+    if E:
         raise ValueError("fp8_mlp: gate, up and down are one matrix each")
-    r = _rows_of(x, D, "fp8_mlp")
-    B = r.x.shape[0]
-    yb = _out(y_bf16, (B, D), torch.bfloat16, "fp8_mlp", r.x.device)
-    yf = _out(y_f32, (B, D), torch.float32, "fp8_mlp", r.x.device) if want_f32 or y_f32 is not None else None
+    x, xs, dtype = _rows_of(x, D, "fp8_mlp")
+    B = x.shape[0]
+    yb = _out(y_bf16, (B, D), torch.bfloat16, "fp8_mlp", x.device)
+    yf = _out(y_f32, (B, D), torch.float32, "fp8_mlp", x.device) if want_f32 or y_f32 is not None else None
     if B:
-        _one_device("fp8_mlp", r.x, r.xs, *gate, *up, *down, yb, yf, workspace)
-        ws = _workspace(workspace, lib().mi_fp8_mlp_workspace(B, D, I), "fp8_mlp", r.x.device)
-        check("mi_fp8_mlp", lib().mi_fp8_mlp(_ptr(r.x), r.dtype, _ptr(r.xs), B, D, I, _ptr(gate.q), _ptr(gate.s),
+        stream = _stream_of("fp8_mlp", x, xs, *gate, *up, *down, yb, yf, workspace)
+        held, ws, nbytes = _workspace(workspace, lib().mi_fp8_mlp_workspace(B, D, I), x.device)
+        check("mi_fp8_mlp", lib().mi_fp8_mlp(x.data_ptr(), dtype, _ptr(xs), B, D, I, _ptr(gate.q), _ptr(gate.s),
                                              _ptr(up.q), _ptr(up.s), _ptr(down.q), _ptr(down.s), float(limit), _ptr(yb),
-                                             _ptr(yf), _ptr(ws), ws.numel(), _stream()))
+                                             _ptr(yf), ws, nbytes, stream))
     return (yb, yf) if want_f32 else yb
 
 
@@ -203,20 +211,19 @@ def fp8_grouped(xs, plan, leaf, want_f32=False, y_bf16=None, y_f32=None, workspa
     bf16 or f32 [Rp, K] (moe_dispatch's rows) or fp8_quantize's pair -> y bf16 [Rp, R] (and y f32 with want_f32), ready
     for moe_combine.  Rows of blocks that the plan does not use, and padding rows, are zero."""
     E, R, K = _leaf_dims(leaf, "fp8_grouped")
-    if leaf.q.dim() != 3:
+    if not E:
         raise ValueError("fp8_grouped: the weights must be [E, R, K]")
-    r = _rows_of(xs, K, "fp8_grouped")
+    x, xs, dtype = _rows_of(xs, K, "fp8_grouped")
     blk, nb, tok = [_as(plan[k], torch.int32) for k in ("blk_expert", "n_blocks", "tok_row")]
-    rows, G = r.x.shape[0], blk.numel()
+    rows, G = x.shape[0], blk.numel()
     if rows != tok.numel() or nb.numel() != 1 or G == 0 or rows % G:
         raise ValueError("fp8_grouped: %d rows do not fit the plan's %d rows in %d blocks" % (rows, tok.numel(), G))
-    yb = _out(y_bf16, (rows, R), torch.bfloat16, "fp8_grouped", r.x.device)
-    yf = _out(y_f32, (rows, R), torch.float32, "fp8_grouped", r.x.device) if want_f32 or y_f32 is not None else None
-    _one_device("fp8_grouped", r.x, r.xs, blk, nb, tok, leaf.q, leaf.s, yb, yf, workspace)
-    ws = _workspace(workspace, lib().mi_fp8_grouped_workspace(rows, K, R), "fp8_grouped", r.x.device)
-    check("mi_fp8_grouped", lib().mi_fp8_grouped(_ptr(r.x), r.dtype, _ptr(r.xs), G, rows // G, _ptr(blk), _ptr(nb),
-                                                 _ptr(tok), _ptr(leaf.q), _ptr(leaf.s), E, K, R, _ptr(yb), _ptr(yf), _ptr(ws),
-                                                 ws.numel(), _stream()))
+    yb = _out(y_bf16, (rows, R), torch.bfloat16, "fp8_grouped", x.device)
+    yf = _out(y_f32, (rows, R), torch.float32, "fp8_grouped", x.device) if want_f32 or y_f32 is not None else None
+    stream = _stream_of("fp8_grouped", x, xs, blk, nb, tok, leaf.q, leaf.s, yb, yf, workspace)
+    held, ws, nbytes = _workspace(workspace, lib().mi_fp8_grouped_workspace(rows, K, R), x.device)
+    check("mi_fp8_grouped", lib().mi_fp8_grouped(x.data_ptr(), dtype, _ptr(xs), G, rows // G, _ptr(blk), _ptr(nb),
+                                                 _ptr(tok), _ptr(leaf.q), _ptr(leaf.s), E, K, R, _ptr(yb), _ptr(yf), ws, nbytes, stream))
     return (yb, yf) if want_f32 else yb
 
 
@@ -228,25 +235,25 @@ def fp8_moe(gate, up, down, x, idx, w, limit, want_f32=True, want_bf16=False, ou
     (out_f32 [T, D] or None, out_bf16 [T, D] or None).  A slot whose expert id is outside [0, E) adds nothing.
     Preallocated outputs and ``workspace`` (mi_fp8_moe_workspace bytes) make the call allocation-free."""
     E, I, D = _mlp_dims(gate, up, down, "fp8_moe")
-    if gate.q.dim() != 3:
+    if not E:
         raise ValueError("fp8_moe: gate, up and down must be [E, ..] experts")
     if isinstance(x, (tuple, list)):
         raise TypeError("fp8_moe: activations are bf16 or f32")
-    r = _rows_of(x, D, "fp8_moe")
-    if idx.dim() != 2 or w.shape != idx.shape or idx.shape[0] != r.x.shape[0]:
-        raise ValueError("fp8_moe: idx and w must be [T, k] for the %d tokens of x" % r.x.shape[0])
+    x, _, dtype = _rows_of(x, D, "fp8_moe")
+    if idx.dim() != 2 or w.shape != idx.shape or idx.shape[0] != x.shape[0]:
+        raise ValueError("fp8_moe: idx and w must be [T, k] for the %d tokens of x" % x.shape[0])
     _no_grad("fp8_moe", w)
     idx, w = _as(idx, torch.int32), _as(w, torch.float32)
     T, k = idx.shape
     of, ob = out_f32, out_bf16
     if of is not None or want_f32:
-        of = _out(of, (T, D), torch.float32, "fp8_moe", r.x.device)
+        of = _out(of, (T, D), torch.float32, "fp8_moe", x.device)
     if ob is not None or want_bf16:
-        ob = _out(ob, (T, D), torch.bfloat16, "fp8_moe", r.x.device)
+        ob = _out(ob, (T, D), torch.bfloat16, "fp8_moe", x.device)
     if T:
-        _one_device("fp8_moe", r.x, idx, w, *gate, *up, *down, of, ob, workspace)
-        ws = _workspace(workspace, lib().mi_fp8_moe_workspace(T, k, E, D, I), "fp8_moe", r.x.device)
+        stream = _stream_of("fp8_moe", x, idx, w, *gate, *up, *down, of, ob, workspace)
+        held, ws, nbytes = _workspace(workspace, lib().mi_fp8_moe_workspace(T, k, E, D, I), x.device)
         check("mi_fp8_moe", lib().mi_fp8_moe(_ptr(gate.q), _ptr(gate.s), _ptr(up.q), _ptr(up.s), _ptr(down.q),
-                                             _ptr(down.s), E, D, I, _ptr(r.x), r.dtype, T, k, _ptr(idx), _ptr(w),
-                                             float(limit), _ptr(of), _ptr(ob), _ptr(ws), ws.numel(), _stream()))
+                                             _ptr(down.s), E, D, I, x.data_ptr(), dtype, T, k, _ptr(idx), _ptr(w),
+                                             float(limit), _ptr(of), _ptr(ob), ws, nbytes, stream))
     return of, ob

@@ -11,12 +11,9 @@ forward's own inputs.  Deterministic: no atomics, sums in f32 in column order, o
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib
 from ._lib import check, lib
-from .fp8 import _aligned, _one_device
+from .fp8 import _DTYPES, _aligned, _stream_of
 from .resident import _as, _ptr, _stream
-
-_DTYPES = {torch.bfloat16: _lib.MI_X_BF16, torch.float32: _lib.MI_X_F32}
 
 
 def _rows_dtype(t, who):
@@ -24,7 +21,6 @@ def _rows_dtype(t, who):
         raise TypeError("%s: rows are bf16 or f32, got %s" % (who, t.dtype))
     if t.dim() != 2:
         raise ValueError("%s: rows are [n, D]" % who)
-    return _DTYPES[t.dtype]
 
 
 def _plan_rows(plan):
@@ -35,7 +31,15 @@ def _plan_rows(plan):
     return tok, slot
 
 
-def _combine(y, slot, w, who):
+def _dispatch(x, tok, slot):
+    xs = torch.empty((tok.numel(), x.shape[1]), dtype=x.dtype, device=x.device)
+    T, k = slot.shape
+    check("mi_moe_dispatch", lib().mi_moe_dispatch(_ptr(x), _DTYPES[x.dtype], T, k, x.shape[1], _ptr(slot), _ptr(tok),
+                                                   tok.numel(), _ptr(xs), _stream()))
+    return xs
+
+
+def _combine(y, slot, w):
     T, k = slot.shape
     out = torch.empty((T, y.shape[1]), dtype=y.dtype, device=y.device)
     check("mi_moe_combine", lib().mi_moe_combine(_ptr(y), _DTYPES[y.dtype], T, k, y.shape[1], _ptr(slot), _ptr(w),
@@ -47,24 +51,20 @@ class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tok, slot):
         ctx.save_for_backward(slot)
-        xs = torch.empty((tok.numel(), x.shape[1]), dtype=x.dtype, device=x.device)
-        T, k = slot.shape
-        check("mi_moe_dispatch", lib().mi_moe_dispatch(_ptr(x), _DTYPES[x.dtype], T, k, x.shape[1], _ptr(slot), _ptr(tok),
-                                                       tok.numel(), _ptr(xs), _stream()))
-        return xs
+        return _dispatch(x, tok, slot)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gxs):
         slot, = ctx.saved_tensors
-        return _combine(_aligned(gxs), slot, None, "moe_dispatch"), None, None
+        return _combine(_aligned(gxs), slot, None), None, None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, w, tok, slot):
         ctx.save_for_backward(y, w, tok, slot)
-        return _combine(y, slot, w, "moe_combine")
+        return _combine(y, slot, w)
 
     @staticmethod
     @once_differentiable
@@ -87,8 +87,11 @@ def moe_dispatch(x, plan):
     tok, slot = _plan_rows(plan)
     if slot.shape[0] != x.shape[0]:
         raise ValueError("moe_dispatch: the plan is of %d tokens, x has %d" % (slot.shape[0], x.shape[0]))
-    _one_device("moe_dispatch", x, tok, slot)
-    return _Dispatch.apply(_aligned(x), tok, slot)
+    _stream_of("moe_dispatch", x, tok, slot)
+    x = _aligned(x)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Dispatch.apply(x, tok, slot)
+    return _dispatch(x, tok, slot)
 
 
 def moe_combine(y, plan, w):
@@ -101,5 +104,8 @@ def moe_combine(y, plan, w):
         raise ValueError("moe_combine: the plan has %d rows, y %d" % (tok.numel(), y.shape[0]))
     if w.dtype != torch.float32 or w.shape != slot.shape:
         raise ValueError("moe_combine: w must be float32 %s" % (tuple(slot.shape),))
-    _one_device("moe_combine", y, w, tok, slot)
-    return _Combine.apply(_aligned(y), w.contiguous(), tok, slot)
+    _stream_of("moe_combine", y, w, tok, slot)
+    y, w = _aligned(y), w.contiguous()
+    if (y.requires_grad or w.requires_grad) and torch.is_grad_enabled():
+        return _Combine.apply(y, w, tok, slot)
+    return _combine(y, slot, w)

@@ -81,9 +81,9 @@ def test_quantize_refusals(L):
 
 
 def test_project_refusals(L):
-    need = L.mi_fp8_project_workspace(5, 256, 100)
-    assert need > 0
-    call = lambda x=X, dt=0, xs=None, B=5, wq=Q, ws=S, K=256, R=100, y=Y, yf=None, w=WS, wb=BIG: L.mi_fp8_project(
+    need = L.mi_fp8_project_workspace(40, 256, 100)
+    assert need > 0 and L.mi_fp8_project_workspace(32, 256, 100) == 0        # few rows need no workspace
+    call = lambda x=X, dt=0, xs=None, B=40, wq=Q, ws=S, K=256, R=100, y=Y, yf=None, w=WS, wb=BIG: L.mi_fp8_project(
         x, dt, xs, B, wq, ws, K, R, y, yf, w, wb, None)
     assert call(x=None) == 1 and call(wq=None) == 1 and call(ws=None) == 1 and call(y=None) == 1
     assert call(dt=2) == 1                                                     # quantised rows without their scales
@@ -205,3 +205,48 @@ def test_python_refusals(pkg):
         pkg.moe_combine(torch.zeros(63, 64), plan, torch.zeros(5, 2))
     with pytest.raises(ValueError, match="w must be"):
         pkg.moe_combine(torch.zeros(64, 64), plan, torch.zeros(5, 3))
+
+
+# ------------------------------------------------------------------------------------------------ a call's own scratch
+class _Lib:
+    """Stands for the library: notes the scratch of every call, and has a second call arrive within the first."""
+
+    def __init__(self, name, arg):
+        self.name, self.arg, self.seen, self.again = name, arg, [], None
+
+    def __getattr__(self, attr):
+        if attr == self.name:
+            return self._call
+        if attr == self.name + "_workspace":
+            return lambda *a: 1 << 16
+        raise AttributeError(attr)
+
+    def _call(self, *args):
+        self.seen.append(args[self.arg])
+        if self.again is not None:
+            again, self.again = self.again, None
+            again()
+        return 0
+
+
+@pytest.mark.parametrize("name,arg", [("mi_fp8_project", 10), ("mi_fp8_mlp", 15), ("mi_fp8_moe", 18),
+                                      ("mi_fp8_grouped", 14)])
+def test_a_call_within_a_call_has_other_scratch(pkg, monkeypatch, name, arg):
+    """The scratch that a call's launches hand each other is held until they are queued: a call from another host thread
+    in between must not be given the same memory."""
+    fake = _Lib(name, arg)
+    monkeypatch.setattr(pkg.fp8, "lib", lambda: fake)
+    monkeypatch.setattr(pkg.fp8, "_stream_of", lambda *a: 0)
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
+    g, d = _leaf(pkg, 144, 256, 3), _leaf(pkg, 256, 144, 3)
+    one = [pkg.Fp8Leaf(l.q[0], l.s[0]) for l in (g, g, d)]
+    plan = {"blk_expert": torch.zeros(4, dtype=torch.int32), "n_blocks": torch.ones(1, dtype=torch.int32),
+            "tok_row": torch.zeros(64, dtype=torch.int32), "row_slot": torch.zeros((5, 2), dtype=torch.int32)}
+    call = {"mi_fp8_project": lambda: pkg.fp8_project(bf(40, 256), one[0]),
+            "mi_fp8_mlp": lambda: pkg.fp8_mlp(bf(40, 256), *one, 7.0),
+            "mi_fp8_moe": lambda: pkg.fp8_moe(g, g, d, bf(4, 256), torch.zeros((4, 2), dtype=torch.int32),
+                                              torch.zeros(4, 2), 7.0),
+            "mi_fp8_grouped": lambda: pkg.fp8_grouped(bf(64, 256), plan, g)}[name]
+    fake.again = call
+    call()
+    assert len(fake.seen) == 2 and fake.seen[0] != fake.seen[1]
