@@ -230,7 +230,7 @@ class _Lib:
 
 
 @pytest.mark.parametrize("name,arg", [("mi_fp8_project", 10), ("mi_fp8_mlp", 15), ("mi_fp8_moe", 18),
-                                      ("mi_fp8_grouped", 14)])
+                                      ("mi_fp8_grouped", 15)])
 def test_a_call_within_a_call_has_other_scratch(pkg, monkeypatch, name, arg):
     """The scratch that a call's launches hand each other is held until they are queued: a call from another host thread
     in between must not be given the same memory."""
