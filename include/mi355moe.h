@@ -495,7 +495,8 @@ int mi_moe_combine_grad(const void *dout, const void *y, int32_t dtype, int32_t 
  * split counts and row tiles of the decode launch families (S1, S2, FS1, FS2, SMV, each with _RTW and _AL; MS1, MS2,
  * CS1, CS2 with _RTW; MGMAX), launch-family switches (CUSTREAM, CUMULTI, PERSIST_ABOVE, FUSE_SWIGLU, CU_FORM_H), the
  * one-launch decode's poll limit (SPIN_LIMIT), the int8 split plan (I8S, I8_WAVES, I8_FUSE) and the many-token MLP's
- * splits and token tile (DG_S1, DG_S2, DG_NT) and the prefill's wide blocks (PF_WIDE).  Overrides change
+ * splits and token tile (DG_S1, DG_S2, DG_NT), the prefill's wide blocks (PF_WIDE), the dense fp8 product's tile and
+ * splits (F8_TW, F8_TT, F8_S) and the fp8 routed layer's streaming limit and rows per block (F8_STREAM, F8_TM).  Overrides change
  * launch shapes and summation orders, never the result beyond f32 rounding; workspace sizes follow them, so set them
  * before sizing a workspace.  Not synchronised with calls running on other host threads.
  */

@@ -309,12 +309,14 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         const int row = row0 + trow(t) + i;
-        if (row >= a.rows || (p.skip && a.live[row] < 0)) continue;
+        if (row >= a.rows) continue;
+        const bool dead = a.live && a.live[row] < 0;
+        if (dead && p.skip) continue;
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int m = PAIR ? r / (RT / 2) : 0;
             const int o = o0 + (PAIR ? wrow(r) - m * (TW / 2) : wrow(r)) + 4 * q;
-            const f32x4 v = acc[r][t];
+            const f32x4 v = dead ? (f32x4){0.f, 0.f, 0.f, 0.f} : acc[r][t];   // (0 times a NaN weight is not 0)
             float *f = p.S > 1 ? p.part[m] + (size_t)split * a.rows * a.R : a.y_f32;
             if (f) {
                 f += (size_t)row * a.R + o;

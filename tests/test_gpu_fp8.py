@@ -166,6 +166,26 @@ def test_project_extremes(pkg, gpu, B):
         assert (yf[3] == 0).all()
 
 
+TILES = [(128, 64), (128, 128), (256, 64), (256, 128), (256, 256)]
+
+
+@pytest.mark.parametrize("tw,tt", TILES)
+@pytest.mark.parametrize("B,K,R", [(33, 144, 20), (64, 1040, 300), (200, 640, 515), (270, 128, 128), (530, 272, 272)])
+def test_project_every_tile(pkg, gpu, tw, tt, B, K, R):
+    """Every tile of the tiled product, whole and split along K, at sizes that end inside a tile, a group and a block; row
+    counts that fill from one to all of a tile's parts."""
+    rng = np.random.default_rng(B + K + tw + tt)
+    bits, s = of8.random_weights(rng, R, K)
+    leaf, x = _leaf(pkg, bits, s), _acts(rng, B, K)
+    want, bound = of8.project(of8.rows_dense(*of8.quantize(_np(x))), of8.weights_dense(bits, s))
+    for S in (1, 2, 5, 8):
+        with pkg.tuning(F8_TW=tw, F8_TT=tt, F8_S=S):
+            yb, yf = pkg.fp8_project(x, leaf, want_f32=True)
+            _check(yb, yf, want, bound)
+            few = max(33, B - 31)                         # fewer rows of the same tile: the same bits
+            assert torch.equal(pkg.fp8_project(x[:few], leaf), yb[:few])
+
+
 def test_project_outputs_and_views(pkg, gpu):
     """Outputs given, a misaligned and a strided x, no tokens, a kept workspace for a smaller batch, a column slice of
     a larger output left as it was."""
@@ -227,6 +247,19 @@ def test_mlp(pkg, gpu, B, D, I):
     assert pkg.fp8_mlp(x[:0], *leaves, LIMIT).shape == (0, D)
 
 
+@pytest.mark.parametrize("tt", [32, 64, 128, 256])
+@pytest.mark.parametrize("B,D,I", [(33, 144, 16), (70, 1040, 272), (300, 512, 400)])
+def test_mlp_every_tile(pkg, gpu, tt, B, D, I):
+    rng = np.random.default_rng(B + D + tt)
+    raw = [of8.random_weights(rng, R, K, 0.05) for R, K in ((I, D), (I, D), (D, I))]
+    x = _acts(rng, B, D)
+    want, bound = of8.mlp(of8.rows_dense(*of8.quantize(_np(x))), *[of8.weights_dense(*r) for r in raw], LIMIT)
+    for S in (1, 3, 8):
+        with pkg.tuning(F8_TT=max(tt, 64) if S == 8 else tt, F8_S=S):
+            yb, yf = pkg.fp8_mlp(x, *[_leaf(pkg, *r) for r in raw], LIMIT, want_f32=True)
+            _check(yb, yf, want, bound)
+
+
 # ------------------------------------------------------------------------------------------------ grouped, moe
 def _experts(rng, E, D, I, std=0.05):
     return [of8.random_weights(rng, R, K, std, E) for R, K in ((I, D), (I, D), (D, I))]
@@ -276,6 +309,10 @@ def test_grouped_plan_out_of_range(pkg, gpu):
     plan["tok_row"][5:16] = -1                            # padding rows: zeros whatever x holds
     z = pkg.fp8_grouped(x, plan, leaf, want_f32=True)[1]
     assert (z[5:16] == 0).all() and torch.equal(z[:5], y[:5]) and torch.equal(z[48:], y[48:])
+    bad = leaf.q.view(torch.uint8).clone()
+    bad[0, 3] = 0x7f                                       # and whatever the weights hold
+    z = pkg.fp8_grouped(x, plan, pkg.Fp8Leaf(bad.view(F8), leaf.s), want_f32=True)[1]
+    assert (z[5:16] == 0).all() and torch.isnan(z[:5, 3]).all()
     plan["n_blocks"].fill_(-5)
     assert (pkg.fp8_grouped(x, plan, leaf) == 0).all()
 
@@ -311,6 +348,43 @@ def test_moe(pkg, gpu, T, E, k, D, I):
     _check(ob, of, want, bound)
     of2, ob2 = pkg.fp8_moe(*leaves, x.float(), it.long(), wt, LIMIT)      # f32 activations of the same values
     assert ob2 is None and torch.equal(of2, of)
+
+
+@pytest.mark.parametrize("tm", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("T,E,k,D,I", [(1, 8, 2, 256, 144), (9, 4, 2, 640, 272), (70, 3, 2, 272, 128), (230, 3, 2, 384, 400)])
+def test_moe_every_block_size(pkg, gpu, tm, T, E, k, D, I):
+    """Each block size of the sorted form from one row a block to full ones, and the streaming form up to its limit: one
+    layer, within one bound."""
+    rng = np.random.default_rng(T + tm + D)
+    raw = _experts(rng, E, D, I)
+    idx, w = _routing(rng, T, E, k, skew=True)
+    if T > 2:
+        idx[1, 0], idx[2, -1] = -1, E
+    x = _acts(rng, T, D)
+    xd = of8.rows_dense(*of8.quantize(_np(x)))
+    want, bound = of8.moe(xd, idx, w, lambda e: [of8.weights_dense(b[e], s[e]) for b, s in raw], LIMIT, E)
+    args = [_leaf(pkg, *r) for r in raw] + [x, torch.from_numpy(idx).cuda(), torch.from_numpy(w).cuda(), LIMIT]
+    with pkg.tuning(F8_STREAM=0, F8_TM=tm):
+        _close(pkg.fp8_moe(*args)[0], want, bound)
+    if T * k <= 128 and tm == 16:
+        with pkg.tuning(F8_STREAM=128):
+            _close(pkg.fp8_moe(*args)[0], want, bound)
+
+
+def test_moe_streams_more_than_16_slots_of_an_expert(pkg, gpu):
+    """The streaming form's tiles of 16 slots: 50 slots on one expert, the rest spread."""
+    rng = np.random.default_rng(77)
+    E, D, I, T = 5, 256, 144, 64
+    raw = _experts(rng, E, D, I)
+    idx = rng.integers(0, E, (T, 2)).astype(np.int32)
+    idx[:50, 0] = 3
+    w = rng.uniform(0.1, 1, (T, 2)).astype(np.float32)
+    x = _acts(rng, T, D)
+    want, bound = of8.moe(of8.rows_dense(*of8.quantize(_np(x))), idx, w,
+                          lambda e: [of8.weights_dense(b[e], s[e]) for b, s in raw], LIMIT, E)
+    with pkg.tuning(F8_STREAM=128):
+        of, _ = pkg.fp8_moe(*[_leaf(pkg, *r) for r in raw], x, torch.from_numpy(idx).cuda(), torch.from_numpy(w).cuda(), LIMIT)
+    _close(of, want, bound)
 
 
 def test_moe_no_live_slots(pkg, gpu):
