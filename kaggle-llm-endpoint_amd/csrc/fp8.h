@@ -57,11 +57,34 @@ __device__ __forceinline__ float fp8_swiglu(float g, float u, float limit) {
 //
 // Its arithmetic, measured: the 8 products of 8 consecutive bytes are added on a grid of 2^-13 of the largest one's power
 // of two, what is below is cut; those sums are added in f32.  On normal values that is 1.3e-5 of the result (root mean
-// square), the same for the 16x16x32 fp8 instruction, whatever the kernel around it: a hundredth of a bf16 rounding of the
-// result.  Converting to bf16 instead would be exact at half the rate and 16 conversions per 32 bytes.
+// square), the same for the 16x16x32 fp8 instruction: a hundredth of a bf16 rounding of the result.
 __device__ __forceinline__ f32x4 fp8_mfma(i32x8 a, i32x8 b) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, zero, 0, 0, 0, 0, 0, 0);
+}
+
+// The same product with every sum in f32: both operands converted to bf16, which holds e4m3 exactly, and four
+// 16x16x32 bf16 instructions, at half the rate and with 16 conversions an operand.  Taken for gate and up where memory
+// bounds the launch: their results are quantised again, and of a value next to a rounding border the last bits decide a
+// whole step of e4m3.  (One token through MLPs of 1360 / 592: 0.0023 of the result with the fp8 instruction on average,
+// 0.0081 at worst, against the definition; 0.0017, a bf16 rounding, with this.)
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ bf16x8_t fp8_to_bf16(int lo, int hi) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+    return (bf16x8_t){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+template <bool EXACT>
+__device__ __forceinline__ f32x4 fp8_product(i32x8 a, i32x8 b) {
+    if constexpr (!EXACT) {
+        return fp8_mfma(a, b);
+    } else {
+        f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 8; k += 2)
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp8_to_bf16(a[k], a[k + 1]), fp8_to_bf16(b[k], b[k + 1]), c, 0, 0, 0);
+        return c;
+    }
 }
 
 // One product's operands.  Rows r of the activations: row r of xq, or row tok_row[r] (-1: a row of zeros).  With

@@ -270,7 +270,7 @@ static int fp8_launch_quantize(const void *x, int x_dtype, int n, int K, long lo
 }
 
 // ---- the tiled product.  Tiles: 256 weight rows (128 where a dense product has few tiles) x tt tokens.
-template <int TW, int TT, int WM, int WN, int NST, bool PAIR>
+template <int TW, int TT, int WM, int WN, int NST, bool PAIR, bool EXACT = false>
 static int fp8_launch_tiled(Fp8Tiled p, hipStream_t st) {
     p.nw = (p.g.R + (PAIR ? TW / 2 : TW) - 1) / (PAIR ? TW / 2 : TW);
     p.nb = (p.g.rows + TT - 1) / TT;
@@ -278,21 +278,28 @@ static int fp8_launch_tiled(Fp8Tiled p, hipStream_t st) {
     // (one more for each XCD where there may be blocks without a product, to write their zeros)
     const long long total = (long long)p.nb * p.nw * p.S, grid = (total + 7) / 8 * 8 + (p.g.blk_expert && !p.skip ? 8 : 0);
     if (grid >= (1ll << 31) / (64 * WM * WN)) return MI_ERR_TOKENS;
-    hipLaunchKernelGGL((fp8_gemm_kernel<TW, TT, WM, WN, NST, PAIR>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, p);
+    hipLaunchKernelGGL((fp8_gemm_kernel<TW, TT, WM, WN, NST, PAIR, EXACT>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, p);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }
 
+constexpr int kFp8ExactRows = 64;                // rows of a dense gate/up product up to which its sums are in f32
 template <bool PAIR>
-static int fp8_tiled(const Fp8Tiled &p, int tw, int tt, hipStream_t st) {
+static int fp8_tiled(const Fp8Tiled &p, int tw, int tt, bool exact, hipStream_t st) {
     if constexpr (!PAIR) {
         if (tw == 128) return tt == 64 ? fp8_launch_tiled<128, 64, 2, 2, 3, false>(p, st)
                                        : fp8_launch_tiled<128, 128, 2, 2, 4, false>(p, st);
     }
     switch (tt) {
-        case 16: return fp8_launch_tiled<256, 16, 4, 1, 4, PAIR>(p, st);
-        case 32: return fp8_launch_tiled<256, 32, 4, 1, 4, PAIR>(p, st);
-        case 64: return fp8_launch_tiled<256, 64, 4, 1, 3, PAIR>(p, st);
-        case 128: return fp8_launch_tiled<256, 128, 4, 2, 3, PAIR>(p, st);
+        case 16: return fp8_launch_tiled<256, 16, 4, 1, 4, PAIR, PAIR>(p, st);
+        case 32: return fp8_launch_tiled<256, 32, 4, 1, 4, PAIR, PAIR>(p, st);
+        case 64:
+            if constexpr (PAIR)
+                if (exact) return fp8_launch_tiled<256, 64, 4, 1, 3, true, true>(p, st);
+            return fp8_launch_tiled<256, 64, 4, 1, 3, PAIR>(p, st);
+        case 128:
+            if constexpr (PAIR)
+                if (exact) return fp8_launch_tiled<256, 128, 4, 2, 3, true, true>(p, st);
+            return fp8_launch_tiled<256, 128, 4, 2, 3, PAIR>(p, st);
         default: return fp8_launch_tiled<256, 256, 2, 4, 2, PAIR>(p, st);
     }
 }
@@ -354,7 +361,7 @@ static int fp8_launch_dense(Fp8Gemm a, float *part, hipStream_t st) {
     p.g = a;
     p.S = pl.S;
     p.part[0] = part;
-    int rc = fp8_tiled<false>(p, pl.tw, pl.tt, st);
+    int rc = fp8_tiled<false>(p, pl.tw, pl.tt, false, st);
     if (rc != MI_OK || pl.S == 1) return rc;
     const long long n = (long long)a.rows * a.R;
     hipLaunchKernelGGL(fp8_reduce_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, pl.S, n, a.y_bf16,
@@ -370,7 +377,7 @@ static int fp8_launch_dense_pair(Fp8Gemm a, float limit, uint8_t *hq, float *hs,
     p.S = pl.S;
     p.limit = limit, p.hq = hq, p.hs = hs;
     p.part[0] = part, p.part[1] = part + (size_t)pl.S * a.rows * a.R;
-    int rc = fp8_tiled<true>(p, 256, pl.tt, st);
+    int rc = fp8_tiled<true>(p, 256, pl.tt, a.rows <= kFp8ExactRows, st);
     if (rc != MI_OK || pl.S == 1) return rc;
     hipLaunchKernelGGL(fp8_swiglu_kernel, dim3(a.rows, fp8_groups(a.R)), dim3(64), 0, st, p.part[0], p.part[1], pl.S,
                        a.rows, a.R, limit, hq, hs);
@@ -597,7 +604,7 @@ extern "C" int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, i
     Fp8Tiled p = {};
     p.g = a;
     p.S = 1;
-    return fp8_tiled<false>(p, 256, tm, st);
+    return fp8_tiled<false>(p, 256, tm, false, st);
 }
 
 namespace mi {
@@ -723,12 +730,12 @@ extern "C" int mi_fp8_moe(const uint8_t *gate_q, const float *gate_s, const uint
         p.S = 1;
         p.skip = 1;
         p.limit = limit, p.hq = m.hq, p.hs = m.hs;
-        if ((rc = fp8_tiled<true>(p, 256, m.tm, st)) != MI_OK) return rc;
+        if ((rc = fp8_tiled<true>(p, 256, m.tm, true, st)) != MI_OK) return rc;
         a.xq = m.hq, a.xs = m.hs;
         a.tok_row = nullptr, a.x_rows = m.rows;
         a.R = D, a.K = I;
         a.wq[0] = down_q, a.ws[0] = down_s, a.y_f32 = m.y;
-        if ((rc = fp8_tiled<false>(p, 256, m.tm, st)) != MI_OK) return rc;
+        if ((rc = fp8_tiled<false>(p, 256, m.tm, false, st)) != MI_OK) return rc;
     }
     hipLaunchKernelGGL(fp8_combine_kernel, dim3(T, (D + 1023) / 1024), dim3(256), 0, st, m.y, m.row_slot, idx, E, w, k, D,
                        out_f32, out_bf16);

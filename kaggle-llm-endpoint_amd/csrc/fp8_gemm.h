@@ -29,7 +29,7 @@ struct Fp8Tiled {
     float *part[2];             // S > 1: f32 [S, rows, R] (PAIR: of gate and of up)
 };
 
-template <int TW, int TT, int WM, int WN, int NST, bool PAIR>
+template <int TW, int TT, int WM, int WN, int NST, bool PAIR, bool EXACT>
 __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8Tiled p) {
     constexpr int W = WM * WN, RT = TW / WM / 16, CT = TT / WN / 16;
     constexpr int WL = TW / 8 / W, TL = TT / 8 >= W ? TT / 8 / W : 1;      // 1 KB loads per wavefront and stage
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
                     }
                     if (n < LAG) add(N - LAG + n, last[n]);
                     else add(n - LAG, s[PAIR ? (n - LAG) / CU / (RT / 2) : 0][(n - LAG) % CU]);
-                    v[n & 3] = fp8_mfma(w[r & 3], b[t]);
+                    v[n & 3] = fp8_product<EXACT>(w[r & 3], b[t]);
                     if (r == RT - 1) read_x(nbuf, nsx, t);
                     __builtin_amdgcn_sched_barrier(0);
                 }

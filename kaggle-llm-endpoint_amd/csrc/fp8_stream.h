@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(64 * W, OCC) fp8_stream_kernel(Fp8Stream a) {
 #pragma unroll
                     for (int r = 0; r < RW; ++r) {
                         const uint4 c0 = wv[u][m][r][0], c1 = wv[u][m][r][1];
-                        const f32x4 v = fp8_mfma((i32x8){(int)c0.x, (int)c0.y, (int)c0.z, (int)c0.w,
+                        const f32x4 v = fp8_product<PAIR>((i32x8){(int)c0.x, (int)c0.y, (int)c0.z, (int)c0.w,
                                                          (int)c1.x, (int)c1.y, (int)c1.z, (int)c1.w}, b);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) acc[m][r][t][j] = fmaf(v[j], sc, acc[m][r][t][j]);
