@@ -282,7 +282,7 @@ static int fp8_launch_tiled(Fp8Tiled p, hipStream_t st) {
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }
 
-constexpr int kFp8ExactRows = 64;                // rows of a dense gate/up product up to which its sums are in f32
+constexpr int kFp8ExactRows = 128;               // rows of a dense gate/up product up to which its sums are in f32
 template <bool PAIR>
 static int fp8_tiled(const Fp8Tiled &p, int tw, int tt, bool exact, hipStream_t st) {
     if constexpr (!PAIR) {
@@ -609,10 +609,12 @@ extern "C" int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, i
 
 namespace mi {
 
-// A call of at most MI_MAX_SLOTS slots whose experts are mostly distinct streams the experts' weights per slot; a larger
-// one sorts its slots by expert and takes the tiled product, its token tile the smaller the fewer rows an expert has.
-constexpr int kFp8StreamSlots = 16;
-static bool fp8_moe_streams(int S) { return S <= std::min(tuning(kTuneF8Stream, kFp8StreamSlots), MI_MAX_SLOTS); }
+// A call of a few slots streams each expert's weights, without a plan (one token in 8 slots at 6144 / 2048: 74 us, sorted
+// 78; two tokens 126 and 120).  A larger one sorts its slots by expert and takes the tiled product, its blocks the smaller
+// the fewer rows an expert has (64 experts, top-8, 48 / 96 / 200 / 512 / 1999 tokens: 443 / 463 / 500 / 585 / 1170 us with
+// 16 / 32 / 64 / 128 / 256 rows; half the rows 6 to 20 % more from 96 tokens on, twice as many 2 to 14 % more).
+constexpr int kFp8StreamSlots = 8;
+static bool fp8_moe_streams(int S) { return S <= std::min(tuning(kTuneF8Stream, kFp8StreamSlots), kFp8TileSlots); }
 static int fp8_moe_tile(int S, int E) {
     const int per = S / E;
     return fp8_tile_of(tuning(kTuneF8Tm, per <= 8 ? 16 : per <= 18 ? 32 : per <= 40 ? 64 : per <= 96 ? 128 : 256));
@@ -665,7 +667,7 @@ static int fp8_moe_check(int T, int k, int E, int D, int I) {
 // Enough for every smaller T too: the streaming form's slots besides the tiled form's rows, which grow with T.
 static size_t fp8_moe_bytes(int T, int k, int E, int D, int I) {
     const int S = T * k;
-    const size_t few = fp8_moe_cut_stream(nullptr, std::min(S, MI_MAX_SLOTS), D, I).bytes;
+    const size_t few = fp8_moe_cut_stream(nullptr, std::min(S, kFp8TileSlots), D, I).bytes;
     return fp8_moe_streams(S) ? few : std::max(few, fp8_moe_cut(nullptr, T, k, E, D, I).bytes);
 }
 

@@ -9,13 +9,15 @@
 
 namespace mi {
 
+constexpr int kFp8TileSlots = 16;                // slots that a workgroup's one token tile holds
+
 struct Fp8Stream {
     const void *x;              // bf16, f32 or e4m3 [x_rows, K] (XD)
     const float *xs;            // XD == MI_X_FP8: its scales
     const uint8_t *wq[2];       // e4m3 [E, R, K]; PAIR: gate, up
     const float *ws[2];
     const int32_t *idx;         // expert of every slot (SLOTS)
-    int rows;                   // rows of x and y; SLOTS: slots, <= MI_MAX_SLOTS
+    int rows;                   // rows of x and y; SLOTS: slots, at most kFp8TileSlots
     int div;                    // SLOTS: slot s reads row s / div of x
     int E, R, K;
     float limit;                // PAIR
@@ -106,25 +108,16 @@ __global__ void __launch_bounds__(64 * W, OCC) fp8_stream_kernel(Fp8Stream a) {
 
     int e = 0, row[NT];                          // this lane's rows of y (-1: none)
     if constexpr (SLOTS) {
-        // the slots of this slot's expert, in order; the tile's 16 start at every 16th of them, the others' workgroups end
+        // the slots of this slot's expert; the first one's workgroups take them all, the others' end
         const int slot = blockIdx.y;
-        const int e0 = lane < a.rows ? a.idx[lane] : -1, e1 = lane + 64 < a.rows ? a.idx[lane + 64] : -1;
+        const int e0 = lane < a.rows ? a.idx[lane] : -1;
         e = __builtin_amdgcn_readfirstlane(a.idx[slot]);
         if (e < 0 || e >= a.E) return;           // the whole workgroup: a slot without an expert has no product
-        uint64_t m0 = __ballot(e0 == e), m1 = __ballot(e1 == e);
-        const uint64_t below0 = slot < 64 ? m0 & ((1ull << slot) - 1) : m0;
-        const uint64_t below1 = slot < 64 ? 0ull : m1 & ((1ull << (slot - 64)) - 1);
-        const int rank = __popcll(below0) + __popcll(below1);
-        if (rank & 15) return;
-        m0 &= ~below0;
-        m1 &= ~below1;
+        uint64_t m = __ballot(e0 == e);
+        if (m & ((1ull << slot) - 1)) return;
         row[0] = -1;
-        for (int j = 0; j < 16 && (m0 | m1); ++j) {
-            const int s = m0 ? __ffsll((unsigned long long)m0) - 1 : 64 + __ffsll((unsigned long long)m1) - 1;
-            if (m0) m0 &= m0 - 1;
-            else m1 &= m1 - 1;
-            if (j == i) row[0] = s;
-        }
+        for (int j = 0; m; ++j, m &= m - 1)
+            if (j == i) row[0] = __ffsll((unsigned long long)m) - 1;
     } else {
 #pragma unroll
         for (int t = 0; t < NT; ++t) row[t] = 16 * t + i < a.rows ? 16 * t + i : -1;

@@ -353,8 +353,7 @@ def test_moe(pkg, gpu, T, E, k, D, I):
 @pytest.mark.parametrize("tm", [16, 32, 64, 128, 256])
 @pytest.mark.parametrize("T,E,k,D,I", [(1, 8, 2, 256, 144), (9, 4, 2, 640, 272), (70, 3, 2, 272, 128), (230, 3, 2, 384, 400)])
 def test_moe_every_block_size(pkg, gpu, tm, T, E, k, D, I):
-    """Each block size of the sorted form from one row a block to full ones, and the streaming form up to its limit: one
-    layer, within one bound."""
+    """Each block size of the sorted form, from one row a block to full ones."""
     rng = np.random.default_rng(T + tm + D)
     raw = _experts(rng, E, D, I)
     idx, w = _routing(rng, T, E, k, skew=True)
@@ -366,25 +365,26 @@ def test_moe_every_block_size(pkg, gpu, tm, T, E, k, D, I):
     args = [_leaf(pkg, *r) for r in raw] + [x, torch.from_numpy(idx).cuda(), torch.from_numpy(w).cuda(), LIMIT]
     with pkg.tuning(F8_STREAM=0, F8_TM=tm):
         _close(pkg.fp8_moe(*args)[0], want, bound)
-    if T * k <= 128 and tm == 16:
-        with pkg.tuning(F8_STREAM=128):
-            _close(pkg.fp8_moe(*args)[0], want, bound)
 
 
-def test_moe_streams_more_than_16_slots_of_an_expert(pkg, gpu):
-    """The streaming form's tiles of 16 slots: 50 slots on one expert, the rest spread."""
-    rng = np.random.default_rng(77)
-    E, D, I, T = 5, 256, 144, 64
+@pytest.mark.parametrize("T,k,E", [(1, 16, 3), (16, 1, 2), (8, 2, 64), (5, 3, 4), (2, 8, 1)])
+def test_moe_streams_up_to_16_slots(pkg, gpu, T, k, E):
+    """The streaming form up to its limit: all slots on one expert, spread ones, some without an expert."""
+    rng = np.random.default_rng(T * k + E)
+    D, I = 256, 144
     raw = _experts(rng, E, D, I)
-    idx = rng.integers(0, E, (T, 2)).astype(np.int32)
-    idx[:50, 0] = 3
-    w = rng.uniform(0.1, 1, (T, 2)).astype(np.float32)
+    idx = rng.integers(0, E, (T, k)).astype(np.int32)
+    if T * k > 3:
+        idx.reshape(-1)[2] = -7
+    w = rng.uniform(-1, 1, (T, k)).astype(np.float32)
     x = _acts(rng, T, D)
     want, bound = of8.moe(of8.rows_dense(*of8.quantize(_np(x))), idx, w,
                           lambda e: [of8.weights_dense(b[e], s[e]) for b, s in raw], LIMIT, E)
-    with pkg.tuning(F8_STREAM=128):
-        of, _ = pkg.fp8_moe(*[_leaf(pkg, *r) for r in raw], x, torch.from_numpy(idx).cuda(), torch.from_numpy(w).cuda(), LIMIT)
-    _close(of, want, bound)
+    for limit in (16, 0):
+        with pkg.tuning(F8_STREAM=limit):
+            of, _ = pkg.fp8_moe(*[_leaf(pkg, *r) for r in raw], x, torch.from_numpy(idx).cuda(),
+                                torch.from_numpy(w).cuda(), LIMIT)
+        _close(of, want, bound)
 
 
 def test_moe_no_live_slots(pkg, gpu):
