@@ -269,6 +269,12 @@ static int fp8_launch_quantize(const void *x, int x_dtype, int n, int K, long lo
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }
 
+constexpr int kFp8Cus = 256;
+// Idle workgroups of an XCD that read weights ahead: a few are enough (6144 x 6144, 64 / 128 / 384 / 768 rows: 24.7 / 25.4 /
+// 45.0 / 72 us with none, 19.5 / 20.9 / 35.4 / 53 with up to 8, 20.5 / 23.1 / 35.7 / 53 with all; nothing is gained or lost
+// where the weights are in the last-level cache).
+constexpr int kFp8Ahead = 8;
+
 // ---- the tiled product.  Tiles: 256 weight rows (128 where a dense product has few tiles) x tt tokens.
 template <int TW, int TT, int WM, int WN, int NST, bool PAIR, bool EXACT = false>
 static int fp8_launch_tiled(Fp8Tiled p, hipStream_t st) {
@@ -276,7 +282,13 @@ static int fp8_launch_tiled(Fp8Tiled p, hipStream_t st) {
     p.nb = (p.g.rows + TT - 1) / TT;
     // ids equal modulo 8 share an XCD and a piece of at most ceil(total / 8) workgroups
     // (one more for each XCD where there may be blocks without a product, to write their zeros)
-    const long long total = (long long)p.nb * p.nw * p.S, grid = (total + 7) / 8 * 8 + (p.g.blk_expert && !p.skip ? 8 : 0);
+    const long long total = (long long)p.nb * p.nw * p.S;
+    long long grid = (total + 7) / 8 * 8 + (p.g.blk_expert && !p.skip ? 8 : 0);
+    // of a dense product, up to kFp8Ahead idle CUs of an XCD
+    constexpr int kSlots = kFp8Cus * (163840 / (NST * (128 * (TW + TT) + 256 * WM * WN) + 8 * kFp8MaxGroups + 8));
+    static_assert(kSlots == kFp8Cus || kSlots == 2 * kFp8Cus, "workgroups per CU");
+    if (!p.g.blk_expert && p.nb <= kFp8Near && grid < kSlots) p.ahead = std::min(kFp8Ahead, (int)(kSlots - grid) / 8);
+    grid += 8 * p.ahead;
     if (grid >= (1ll << 31) / (64 * WM * WN)) return MI_ERR_TOKENS;
     hipLaunchKernelGGL((fp8_gemm_kernel<TW, TT, WM, WN, NST, PAIR, EXACT>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, p);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
@@ -304,15 +316,16 @@ static int fp8_tiled(const Fp8Tiled &p, int tw, int tt, bool exact, hipStream_t 
     }
 }
 
-// The tile and the splits of K of a dense product of B rows: the pair of least estimated time.  A round of tiles (one per CU,
-// two of the smallest) takes `step` us per group of 128 columns -- measured with weights from memory, 144 to 576 tiles, 2048
-// and 6144 columns, within a tenth -- and a split adds a launch and a pass over its partial sums.  Splits only fill CUs of
-// the first round.  (6144 x 6144, 96 / 384 / 1536 rows: 22 us with 128 x 64 in two splits, 45 with 128 x 128, 97 with
-// 256 x 256; each of the others takes 1.1 to 3 times as long at two of the three sizes.)
+// The tile and the splits of K of a dense product of B rows: the pair of least estimated time.  A group of 128 columns of a
+// tile takes `one` us in a launch of at most one workgroup per CU and `more` for each round of `slots` workgroups otherwise;
+// a split adds a launch and a pass over its partial sums, and only fills CUs of the first round.  The times are those of
+// weights from memory, 40 to 4096 rows at 6144 x 6144, 2048 x 6144 and 6144 x 2048 with all tiles and splits: over these 45
+// the choice takes 1.5 % more than the best of all on average, 17 % at worst.  (6144 x 6144, 100 / 517 / 1024 / 2048 rows:
+// 20.6 us with 128 x 64 in two splits, 36.4 with 128 x 128, 52 with 256 x 128, 86 with 256 x 256; the best of the other
+// tiles take 22.1 / 44 / 78 / 126.)
 struct Fp8Plan {
     int tw, tt, S;
 };
-constexpr int kFp8Cus = 256;
 constexpr int kFp8SplitTiles = 512;              // tiles x splits at most
 
 // Floats of split sums that any B up to the given one may need.
@@ -327,12 +340,13 @@ static int fp8_tile_of(int tt) { return tt <= 16 ? 16 : tt <= 32 ? 32 : tt <= 64
 static Fp8Plan fp8_plan(int B, int R, int K, bool pair) {
     struct Tile {
         int tw, tt, slots;
-        float step;
+        float one, more;
     };
-    static const Tile dense[] = {{128, 64, 2 * kFp8Cus, 0.7f}, {128, 128, kFp8Cus, 0.85f}, {256, 64, kFp8Cus, 0.9f},
-                                 {256, 128, kFp8Cus, 1.35f}, {256, 256, kFp8Cus, 2.1f}};
-    static const Tile gate_up[] = {{256, 32, kFp8Cus, 0.75f}, {256, 64, kFp8Cus, 0.9f}, {256, 128, kFp8Cus, 1.35f},
-                                   {256, 256, kFp8Cus, 2.1f}};
+    static const Tile dense[] = {{128, 64, 2 * kFp8Cus, 0.46f, 1.02f}, {128, 128, kFp8Cus, 0.72f, 0.82f},
+                                 {256, 64, kFp8Cus, 0.76f, 0.85f}, {256, 128, kFp8Cus, 1.02f, 1.33f},
+                                 {256, 256, kFp8Cus, 1.65f, 2.05f}};
+    static const Tile gate_up[] = {{256, 32, kFp8Cus, 0.90f, 0.95f}, {256, 64, kFp8Cus, 0.76f, 0.85f},
+                                   {256, 128, kFp8Cus, 1.02f, 1.33f}, {256, 256, kFp8Cus, 1.65f, 2.05f}};
     const Tile *c = pair ? gate_up : dense;
     const int n = pair ? 4 : 5, KB = fp8_groups(K);
     const int tw = tuning(kTuneF8Tw, 0), tt = tuning(kTuneF8Tt, 0), fs = tuning(kTuneF8S, 0);
@@ -346,9 +360,11 @@ static Fp8Plan fp8_plan(int B, int R, int K, bool pair) {
             const double floats = (double)S * B * R * (pair ? 2 : 1);
             if (S > 1 && (tiles * S > c[i].slots || floats > (double)fp8_split_floats(R, pair))) break;
             if (fs && S != fs) continue;
-            const float rounds = (float)((tiles * S + c[i].slots - 1) / c[i].slots);
-            const float step = tiles * S <= c[i].slots / 2 ? 0.8f * c[i].step : c[i].step;
-            const float us = rounds * step * ((KB + S - 1) / S) + (S > 1 ? 2.0f + (float)(floats * 8 / 3.5e6) : 0.0f);
+            const long long n_wg = tiles * S, left = n_wg % c[i].slots;
+            const bool light = c[i].slots > kFp8Cus && left <= kFp8Cus;          // the last round has one per CU
+            const float step = n_wg <= kFp8Cus ? c[i].one
+                                               : n_wg / c[i].slots * c[i].more + (!left ? 0.0f : light ? c[i].one : c[i].more);
+            const float us = step * ((KB + S - 1) / S + 1) + (S > 1 ? 3.0f + (float)(floats * 8 / 3.5e6) : 0.0f);
             if (us < least) least = us, best = Fp8Plan{c[i].tw, c[i].tt, S};
         }
     }

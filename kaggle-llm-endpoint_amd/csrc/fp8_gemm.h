@@ -23,6 +23,7 @@ struct Fp8Tiled {
     int nb;                     // token tiles (grouped: at most; *g.n_blocks are used)
     int S;                      // splits of K
     int skip;                   // rows without a token are not written (else: zeros)
+    int ahead;                  // workgroups of an XCD that only read its weights, ahead of the others
     float limit;                // PAIR
     uint8_t *hq;                // PAIR: e4m3 [rows, R] and its scales
     float *hs;
@@ -61,6 +62,26 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
                 if (a.y_bf16) a.y_bf16[n] = 0;
             }
     };
+    if (p.ahead && li >= (int)((total + 7) / 8)) {
+        // An idle CU reads the XCD's weights into its L2 in the order of their use, one word of each 128-byte line, so that
+        // the CUs at work find them there: a stage's loads have one to three steps to come back, less than a read of HBM
+        // takes under load.  (nb <= kFp8Near: the XCD's items are all token tiles of some weight tiles.)
+        const int lo = (int)(first / nb), tiles = (int)((end - 1) / nb) - lo + 1, rows = tiles * TW;
+        const int lines = rows * ((KB + p.S - 1) / p.S), step = p.ahead * 64 * W;
+        for (int l = (li - (int)((total + 7) / 8)) * 64 * W + tid; l < lines; l += 4 * step) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int at = min(l + k * step, lines - 1), r = at % rows, item = lo + r / TW;
+                const int m = PAIR ? r % TW / (TW / 2) : 0, o = item % p.nw * (PAIR ? TW / 2 : TW) + r % (PAIR ? TW / 2 : TW);
+                const int g = item / p.nw * KB / p.S + at / rows;
+                v[k] = *(const uint32_t *)(a.wq[m] + (size_t)min(o, a.R - 1) * a.K + min(g * kFp8Group, a.K - 16));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) asm volatile("" ::"v"(v[k]));    // (the loads stay)
+        }
+        return;
+    }
     if (at >= end) {
         // this workgroup has none: the blocks behind the last one in use are dealt out to those that every XCD has over
         const int over = (int)(gridDim.x >> 3) - (int)((total + 7) / 8), z = (int)(at - end);
