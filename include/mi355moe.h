@@ -496,9 +496,10 @@ int mi_moe_combine_grad(const void *dout, const void *y, int32_t dtype, int32_t 
  * CS1, CS2 with _RTW; MGMAX), launch-family switches (CUSTREAM, CUMULTI, PERSIST_ABOVE, FUSE_SWIGLU, CU_FORM_H), the
  * one-launch decode's poll limit (SPIN_LIMIT), the int8 split plan (I8S, I8_WAVES, I8_FUSE) and the many-token MLP's
  * splits and token tile (DG_S1, DG_S2, DG_NT), the prefill's wide blocks (PF_WIDE), the dense fp8 product's tile and
- * splits (F8_TW, F8_TT, F8_S) and the fp8 routed layer's streaming limit and rows per block (F8_STREAM, F8_TM).  Overrides change
- * launch shapes and summation orders, never the result beyond f32 rounding; workspace sizes follow them, so set them
- * before sizing a workspace.  Not synchronised with calls running on other host threads.
+ * splits (F8_TW, F8_TT, F8_S) and the fp8 routed layer's streaming limit and rows per block (F8_STREAM, F8_TM).
+ * Overrides change launch shapes and summation orders, never the result beyond f32 rounding (of the fp8 MLP and routed
+ * layer: beyond that of h before it is rounded to e4m3); workspace sizes follow them, so set them before sizing a
+ * workspace.  Not synchronised with calls running on other host threads.
  */
 int mi_tuning_set(const char *name, int32_t value);
 void mi_tuning_reset(void);

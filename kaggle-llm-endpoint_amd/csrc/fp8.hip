@@ -320,7 +320,7 @@ static int fp8_tiled(const Fp8Tiled &p, int tw, int tt, bool exact, hipStream_t 
 // tile takes `one` us in a launch of at most one workgroup per CU and `more` for each round of `slots` workgroups otherwise;
 // a split adds a launch and a pass over its partial sums, and only fills CUs of the first round.  The times are those of
 // weights from memory, 40 to 4096 rows at 6144 x 6144, 2048 x 6144 and 6144 x 2048 with all tiles and splits: over these 45
-// the choice takes 1.5 % more than the best of all on average, 17 % at worst.  (6144 x 6144, 100 / 517 / 1024 / 2048 rows:
+// the choice takes 1.1 % more than the best of all on average, 10 % at worst.  (6144 x 6144, 100 / 517 / 1024 / 2048 rows:
 // 20.6 us with 128 x 64 in two splits, 36.4 with 128 x 128, 52 with 256 x 128, 86 with 256 x 256; the best of the other
 // tiles take 22.1 / 44 / 78 / 126.)
 struct Fp8Plan {
@@ -340,13 +340,13 @@ static int fp8_tile_of(int tt) { return tt <= 16 ? 16 : tt <= 32 ? 32 : tt <= 64
 static Fp8Plan fp8_plan(int B, int R, int K, bool pair) {
     struct Tile {
         int tw, tt, slots;
-        float one, more;
+        float one, more, ends;             // ends: a tile's start and epilogue, in groups
     };
-    static const Tile dense[] = {{128, 64, 2 * kFp8Cus, 0.46f, 1.02f}, {128, 128, kFp8Cus, 0.72f, 0.82f},
-                                 {256, 64, kFp8Cus, 0.76f, 0.85f}, {256, 128, kFp8Cus, 1.02f, 1.33f},
-                                 {256, 256, kFp8Cus, 1.65f, 2.05f}};
-    static const Tile gate_up[] = {{256, 32, kFp8Cus, 0.90f, 0.95f}, {256, 64, kFp8Cus, 0.76f, 0.85f},
-                                   {256, 128, kFp8Cus, 1.02f, 1.33f}, {256, 256, kFp8Cus, 1.65f, 2.05f}};
+    static const Tile dense[] = {{128, 64, 2 * kFp8Cus, 0.46f, 1.02f, 1}, {128, 128, kFp8Cus, 0.72f, 0.82f, 1},
+                                 {256, 64, kFp8Cus, 0.76f, 0.85f, 1}, {256, 128, kFp8Cus, 1.02f, 1.36f, 1},
+                                 {256, 256, kFp8Cus, 1.60f, 1.86f, 4}};
+    static const Tile gate_up[] = {{256, 32, kFp8Cus, 0.90f, 0.95f, 1}, {256, 64, kFp8Cus, 0.76f, 0.85f, 1},
+                                   {256, 128, kFp8Cus, 1.02f, 1.36f, 1}, {256, 256, kFp8Cus, 1.60f, 1.86f, 4}};
     const Tile *c = pair ? gate_up : dense;
     const int n = pair ? 4 : 5, KB = fp8_groups(K);
     const int tw = tuning(kTuneF8Tw, 0), tt = tuning(kTuneF8Tt, 0), fs = tuning(kTuneF8S, 0);
@@ -364,7 +364,7 @@ static Fp8Plan fp8_plan(int B, int R, int K, bool pair) {
             const bool light = c[i].slots > kFp8Cus && left <= kFp8Cus;          // the last round has one per CU
             const float step = n_wg <= kFp8Cus ? c[i].one
                                                : n_wg / c[i].slots * c[i].more + (!left ? 0.0f : light ? c[i].one : c[i].more);
-            const float us = step * ((KB + S - 1) / S + 1) + (S > 1 ? 3.0f + (float)(floats * 8 / 3.5e6) : 0.0f);
+            const float us = step * ((KB + S - 1) / S + c[i].ends) + (S > 1 ? 3.0f + (float)(floats * 8 / 3.5e6) : 0.0f);
             if (us < least) least = us, best = Fp8Plan{c[i].tw, c[i].tt, S};
         }
     }
@@ -593,7 +593,8 @@ extern "C" size_t mi_fp8_grouped_workspace(int32_t rows, int32_t K, int32_t R) {
 
 extern "C" int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, int32_t n_blk, int32_t tm,
                               const int32_t *blk_expert, const int32_t *n_blocks, const int32_t *tok_row,
-                              const uint8_t *wq, const float *ws, int32_t E, int32_t K, int32_t R, uint16_t *y_bf16, float *y_f32, void *workspace,
+                              const uint8_t *wq, const float *ws, int32_t E, int32_t K, int32_t R, uint16_t *y_bf16,
+                              float *y_f32, void *workspace,
                               size_t workspace_bytes, void *stream) {
     if (tm != 16 && tm != 32 && tm != 64 && tm != 128) return MI_ERR_ARG;
     if (n_blk <= 0 || n_blk > kFp8MaxRows / tm) return MI_ERR_TOKENS;

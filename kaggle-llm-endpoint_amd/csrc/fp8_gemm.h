@@ -1,4 +1,21 @@
-// Tiled block-scaled fp8 product (fp8.h) for many rows, dense or of sorted rows by expert.
+// Tiled block-scaled fp8 product (fp8.h) for many rows, dense or of sorted rows by expert; PAIR: of gate and up, with
+// h = swiglu quantised again in the epilogue.
+//
+// A workgroup computes TW weight rows x TT tokens, its wavefronts WM x WN of them, one group of 128 columns a step: NST
+// stages of both operands are in LDS, filled from memory without registers, and a step is RT x CT matrix instructions a
+// wavefront.  An instruction's operands come from LDS as whole fragments (weights in use for CT instructions, tokens for
+// the whole step), its result is scaled and added by 4 fused multiply-adds.
+//
+// What bounds it: a step of 256 x 256 takes 3450 clocks where its matrix instructions take 2048 and 1720 are reached with
+// both loads and barriers left out; the loads cost 970 and the barrier 760 of them.  Those loads mostly wait for memory
+// under load, which takes longer to answer than the stages in flight last: weights that already are in the last-level
+// cache save up to a third.  4096 x 6144 x 6144 takes 205 us (1.5 PFLOP/s; a library's product with one scale for the
+// whole tensor takes 123), 64 experts of 2.4 GB read once for 200 tokens in 8 each 500 us (4.9 TB/s).
+//
+// Measured and not kept: touching lines two or three stages ahead from the same wavefronts (loads return in order, so they
+// are waited for as well: 3 to 13 % slower), two 128 x 128 workgroups per CU (20 % faster at 768 rows, up to 15 % slower at
+// 900 to 3000), higher priority around the matrix instructions, loads spread over the whole step, 2, 4 or 16 in
+// kFp8Near (within 2 %).
 #pragma once
 #include <type_traits>
 
@@ -35,7 +52,8 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     constexpr int W = WM * WN, RT = TW / WM / 16, CT = TT / WN / 16;
     constexpr int WL = TW / 8 / W, TL = TT / 8 >= W ? TT / 8 / W : 1;      // 1 KB loads per wavefront and stage
     constexpr int ROWS = TW + TT;
-    static_assert(TW % (8 * W) == 0 && (CT == 1 || CT == 2 || CT == 4) && (!PAIR || (TW == 256 && RT % 2 == 0 && 16 % W == 0)), "");
+    static_assert(TW % (8 * W) == 0 && (CT == 1 || CT == 2 || CT == 4), "");
+    static_assert(!PAIR || (TW == 256 && RT % 2 == 0 && 16 % W == 0), "");
     __shared__ uint4 buf0[ROWS * 8], buf1[ROWS * 8], buf2[NST > 2 ? ROWS * 8 : 1], buf3[NST > 3 ? ROWS * 8 : 1];
     __shared__ float sx0[W * 64], sx1[W * 64], sx2[NST > 2 ? W * 64 : 1], sx3[NST > 3 ? W * 64 : 1];
     __shared__ float sw[2][kFp8MaxGroups + 1];     // (a step reads one group ahead)
@@ -45,8 +63,8 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     const int wm = wave / WN, wn = wave % WN;
     const int KB = fp8_groups(a.K), RB = fp8_groups(a.R);
 
-    // An XCD's workgroups (ids equal modulo 8) take one contiguous piece of the work: kFp8Near token tiles of a weight tile,
-    // then of the next.  Its 32 CUs then work on about 8 token tiles x 4 weight tiles at a time and meet each other's
+    // An XCD's workgroups (ids equal modulo 8) take one contiguous piece of the work: kFp8Near token tiles of a weight
+    // tile, then of the next.  Its 32 CUs then work on about 8 token tiles x 4 weight tiles at a time and meet each other's
     // loads in that XCD's L2; the blocks of one expert are next to each other and share its weights.
     const int nb = a.n_blocks ? min(max(*a.n_blocks, 0), p.nb) : p.nb;
     const long long total = (long long)nb * p.nw * p.S;
@@ -72,9 +90,10 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
             uint32_t v[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int at = min(l + k * step, lines - 1), r = at % rows, item = lo + r / TW;
-                const int m = PAIR ? r % TW / (TW / 2) : 0, o = item % p.nw * (PAIR ? TW / 2 : TW) + r % (PAIR ? TW / 2 : TW);
-                const int g = item / p.nw * KB / p.S + at / rows;
+                const int n = min(l + k * step, lines - 1), r = n % rows, item = lo + r / TW;
+                const int m = PAIR ? r % TW / (TW / 2) : 0;
+                const int o = item % p.nw * (PAIR ? TW / 2 : TW) + r % (PAIR ? TW / 2 : TW);
+                const int g = item / p.nw * KB / p.S + n / rows;
                 v[k] = *(const uint32_t *)(a.wq[m] + (size_t)min(o, a.R - 1) * a.K + min(g * kFp8Group, a.K - 16));
             }
 #pragma unroll
@@ -185,9 +204,9 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
         return (i32x8){(int)u.x, (int)u.y, (int)u.z, (int)u.w, (int)v.x, (int)v.y, (int)v.z, (int)v.w};
     };
     // One matrix instruction after the other, n = r CU + t, each behind the scaling of the result two instructions
-    // older, which is done by then; weights are read from LDS WD row tiles ahead (one where registers are short), the next stage's tokens where this
-    // stage's are used last.  The order below is the order of the instructions: left alone the compiler puts each
-    // result's use right behind its instruction and waits for it.
+    // older, which is done by then; weights are read from LDS WD row tiles ahead (one where registers are short), the
+    // next stage's tokens where this stage's are used last.  The order below is the order of the instructions: left
+    // alone the compiler puts each result's use right behind its instruction and waits for it.
     //
     // The only barrier of a stage is where its last fragment has been read: then the next stage must have landed (the
     // later ones stay in flight), and this one's buffer may be overwritten.

@@ -60,7 +60,10 @@ __device__ __forceinline__ i32x8 fp8_x_quantize(const Fp8X<XD> &f, float &scale)
     } else {
         uint32_t u[4 * Fp8X<XD>::N];
 #pragma unroll
-        for (int j = 0; j < Fp8X<XD>::N; ++j) u[4 * j] = f.v[j].x, u[4 * j + 1] = f.v[j].y, u[4 * j + 2] = f.v[j].z, u[4 * j + 3] = f.v[j].w;
+        for (int j = 0; j < Fp8X<XD>::N; ++j) {
+            u[4 * j] = f.v[j].x, u[4 * j + 1] = f.v[j].y;
+            u[4 * j + 2] = f.v[j].z, u[4 * j + 3] = f.v[j].w;
+        }
         uint32_t a = 0;
         if constexpr (XD == MI_X_BF16) {
             u16x2 m = {0, 0};

@@ -59,7 +59,7 @@ __device__ __forceinline__ void zero_padding(const int32_t *__restrict__ tok_row
     }
 }
 
-// A token is read once and stored to its k rows (by row, reading tok_row's token, took 122 us instead of DISPATCH_US for
+// A token is read once and stored to its k rows (by row, reading tok_row's token, took 122 us instead of 93 for
 // 4096 tokens of 6144 bf16 values in 8 rows each: the token's row comes from memory again where its rows are far apart).
 // Workgroups 0 .. T - 1: one token each; the others zero the padding rows.
 template <int XD>
@@ -202,7 +202,8 @@ extern "C" int mi_moe_combine_grad(const void *dout, const void *y, int32_t dtyp
     if (rc != MI_OK) return rc;
     if (!moe_rows_aligned(dout, y, dy) || !words_aligned(row_slot, tok_row, w) || !words_aligned(dw)) return MI_ERR_ARG;
     auto kern = dtype == MI_X_BF16 ? moe_combine_grad_kernel<MI_X_BF16> : moe_combine_grad_kernel<MI_X_F32>;
-    hipLaunchKernelGGL(kern, dim3(T + (rows + kPadRows - 1) / kPadRows), dim3(256), 0, (hipStream_t)stream, dout, y, row_slot, tok_row, w, T, k, D,
+    hipLaunchKernelGGL(kern, dim3(T + (rows + kPadRows - 1) / kPadRows), dim3(256), 0, (hipStream_t)stream, dout, y,
+                       row_slot, tok_row, w, T, k, D,
                        rows, dy, dw);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }

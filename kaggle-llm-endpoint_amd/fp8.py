@@ -223,7 +223,8 @@ def fp8_grouped(xs, plan, leaf, want_f32=False, y_bf16=None, y_f32=None, workspa
     stream = _stream_of("fp8_grouped", x, xs, blk, nb, tok, leaf.q, leaf.s, yb, yf, workspace)
     held, ws, nbytes = _workspace(workspace, lib().mi_fp8_grouped_workspace(rows, K, R), x.device)
     check("mi_fp8_grouped", lib().mi_fp8_grouped(x.data_ptr(), dtype, _ptr(xs), G, rows // G, _ptr(blk), _ptr(nb),
-                                                 _ptr(tok), _ptr(leaf.q), _ptr(leaf.s), E, K, R, _ptr(yb), _ptr(yf), ws, nbytes, stream))
+                                                 _ptr(tok), _ptr(leaf.q), _ptr(leaf.s), E, K, R, _ptr(yb), _ptr(yf), ws, nbytes,
+                                                 stream))
     return (yb, yf) if want_f32 else yb
 
 
