@@ -270,9 +270,10 @@ static int fp8_launch_quantize(const void *x, int x_dtype, int n, int K, long lo
 }
 
 constexpr int kFp8Cus = 256;
-// Idle workgroups of an XCD that read weights ahead: a few are enough (6144 x 6144, 64 / 128 / 384 / 768 rows: 24.7 / 25.4 /
-// 45.0 / 72 us with none, 19.5 / 20.9 / 35.4 / 53 with up to 8, 20.5 / 23.1 / 35.7 / 53 with all; nothing is gained or lost
-// where the weights are in the last-level cache).
+// Idle workgroups of an XCD that read weights ahead.  6144 x 6144, 40 / 64 / 128 / 300 / 768 rows: 22.9 / 24.7 / 25.4 / 37 /
+// 72 us with none, 16.3 / 18.1 / 21.4 / 32.7 / 53 with up to 8 of idle CUs; sharing CUs with the others (where a CU takes two
+// workgroups) 40 and 300 rows took 20.5 and 37.5, all idle CUs instead of 8 up to 2 us more.  Nothing is gained or lost where
+// the weights are in the last-level cache.
 constexpr int kFp8Ahead = 8;
 
 // ---- the tiled product.  Tiles: 256 weight rows (128 where a dense product has few tiles) x tt tokens.
@@ -287,7 +288,8 @@ static int fp8_launch_tiled(Fp8Tiled p, hipStream_t st) {
     // of a dense product, up to kFp8Ahead idle CUs of an XCD
     constexpr int kSlots = kFp8Cus * (163840 / (NST * (128 * (TW + TT) + 256 * WM * WN) + 8 * kFp8MaxGroups + 8));
     static_assert(kSlots == kFp8Cus || kSlots == 2 * kFp8Cus, "workgroups per CU");
-    if (!p.g.blk_expert && p.nb <= kFp8Near && grid < kSlots) p.ahead = std::min(kFp8Ahead, (int)(kSlots - grid) / 8);
+    const long long slots = grid < kFp8Cus ? kFp8Cus : kSlots;
+    if (!p.g.blk_expert && p.nb <= kFp8Near && grid < slots) p.ahead = std::min(kFp8Ahead, (int)(slots - grid) / 8);
     grid += 8 * p.ahead;
     if (grid >= (1ll << 31) / (64 * WM * WN)) return MI_ERR_TOKENS;
     hipLaunchKernelGGL((fp8_gemm_kernel<TW, TT, WM, WN, NST, PAIR, EXACT>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, p);

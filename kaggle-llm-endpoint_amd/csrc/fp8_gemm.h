@@ -9,7 +9,7 @@
 // What bounds it: a step of 256 x 256 takes 3450 clocks where its matrix instructions take 2048 and 1720 are reached with
 // both loads and barriers left out; the loads cost 970 and the barrier 760 of them.  Those loads mostly wait for memory
 // under load, which takes longer to answer than the stages in flight last: weights that already are in the last-level
-// cache save up to a third.  4096 x 6144 x 6144 takes 205 us (1.5 PFLOP/s; a library's product with one scale for the
+// cache save up to a third.  4096 x 6144 x 6144 takes 198 us (1.56 PFLOP/s; a library's product with one scale for the
 // whole tensor takes 123), 64 experts of 2.4 GB read once for 200 tokens in 8 each 500 us (4.9 TB/s).
 //
 // Measured and not kept: touching lines two or three stages ahead from the same wavefronts (loads return in order, so they
@@ -24,6 +24,8 @@
 namespace mi {
 
 constexpr int kFp8Near = 8;                      // token tiles of a weight tile that run next to each other
+constexpr int kFp8AheadLoads = 4;                // lines in flight of a lane that reads ahead
+constexpr int kFp8AheadRows = 512;               // weight rows that one workgroup reads ahead
 constexpr int kFp8MaxGroups = 512;              // K / 128: the weight scales of a tile's blocks are kept in LDS
 
 // Memory to LDS without registers: lane l's 16 (4) bytes to dst + 16 l (4 l).
@@ -84,12 +86,14 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
         // An idle CU reads the XCD's weights into its L2 in the order of their use, one word of each 128-byte line, so that
         // the CUs at work find them there: a stage's loads have one to three steps to come back, less than a read of HBM
         // takes under load.  (nb <= kFp8Near: the XCD's items are all token tiles of some weight tiles.)
-        const int lo = (int)(first / nb), tiles = (int)((end - 1) / nb) - lo + 1, rows = tiles * TW;
+        // One CU reads about 90 bytes a ns, 512 rows in 0.7 us a group: with more than that for each it would end last.
+        const int lo = (int)(first / nb), tiles = (int)((end - 1) / nb) - lo + 1;
+        const int rows = min(tiles * TW, p.ahead * kFp8AheadRows);
         const int lines = rows * ((KB + p.S - 1) / p.S), step = p.ahead * 64 * W;
-        for (int l = (li - (int)((total + 7) / 8)) * 64 * W + tid; l < lines; l += 4 * step) {
-            uint32_t v[4];
+        for (int l = (li - (int)((total + 7) / 8)) * 64 * W + tid; l < lines; l += kFp8AheadLoads * step) {
+            uint32_t v[kFp8AheadLoads];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < kFp8AheadLoads; ++k) {
                 const int n = min(l + k * step, lines - 1), r = n % rows, item = lo + r / TW;
                 const int m = PAIR ? r % TW / (TW / 2) : 0;
                 const int o = item % p.nw * (PAIR ? TW / 2 : TW) + r % (PAIR ? TW / 2 : TW);
@@ -97,7 +101,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
                 v[k] = *(const uint32_t *)(a.wq[m] + (size_t)min(o, a.R - 1) * a.K + min(g * kFp8Group, a.K - 16));
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) asm volatile("" ::"v"(v[k]));    // (the loads stay)
+            for (int k = 0; k < kFp8AheadLoads; ++k) asm volatile("" ::"v"(v[k]));    // (the loads stay)
         }
         return;
     }
