@@ -475,10 +475,11 @@ size_t mi_fp8_moe_workspace(int32_t T, int32_t k, int32_t E, int32_t D, int32_t 
  * Tokens into expert order and back over mi_ragged_plan's layout (the gather and combine of _apply_ragged_kernel,
  * resident.py:153-165), and their gradients; dtype MI_X_BF16 or MI_X_F32 for every row buffer, D % 8 == 0, rows
  * 16-byte aligned, sums in f32 and in column order, one rounding:
- *   mi_moe_dispatch      xs[row_slot[t, j]] = x[t], zeros on padding rows (tok_row -1)
+ *   mi_moe_dispatch      xs[row_slot[t, j]] = x[t], zeros on all other rows
  *   mi_moe_combine       out[t] = sum_j w[t, j] y[row_slot[t, j]]; w NULL: weights 1 (dispatch's gradient)
- *   mi_moe_combine_grad  dy[row_slot[t, j]] = w[t, j] dout[t], zeros on padding rows; dw[t, j] = <dout[t], y[row_slot[t, j]]>
- * A slot without a row (row_slot -1) adds nothing and gets dw 0.
+ *   mi_moe_combine_grad  dy[row_slot[t, j]] = w[t, j] dout[t], zeros on all others; dw[t, j] = <dout[t], y[row_slot[t, j]]>
+ * tok_row[row_slot[t, j]] is t, as the plan has it.  A slot without a row (row_slot -1: an expert id outside [0, E), or
+ * taken out by the caller) adds nothing and gets dw 0.
  */
 int mi_moe_dispatch(const void *x, int32_t dtype, int32_t T, int32_t k, int32_t D, const int32_t *row_slot,
                     const int32_t *tok_row, int32_t rows, void *xs, void *stream);

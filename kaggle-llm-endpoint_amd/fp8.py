@@ -8,7 +8,8 @@ scale per 128 x 128 block, contracted as fp8 on the matrix cores with activation
     o, _ = fp8_moe(gate, up, down, x, idx, w, limit)    the routed experts of a layer
 
 Everything runs on the current torch (HIP) stream of the current device.  The weights are a checkpoint's and the
-products have no gradient: an input that requires one is refused while gradients are recorded.
+products have no gradient: an input (rows, scales, routing weights) that requires one is refused while gradients are
+recorded.  Outputs and workspaces must not overlap the inputs or each other.
 """
 from typing import NamedTuple
 
@@ -37,7 +38,7 @@ def fp8_leaf(leaf, device="cuda"):
     """{"q": float8_e4m3fn [..., n_out, n_in], "s": [..., ceil(n_out / 128), ceil(n_in / 128)]}, as a checkpoint stores
     a matrix (or E of them) and its scales -> Fp8Leaf on the device."""
     q, s = (leaf["q"], leaf["s"]) if isinstance(leaf, dict) else leaf
-    leaf = Fp8Leaf(q.to(device).contiguous(), s.to(device=device, dtype=torch.float32).contiguous())
+    leaf = Fp8Leaf(q.detach().to(device).contiguous(), s.detach().to(device=device, dtype=torch.float32).contiguous())
     _leaf_dims(leaf, "fp8_leaf")
     return leaf
 
@@ -57,6 +58,7 @@ def _leaf_dims(leaf, who):
         raise ValueError("%s: scales %s do not fit weights %s: one per 128 x 128 block" % (who, tuple(ss), tuple(qs)))
     if not (q.is_contiguous() and s.is_contiguous()):
         raise ValueError("%s: weights and scales must be contiguous (fp8_leaf makes them so)" % who)
+    _no_grad(who, s)
     return E, R, K
 
 
@@ -112,6 +114,7 @@ def _rows_of(x, K, who):
             raise TypeError("%s: quantised activations are (float8_e4m3fn, float32 scales)" % who)
         if q.dim() != 2 or tuple(s.shape) != (q.shape[0], _blocks(q.shape[1])):
             raise ValueError("%s: quantised activations are q [B, n_in] with s [B, ceil(n_in / 128)]" % who)
+        _no_grad(who, s)
         x, xs, dtype = _aligned(q), s.contiguous(), _lib.MI_X_FP8
     else:
         xs, dtype = None, _DTYPES.get(x.dtype)

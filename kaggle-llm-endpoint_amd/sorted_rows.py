@@ -6,7 +6,9 @@ combine around the ragged products (resident.py:153-165), with their gradients:
     out  = moe_combine(y, plan, w)          [T, D]
 
 Both record gradients (x; y and w), first order only, and save no copies: the rows a backward pass reads are the
-forward's own inputs.  Deterministic: no atomics, sums in f32 in column order, one rounding.
+forward's own inputs.  Deterministic: no atomics, sums in f32 in column order, one rounding.  A captured backward pass
+needs leaves of its own (``x.detach().requires_grad_()`` inside the capture): an eager graph that still holds the same
+leaves has bound their gradients to another stream.
 """
 import torch
 from torch.autograd.function import once_differentiable
@@ -81,8 +83,8 @@ class _Combine(torch.autograd.Function):
 
 def moe_dispatch(x, plan):
     """Tokens into expert order: x bf16 or f32 [T, D] (D a multiple of 8), plan = ragged_plan(idx, w, E, tm) ->
-    xs [Rp, D] of x's dtype, xs[r] = x[tok_row[r]], zeros on padding rows.  Records the gradient of x: the sum over a
-    token's rows."""
+    xs [Rp, D] of x's dtype, xs[row_slot[t, j]] = x[t], zeros on all other rows (padding, and rows of slots that the
+    caller has taken out: row_slot -1).  Records the gradient of x: the sum over a token's rows."""
     _rows_dtype(x, "moe_dispatch")
     tok, slot = _plan_rows(plan)
     if slot.shape[0] != x.shape[0]:
@@ -97,7 +99,7 @@ def moe_dispatch(x, plan):
 def moe_combine(y, plan, w):
     """The way back: y bf16 or f32 [Rp, D] in the plan's row order, w f32 [T, k] -> out [T, D] of y's dtype, out[t] =
     sum_j w[t, j] * y[row_slot[t, j]] in f32, in column order, rounded once; a slot without a row (an expert id outside
-    [0, E)) adds nothing.  Records the gradients of y (zeros on padding rows) and w."""
+    [0, E), or row_slot set to -1) adds nothing.  Records the gradients of y (zeros on rows without a slot) and w."""
     _rows_dtype(y, "moe_combine")
     tok, slot = _plan_rows(plan)
     if tok.numel() != y.shape[0]:

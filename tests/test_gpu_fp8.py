@@ -518,3 +518,39 @@ def test_layer_from_its_parts(pkg, gpu, T, tm):
             slack[t] += abs(nw[t, j]) * (e + 2.0 ** -8 * (y + e))
     slack += 2.0 ** -8 * (np.abs(want) + slack)
     _close(out, want, bound + slack)
+
+
+def test_weights_past_32_bits(pkg, gpu):
+    """Experts that begin past 2^32 bytes of weights: the same bits as of a leaf that holds those experts alone."""
+    rng = np.random.default_rng(5)
+    E, I, D = 1024, 1040, 4112                            # 4.4 GB a matrix
+    at = [3, 1019, 1023]
+    small = [_leaf(pkg, *r) for r in _experts(rng, 3, D, I)]
+    big = []
+    for q, s in small:
+        bq = torch.zeros((E,) + tuple(q.shape[1:]), dtype=torch.uint8, device="cuda")
+        bs = torch.ones((E,) + tuple(s.shape[1:]), device="cuda")
+        for j, e in enumerate(at):
+            bq[e], bs[e] = q[j].view(torch.uint8), s[j]
+        big.append(pkg.Fp8Leaf(bq.view(F8), bs))
+    names = torch.tensor(at, dtype=torch.int32, device="cuda")
+    for T, tm in ((2, None), (40, None), (200, 64), (200, 256)):
+        x = _acts(rng, T, D)
+        idx = torch.from_numpy(rng.integers(0, 3, (T, 2)).astype(np.int32)).cuda()
+        w = torch.rand((T, 2), device="cuda")
+        with pkg.tuning(**({} if tm is None else {"F8_TM": tm})):
+            got, _ = pkg.fp8_moe(*big, x, names[idx.long()], w, LIMIT)
+        with pkg.tuning(F8_TM=16 if T == 40 else tm or 0) if T > 2 else pkg.tuning():
+            want, _ = pkg.fp8_moe(*small, x, idx, w, LIMIT)
+        assert torch.equal(got, want)
+
+
+def test_outputs_past_32_bits(pkg, gpu):
+    """An output of more than 2^32 values: its rows are those of a smaller call."""
+    rng = np.random.default_rng(6)
+    B, K, R = 65600, 16, 65536
+    leaf = _leaf(pkg, *of8.random_weights(rng, R, K))
+    x = _acts(rng, B, K)
+    y = pkg.fp8_project(x, leaf)
+    few = pkg.fp8_project(x[-300:], leaf)
+    assert torch.equal(y[-300:], few) and torch.equal(y[:64], pkg.fp8_project(x[:64], leaf))

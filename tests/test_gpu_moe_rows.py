@@ -149,6 +149,28 @@ def test_rows_outside_the_buffers_count_as_none(pkg, gpu):
     assert torch.equal(pkg.moe_combine(y, plan, w), y[[0, 5, 3]])
 
 
+@pytest.mark.parametrize("T,E,k,tm,D", [(5, 4, 2, 1, 8), (40, 8, 3, 16, 136), (300, 6, 17, 40, 520)])
+def test_slots_taken_out_of_a_plan(pkg, gpu, T, E, k, tm, D):
+    """Slots dropped by the caller (row_slot -1): their rows are zeros in xs and dy, their weights' gradients zero, the
+    others as before."""
+    rng = np.random.default_rng(T)
+    plan, x, y, w = _setup(pkg, rng, T, E, k, tm, D, torch.float32)
+    gone = torch.from_numpy(rng.random((T, k)) < 0.4).cuda()
+    gone[0], gone[1] = True, False                        # a token that keeps none, one that keeps all
+    slot = plan["row_slot"]
+    plan["row_slot"] = torch.where(gone, -1, slot)
+    y.requires_grad_(), w.requires_grad_()
+    out = pkg.moe_combine(y, plan, w)
+    gout = torch.randn_like(out)
+    dy, dw = torch.autograd.grad(out, [y, w], gout)
+    want = _want(plan, _np(x), _np(y), _np(w), np.zeros(y.shape), _np(gout))
+    assert np.array_equal(_np(pkg.moe_dispatch(x, plan)), want[0])
+    _near(out, *want[1], k, torch.float32)
+    assert (out[0] == 0).all() and (dw[gone] == 0).all()
+    _near(dy, want[3], np.abs(want[3]), 1, torch.float32)
+    _near(dw, *want[4], D, torch.float32)
+
+
 def test_training_step_captured(pkg, gpu):
     """Forward and backward of the pair in one captured graph, replayed three times with new inputs."""
     rng = np.random.default_rng(9)

@@ -250,3 +250,16 @@ def test_a_call_within_a_call_has_other_scratch(pkg, monkeypatch, name, arg):
     fake.again = call
     call()
     assert len(fake.seen) == 2 and fake.seen[0] != fake.seen[1]
+
+
+def test_scales_that_require_a_gradient_are_refused(pkg):
+    leaf = _leaf(pkg, 100, 256)
+    with_grad = pkg.Fp8Leaf(leaf.q, leaf.s.clone().requires_grad_())
+    x = torch.zeros((2, 256), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        pkg.fp8_project(x, with_grad)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        pkg.fp8_project((x.to(F8), torch.ones((2, 2), requires_grad=True)), leaf)
+    with torch.no_grad():
+        assert pkg.fp8._leaf_dims(with_grad, "fp8_project") == (0, 100, 256)
+    assert not pkg.fp8_leaf({"q": leaf.q, "s": torch.nn.Parameter(leaf.s)}, device="cpu").s.requires_grad
