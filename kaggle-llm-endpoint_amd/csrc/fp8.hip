@@ -431,6 +431,23 @@ static int fp8_stream_dense(const Fp8Stream &a, int xd, hipStream_t st) {
          : xd == MI_X_F32 ? fp8_stream_dense_as<MI_X_F32, PAIR>(a, st) : fp8_stream_dense_as<MI_X_FP8, PAIR>(a, st);
 }
 
+// Of the routed layer, more row tiles a wavefront where that leaves enough workgroups: the rows that a workgroup quantises
+// serve them all.  Whole calls at 6144 / 2048: 8 slots 68 us with one row tile of gate and up and four of down, 65 with two
+// and four, 73 with one and two; 2 slots 25, 30 and 26.
+static int fp8_stream_gate_up(const Fp8Stream &a, int xd, hipStream_t st) {
+    const bool two = (long long)(a.R / 32) * a.rows >= kFp8Cus;
+    if (xd == MI_X_F32)
+        return two ? fp8_launch_stream_as<MI_X_F32, 1, 2, true, true, 4, 1, 2>(a, st)
+                   : fp8_launch_stream_as<MI_X_F32, 1, 1, true, true, 4, 2, 3>(a, st);
+    return two ? fp8_launch_stream_as<MI_X_BF16, 1, 2, true, true, 4, 2, 2>(a, st)
+               : fp8_launch_stream_as<MI_X_BF16, 1, 1, true, true, 4, 3, 3>(a, st);
+}
+static int fp8_stream_down(const Fp8Stream &a, hipStream_t st) {
+    return (long long)(a.R / 64) * a.rows >= kFp8Cus / 2
+               ? fp8_launch_stream_as<MI_X_F32, 1, 4, false, true, 4, 1, 3>(a, st)
+               : fp8_launch_stream_as<MI_X_F32, 1, 2, false, true, 4, 2, 3>(a, st);
+}
+
 // A workspace cut into pieces of whole 256 bytes.
 struct Fp8Cut {
     uint8_t *p;
@@ -628,11 +645,11 @@ extern "C" int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, i
 
 namespace mi {
 
-// A call of a few slots streams each expert's weights, without a plan (one token in 8 slots at 6144 / 2048: 74 us, sorted
-// 78; two tokens 126 and 120).  A larger one sorts its slots by expert and takes the tiled product, its blocks the smaller
+// A call of a few slots streams each expert's weights, without a plan (6144 / 2048, one and two tokens in 8 slots each: 65
+// and 113 us, sorted 78 and 124; 12 slots 87 to 90 and 98 to 105).  A larger one sorts its slots by expert and takes the tiled product, its blocks the smaller
 // the fewer rows an expert has (64 experts, top-8, 48 / 96 / 200 / 512 / 1999 tokens: 443 / 463 / 500 / 585 / 1170 us with
 // 16 / 32 / 64 / 128 / 256 rows; half the rows 6 to 20 % more from 96 tokens on, twice as many 2 to 14 % more).
-constexpr int kFp8StreamSlots = 8;
+constexpr int kFp8StreamSlots = kFp8TileSlots;
 static bool fp8_moe_streams(int S) { return S <= std::min(tuning(kTuneF8Stream, kFp8StreamSlots), kFp8TileSlots); }
 static int fp8_moe_tile(int S, int E) {
     const int per = S / E;
@@ -723,15 +740,14 @@ extern "C" int mi_fp8_moe(const uint8_t *gate_q, const float *gate_s, const uint
         f.E = E, f.R = I, f.K = D;
         f.limit = limit;
         f.y_f32 = m.h;
-        rc = x_dtype == MI_X_BF16 ? fp8_launch_stream_as<MI_X_BF16, 1, 1, true, true, 4, 3, 3>(f, st)
-                                  : fp8_launch_stream_as<MI_X_F32, 1, 1, true, true, 4, 2, 3>(f, st);
+        rc = fp8_stream_gate_up(f, x_dtype, st);
         if (rc != MI_OK) return rc;
         f.x = m.h;
         f.wq[0] = down_q, f.ws[0] = down_s;
         f.div = 1;
         f.R = D, f.K = I;
         f.y_f32 = m.y;
-        if ((rc = fp8_launch_stream_as<MI_X_F32, 1, 2, false, true, 4, 2, 3>(f, st)) != MI_OK) return rc;
+        if ((rc = fp8_stream_down(f, st)) != MI_OK) return rc;
     } else {
         m = fp8_moe_cut((uint8_t *)workspace, T, k, E, D, I);
         const Fp8Prepare f = {x, m.xq, m.xs, idx, m.blk_expert, m.n_blocks, m.tok_row, m.row_slot, T, k, D, E, m.tm};

@@ -387,6 +387,14 @@ def test_moe_streams_up_to_16_slots(pkg, gpu, T, k, E):
         _close(of, want, bound)
 
 
+@pytest.mark.parametrize("T,E,k,D,I", [(1, 8, 8, 1104, 1072), (2, 8, 4, 1040, 1040), (4, 6, 2, 1296, 1040),
+                                       (8, 3, 1, 1168, 1040), (1, 9, 7, 1184, 1200)])
+def test_moe_streams_several_row_tiles(pkg, gpu, T, E, k, D, I):
+    """Few slots of wider layers, whose wavefronts take two row tiles of gate and up and four of down; the last ones
+    end inside a wavefront's."""
+    test_moe(pkg, gpu, T, E, k, D, I)
+
+
 def test_moe_no_live_slots(pkg, gpu):
     rng = np.random.default_rng(0)
     leaves = [_leaf(pkg, *r) for r in _experts(rng, 3, 256, 128)]
