@@ -6,11 +6,11 @@
 // wavefront.  An instruction's operands come from LDS as whole fragments (weights in use for CT instructions, tokens for
 // the whole step), its result is scaled and added by 4 fused multiply-adds.
 //
-// What bounds it: a step of 256 x 256 takes 3450 clocks where its matrix instructions take 2048 and 1720 are reached with
-// both loads and barriers left out; the loads cost 970 and the barrier 760 of them.  Those loads mostly wait for memory
-// under load, which takes longer to answer than the stages in flight last: weights that already are in the last-level
-// cache save up to a third.  4096 x 6144 x 6144 takes 198 us (1.56 PFLOP/s; a library's product with one scale for the
-// whole tensor takes 123), 64 experts of 2.4 GB read once for 200 tokens in 8 each 500 us (4.9 TB/s).
+// What bounds it: a step of 256 x 256 would take 72 % of its time without its loads and 50 %, about that of its matrix
+// instructions, with neither loads nor barriers.  The loads mostly wait for memory under load, which takes longer to answer
+// than the stages in flight last: weights that already are in the last-level cache save up to a third.  4096 x 6144 x 6144
+// takes 198 us (1.56 PFLOP/s; a library's product with one scale for the whole tensor takes 123), the routed layer's 2.4 GB
+// of weights for 200 tokens in 8 slots each 500 us (4.9 TB/s).
 //
 // Measured and not kept: touching lines two or three stages ahead from the same wavefronts (loads return in order, so they
 // are waited for as well: 3 to 13 % slower), two 128 x 128 workgroups per CU (20 % faster at 768 rows, up to 15 % slower at
@@ -26,7 +26,7 @@ namespace mi {
 constexpr int kFp8Near = 8;                      // token tiles of a weight tile that run next to each other
 constexpr int kFp8AheadLoads = 4;                // lines in flight of a lane that reads ahead
 constexpr int kFp8AheadRows = 512;               // weight rows that one workgroup reads ahead
-constexpr int kFp8MaxGroups = 512;              // K / 128: the weight scales of a tile's blocks are kept in LDS
+constexpr int kFp8MaxGroups = 512;               // K / 128: the weight scales of a tile's blocks are kept in LDS
 
 // Memory to LDS without registers: lane l's 16 (4) bytes to dst + 16 l (4 l).
 __device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint4 *dst, uint32_t voff, int soff) {

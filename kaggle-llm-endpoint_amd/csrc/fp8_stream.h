@@ -4,6 +4,10 @@
 // 128 columns, each holds U groups' weights in flight, quantises its own part of the activations in registers (a group of a
 // row is 32 values in each of 4 lanes: two exchanges give its maximum) and multiplies with one instruction per group and
 // tile; the W sums are added through LDS in wavefront order.
+//
+// Memory bounds it: one token's 8 experts of 6144 / 2048 take 38 us for gate and up (201 MB, 5.3 TB/s) and 21 us for down
+// (101 MB), a 6144 x 6144 matrix one row 9 us (4.1 TB/s, most of the rest its start).  The rows are quantised once in each
+// workgroup, which costs no pass over memory and, with several row tiles to serve, no time that the stream does not cover.
 #pragma once
 #include "fp8.h"
 
