@@ -647,9 +647,10 @@ extern "C" int mi_fp8_grouped(const void *x, int32_t x_dtype, const float *xs, i
 namespace mi {
 
 // A call of a few slots streams each expert's weights, without a plan (6144 / 2048, one and two tokens in 8 slots each: 65
-// and 113 us, sorted 78 and 124; 12 slots 87 to 90 and 98 to 105).  A larger one sorts its slots by expert and takes the tiled product, its blocks the smaller
-// the fewer rows an expert has (64 experts, top-8, 48 / 96 / 200 / 512 / 1999 tokens: 443 / 463 / 500 / 585 / 1170 us with
-// 16 / 32 / 64 / 128 / 256 rows; half the rows 6 to 20 % more from 96 tokens on, twice as many 2 to 14 % more).
+// and 113 us, sorted 78 and 124; 12 slots 87 to 90 and 98 to 105).  A larger one sorts its slots by expert and takes the
+// tiled product, its blocks the smaller the fewer rows an expert has (64 experts, top-8, 48 / 96 / 200 / 512 / 1999 tokens:
+// 443 / 463 / 500 / 585 / 1170 us with 16 / 32 / 64 / 128 / 256 rows; half the rows 6 to 20 % more from 96 tokens on, twice
+// as many 2 to 14 % more).
 constexpr int kFp8StreamSlots = kFp8TileSlots;
 static bool fp8_moe_streams(int S) { return S <= std::min(tuning(kTuneF8Stream, kFp8StreamSlots), kFp8TileSlots); }
 static int fp8_moe_tile(int S, int E) {
