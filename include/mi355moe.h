@@ -413,6 +413,8 @@ size_t mi_mlp_many_workspace(int32_t B, int32_t D, int32_t I);
  * (checkpoint.py:202), which the reference dequantises:
  *   wq [E, R, K] row-major, ws f32 [E, ceil(R / 128), ceil(K / 128)];  xq [rows, K], xs f32 [rows, ceil(K / 128)]
  *   y[b, o] = sum_c xs[b, c] ws[o / 128, c] sum_{i in group c} xq[b, i] wq[o, i]     exact products, f32 sums
+ * Weight scales may be any f32, xs 2^-100 to 2^120 as mi_fp8_quantize makes them: a product of the two that leaves f32 does
+ * not make the scaled sum wrong.
  * The last group and block may be partial.  K (n_in, D, I) % 16 == 0 and R, K <= 2^16; x and the weights 16-byte
  * aligned; rows * K < 2^31, at most 2^22 rows.
  *

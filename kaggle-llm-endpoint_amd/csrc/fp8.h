@@ -13,7 +13,8 @@ namespace mi {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kFp8Group = 128;                   // columns per scale; rows and columns per weight scale
-constexpr int kFp8MinExp = -100;                 // least scale 2^-100: a product of scales stays a normal f32
+constexpr int kFp8MaxGroups = 512;               // K / 128: the weight scales of a tile's blocks are kept in LDS
+constexpr int kFp8MinExp = -100;                 // least scale of a row's group: 2^-100
 constexpr uint32_t kFp8Out = 0x80000000u;        // a buffer offset past every range: reads zero
 constexpr int kFp8Word3 = 0x00020000;            // gfx9 buffer descriptor word 3 (32-bit data format)
 
@@ -27,6 +28,24 @@ __device__ __forceinline__ int fp8_exponent(uint32_t abits) {
     return max((int)((abits + 0x1fffffu) >> 23) - 135, kFp8MinExp);
 }
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// A group's sum is scaled by xs * ws.  xs is 2^-100 to 2^120, ws any f32, and as it stands their product may leave f32 where
+// the scaled sum does not: 2^120 times 2^8 is infinite, times a sum of 0 NaN.  So a row of weight blocks is computed with
+// its scales times 2^-n and its sums are multiplied by 2^n in the end, n by the largest of them: 0 from 2^-26 to below
+// 2^7, where xs * ws is a normal f32 (a checkpoint's scales are there, and keep their products and bits), otherwise what
+// brings the largest there.  Next to that one, a scale below 2^-26 of its size may still meet an xs with which the product
+// is subnormal: an error of at most 2^(n - 125) in its group's term.  (With an infinite scale the row has no finite output.)
+__device__ __forceinline__ int fp8_scale_shift(float largest) {
+    const int e = __builtin_amdgcn_frexp_expf(largest) - 1;          // 2^e <= largest < 2^(e + 1)
+    return !(largest > 0.0f && largest < INFINITY) ? 0 : e > 6 ? e - 6 : e < -26 ? e + 26 : 0;
+}
+// n of a wavefront's scales, m the largest magnitude among a lane's.
+__device__ __forceinline__ int fp8_wave_shift(float m) {
+    if (__ballot(m >= 0x1p7f) == 0 && __ballot(m >= 0x1p-26f) != 0) return 0;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    return __builtin_amdgcn_readfirstlane(fp8_scale_shift(m));
+}
 
 // Two values to e4m3 (nearest even), in the low or high half of `old`; |a|, |b| <= 448 or NaN.
 template <bool HI>

@@ -26,7 +26,6 @@ namespace mi {
 constexpr int kFp8Near = 8;                      // token tiles of a weight tile that run next to each other
 constexpr int kFp8AheadLoads = 4;                // lines in flight of a lane that reads ahead
 constexpr int kFp8AheadRows = 512;               // weight rows that one workgroup reads ahead
-constexpr int kFp8MaxGroups = 512;               // K / 128: the weight scales of a tile's blocks are kept in LDS
 
 // Memory to LDS without registers: lane l's 16 (4) bytes to dst + 16 l (4 l).
 __device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t r, uint4 *dst, uint32_t voff, int soff) {
@@ -199,6 +198,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int t = 0; t < CT; ++t) acc[r][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    int shift[2] = {0, 0};                       // of the scales (fp8_scale_shift); PAIR: of gate's and up's
     auto wrow = [&](int r) {                     // LDS row of row tile r; PAIR: gate tiles, then the same rows of up
         return PAIR ? (r / (RT / 2)) * (TW / 2) + wm * (TW / 2 / WM) + (r % (RT / 2)) * 16 : wm * (TW / WM) + 16 * r;
     };
@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
         i32x8 b[CU], w[4];
         f32x4 v[4];
         float x[CU], w0, w1, s[PAIR ? 2 : 1][CU], last[LAG];
+        const int own = PAIR || TW == 128 ? 0 : wm * 2 / WM;         // the block whose scales this wavefront uses first
         auto add = [&](int n, float sc) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[n / CU][n % CU][j] = fmaf(v[n & 3][j], sc, acc[n / CU][n % CU][j]);
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
             x[t] = sx[64 * wave + 16 * t + i];
         };
         auto read_sw = [&](int g) __attribute__((always_inline)) {
-            w0 = sw[PAIR || TW == 128 ? 0 : wm * 2 / WM][g];
+            w0 = sw[own][g];
             if (PAIR) w1 = sw[1][g];
         };
         // stage g in buf; the next stage in nbuf; buf takes stage g + NST
@@ -252,6 +253,10 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
                 for (int t = 0; t < CU; ++t) {
                     const int n = r * CU + t;
                     if (r == 0) {
+                        if (t == 0) {
+                            w0 = ldexpf(w0, -shift[0]);
+                            if (PAIR) w1 = ldexpf(w1, -shift[1]);
+                        }
                         s[0][t] = x[t] * w0;
                         if (PAIR) s[PAIR ? 1 : 0][t] = x[t] * w1;
                     }
@@ -272,6 +277,13 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
         for (int st = 0; st < NST; ++st)
 #pragma unroll
             for (int j = 0; j < PER; ++j) load_piece(bufs[st], sxs[st], t0 + st, past(t0 + st), j);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int m = 0; m < (PAIR ? 2 : 1); ++m) {   // while the first stages are on their way
+            float big = 0.0f;
+            for (int g = lane; g < KB; g += 64) big = fmaxf(big, fabsf(sw[PAIR ? m : own][g]));
+            shift[m] = fp8_wave_shift(big);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -300,6 +312,14 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) fp8_gemm_kernel(Fp8
     else if (CT >= 2 && ct >= 2) main_loop(std::integral_constant<int, CT >= 2 ? 2 : 1>{});
     else main_loop(std::integral_constant<int, 1>{});
     vm_wait<0>();
+    if (shift[0] | shift[1]) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[r][t][j] = ldexpf(acc[r][t][j], shift[PAIR ? r / (RT / 2) : 0]);
+    }
 
     // ---- lane (i, q) holds outputs 4 q .. 4 q + 3 of each row tile for row 16 t + i
     if constexpr (PAIR) {

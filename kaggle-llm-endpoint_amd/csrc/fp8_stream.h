@@ -174,12 +174,36 @@ __global__ void __launch_bounds__(64 * W, OCC) fp8_stream_kernel(Fp8Stream a) {
         for (int t = 0; t < NT; ++t) fp8_x_load<XD>(xv[u][t], rx, rs, xo[t], so[t], p0, p1, end, g);
     };
     f32x4 acc[M][RW][NT];
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int m = 0; m < M; ++m)
+        for (int m = 0; m < M; ++m)
 #pragma unroll
-        for (int r = 0; r < RW; ++r)
+            for (int r = 0; r < RW; ++r)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[m][r][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < NT; ++t) acc[m][r][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    };
+    // the group in place u of the ring, its weight scales as given
+    auto add = [&](int u, const float (&ws)[M]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float xs;
+            const i32x8 b = fp8_x_quantize<XD>(xv[u][t], xs);
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const float sc = xs * ws[m];
+#pragma unroll
+                for (int r = 0; r < RW; ++r) {
+                    const uint4 c0 = wv[u][m][r][0], c1 = wv[u][m][r][1];
+                    const f32x4 v = fp8_product<PAIR>((i32x8){(int)c0.x, (int)c0.y, (int)c0.z, (int)c0.w,
+                                                     (int)c1.x, (int)c1.y, (int)c1.z, (int)c1.w}, b);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[m][r][t][j] = fmaf(v[j], sc, acc[m][r][t][j]);
+                }
+            }
+        }
+    };
+    clear();
+    float big[M] = {};                           // the largest scale (fp8_scale_shift)
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         load(u, g0 + u);
@@ -189,27 +213,35 @@ __global__ void __launch_bounds__(64 * W, OCC) fp8_stream_kernel(Fp8Stream a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             // past the last group everything reads zero and adds zero
+            add(u, wsv[u]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                float xs;
-                const i32x8 b = fp8_x_quantize<XD>(xv[u][t], xs);
-#pragma unroll
-                for (int m = 0; m < M; ++m) {
-                    const float sc = xs * wsv[u][m];
-#pragma unroll
-                    for (int r = 0; r < RW; ++r) {
-                        const uint4 c0 = wv[u][m][r][0], c1 = wv[u][m][r][1];
-                        const f32x4 v = fp8_product<PAIR>((i32x8){(int)c0.x, (int)c0.y, (int)c0.z, (int)c0.w,
-                                                         (int)c1.x, (int)c1.y, (int)c1.z, (int)c1.w}, b);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) acc[m][r][t][j] = fmaf(v[j], sc, acc[m][r][t][j]);
-                    }
-                }
-            }
+            for (int m = 0; m < M; ++m) big[m] = fmaxf(big[m], fabsf(wsv[u][m]));
             __builtin_amdgcn_sched_barrier(0);
             load(u, g + u + U);
             __builtin_amdgcn_sched_barrier(0);
         }
+    }
+    int shift[M], any = 0;
+#pragma unroll
+    for (int m = 0; m < M; ++m) any |= shift[m] = fp8_wave_shift(big[m]);
+    if (any) {                                   // again, one group at a time, with this wavefront's scales shifted
+        clear();
+#pragma unroll 1
+        for (int g = g0; g < g1; ++g) {
+            load(0, g);
+            float ws[M];
+#pragma unroll
+            for (int m = 0; m < M; ++m) ws[m] = ldexpf(wsv[0][m], -shift[m]);
+            add(0, ws);
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int r = 0; r < RW; ++r)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[m][r][t][j] = ldexpf(acc[m][r][t][j], shift[m]);
     }
 
 #pragma unroll
