@@ -9,11 +9,12 @@ scale per 128 x 128 block, contracted as fp8 on the matrix cores with activation
 
 Everything runs on the current torch (HIP) stream of the current device.  The weights are a checkpoint's and the
 products have no gradient: an input (rows, scales, routing weights) that requires one is refused while gradients are
-recorded.  Outputs and workspaces must not overlap the inputs or each other.
+recorded, and one that carries a forward-mode tangent always.  Outputs and workspaces must not overlap the inputs or each other.
 """
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
@@ -72,7 +73,16 @@ def _stream_of(who, *tensors):
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
+def _no_tangent(who, *tensors):
+    """A tangent would be lost without a word: a dual tensor does not require a gradient, and its address is read."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("%s has no forward-mode derivative: call it on the primal (forward_ad.unpack_dual)" % who)
+
+
 def _no_grad(who, t):
+    _no_tangent(who, t)
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("%s has no gradient: detach its inputs or call it under torch.no_grad()" % who)
 

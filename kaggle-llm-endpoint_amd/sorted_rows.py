@@ -5,16 +5,16 @@ combine around the ragged products (resident.py:153-165), with their gradients:
     xs   = moe_dispatch(x, plan)            [Rp, D]; the experts' products of xs give y [Rp, D]
     out  = moe_combine(y, plan, w)          [T, D]
 
-Both record gradients (x; y and w), first order only, and save no copies: the rows a backward pass reads are the
-forward's own inputs.  Deterministic: no atomics, sums in f32 in column order, one rounding.  A captured backward pass
-needs leaves of its own (``x.detach().requires_grad_()`` inside the capture): an eager graph that still holds the same
-leaves has bound their gradients to another stream.
+Both record gradients (x; y and w), first order and reverse mode only (a forward-mode tangent is refused), and save no
+copies: the rows a backward pass reads are the forward's own inputs.  Deterministic: no atomics, sums in f32 in column
+order, one rounding.  A captured backward pass needs leaves of its own (``x.detach().requires_grad_()`` inside the
+capture): an eager graph that still holds the same leaves has bound their gradients to another stream.
 """
 import torch
 from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
-from .fp8 import _DTYPES, _aligned, _stream_of
+from .fp8 import _DTYPES, _aligned, _no_tangent, _stream_of
 from .resident import _as, _ptr, _stream
 
 
@@ -59,6 +59,7 @@ class _Dispatch(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gxs):
         slot, = ctx.saved_tensors
+        _no_tangent("moe_dispatch's gradient", gxs)
         return _combine(_aligned(gxs), slot, None), None, None
 
 
@@ -72,6 +73,7 @@ class _Combine(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, gout):
         y, w, tok, slot = ctx.saved_tensors
+        _no_tangent("moe_combine's gradient", gout)
         gout = _aligned(gout)
         T, k = slot.shape
         dy, dw = torch.empty_like(y), torch.empty_like(w)
@@ -86,6 +88,7 @@ def moe_dispatch(x, plan):
     xs [Rp, D] of x's dtype, xs[row_slot[t, j]] = x[t], zeros on all other rows (padding, and rows of slots that the
     caller has taken out: row_slot -1).  Records the gradient of x: the sum over a token's rows."""
     _rows_dtype(x, "moe_dispatch")
+    _no_tangent("moe_dispatch", x)
     tok, slot = _plan_rows(plan)
     if slot.shape[0] != x.shape[0]:
         raise ValueError("moe_dispatch: the plan is of %d tokens, x has %d" % (slot.shape[0], x.shape[0]))
@@ -101,6 +104,7 @@ def moe_combine(y, plan, w):
     sum_j w[t, j] * y[row_slot[t, j]] in f32, in column order, rounded once; a slot without a row (an expert id outside
     [0, E), or row_slot set to -1) adds nothing.  Records the gradients of y (zeros on rows without a slot) and w."""
     _rows_dtype(y, "moe_combine")
+    _no_tangent("moe_combine", y, w)
     tok, slot = _plan_rows(plan)
     if tok.numel() != y.shape[0]:
         raise ValueError("moe_combine: the plan has %d rows, y %d" % (tok.numel(), y.shape[0]))
