@@ -8,7 +8,7 @@ scale per 128 x 128 block, contracted as fp8 on the matrix cores with activation
     o, _ = fp8_moe(gate, up, down, x, idx, w, limit)    the routed experts of a layer
 
 Everything runs on the current torch (HIP) stream of the current device.  The weights are a checkpoint's and the
-products have no gradient: an input (rows, scales, routing weights) that requires one is refused while gradients are
+products have no gradient: an input (rows, weights, scales, routing weights) that requires one is refused while gradients are
 recorded, and one that carries a forward-mode tangent always.  Outputs and workspaces must not overlap the inputs or each other.
 """
 from typing import NamedTuple
@@ -59,7 +59,7 @@ def _leaf_dims(leaf, who):
         raise ValueError("%s: scales %s do not fit weights %s: one per 128 x 128 block" % (who, tuple(ss), tuple(qs)))
     if not (q.is_contiguous() and s.is_contiguous()):
         raise ValueError("%s: weights and scales must be contiguous (fp8_leaf makes them so)" % who)
-    _no_grad(who, s)
+    _no_grad(who, q, s)
     return E, R, K
 
 
@@ -81,9 +81,9 @@ def _no_tangent(who, *tensors):
                 raise RuntimeError("%s has no forward-mode derivative: call it on the primal (forward_ad.unpack_dual)" % who)
 
 
-def _no_grad(who, t):
-    _no_tangent(who, t)
-    if t.requires_grad and torch.is_grad_enabled():
+def _no_grad(who, *tensors):
+    _no_tangent(who, *tensors)
+    if any([t.requires_grad for t in tensors]) and torch.is_grad_enabled():
         raise RuntimeError("%s has no gradient: detach its inputs or call it under torch.no_grad()" % who)
 
 
@@ -124,7 +124,7 @@ def _rows_of(x, K, who):
             raise TypeError("%s: quantised activations are (float8_e4m3fn, float32 scales)" % who)
         if q.dim() != 2 or tuple(s.shape) != (q.shape[0], _blocks(q.shape[1])):
             raise ValueError("%s: quantised activations are q [B, n_in] with s [B, ceil(n_in / 128)]" % who)
-        _no_grad(who, s)
+        _no_grad(who, q, s)
         x, xs, dtype = _aligned(q), s.contiguous(), _lib.MI_X_FP8
     else:
         xs, dtype = None, _DTYPES.get(x.dtype)

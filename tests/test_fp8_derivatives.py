@@ -95,3 +95,21 @@ def test_function_transforms_are_refused(host, name):
         torch.func.grad(lambda t: first(t).sum())(x)
     with pytest.raises(RuntimeError):
         torch.func.vmap(first)(torch.stack([x, x]))
+
+
+@pytest.mark.parametrize("what", ["rows", "weights"])
+def test_e4m3_values_that_require_a_gradient_are_refused(host, what):
+    """``t.to(torch.float8_e4m3fn)`` records a gradient: quantised rows and weights made so are refused like scales."""
+    leaf, x = _leaf(host, 100, 256), torch.ones((5, 256))
+    rows = lambda t: host.fp8_project((t.to(F8), torch.ones((5, 2))), leaf)
+    weights = lambda t: host.fp8_project(x, host.Fp8Leaf(t.to(F8), leaf.s))
+    f, t = (rows, x) if what == "rows" else (weights, torch.ones((100, 256)))
+    f(t)
+    t = t.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        f(t)
+    with torch.no_grad():
+        f(t)
+    f(t.detach())
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        f(forward_ad.make_dual(t.detach(), torch.ones_like(t)))
