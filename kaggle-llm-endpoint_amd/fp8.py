@@ -110,6 +110,8 @@ def _workspace(workspace, need, device):
         if need == 0:
             return None, None, 0
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    elif not workspace.is_contiguous():
+        raise ValueError("a workspace must be contiguous: a view's elements may be more than its memory")
     return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 

@@ -263,3 +263,31 @@ def test_scales_that_require_a_gradient_are_refused(pkg):
     with torch.no_grad():
         assert pkg.fp8._leaf_dims(with_grad, "fp8_project") == (0, 100, 256)
     assert not pkg.fp8_leaf({"q": leaf.q, "s": torch.nn.Parameter(leaf.s)}, device="cpu").s.requires_grad
+
+
+@pytest.mark.parametrize("name,arg", [("mi_fp8_project", 10), ("mi_fp8_mlp", 15), ("mi_fp8_moe", 18),
+                                      ("mi_fp8_grouped", 15)])
+def test_a_workspace_is_as_long_as_its_memory(pkg, monkeypatch, name, arg):
+    """The bytes that a call is told of lie behind the address that it is given: an expanded or strided view has more
+    elements, or a wider span, than memory of its own."""
+    fake = _Lib(name, arg + 1)
+    monkeypatch.setattr(pkg.fp8, "lib", lambda: fake)
+    monkeypatch.setattr(pkg.fp8, "_stream_of", lambda *a: 0)
+    bf = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
+    g, d = _leaf(pkg, 144, 256, 3), _leaf(pkg, 256, 144, 3)
+    one = [pkg.Fp8Leaf(l.q[0], l.s[0]) for l in (g, g, d)]
+    plan = {"blk_expert": torch.zeros(4, dtype=torch.int32), "n_blocks": torch.ones(1, dtype=torch.int32),
+            "tok_row": torch.zeros(64, dtype=torch.int32), "row_slot": torch.zeros((5, 2), dtype=torch.int32)}
+    call = {"mi_fp8_project": lambda ws: pkg.fp8_project(bf(40, 256), one[0], workspace=ws),
+            "mi_fp8_mlp": lambda ws: pkg.fp8_mlp(bf(40, 256), *one, 7.0, workspace=ws),
+            "mi_fp8_moe": lambda ws: pkg.fp8_moe(g, g, d, bf(4, 256), torch.zeros((4, 2), dtype=torch.int32),
+                                                 torch.zeros(4, 2), 7.0, workspace=ws),
+            "mi_fp8_grouped": lambda ws: pkg.fp8_grouped(bf(64, 256), plan, g, workspace=ws)}[name]
+    buf = torch.zeros(1 << 16, dtype=torch.uint8)
+    for ws, size in ((buf, 1 << 16), (buf.view(256, 256), 1 << 16), (buf.view(torch.int32), 1 << 16), (buf[256:], 65280)):
+        call(ws)
+        assert fake.seen.pop() == size
+    for ws in (buf[:1].expand(1 << 16), buf[:256].expand(256, 256), buf[::2], buf.view(256, 256).t(), buf.view(256, 256)[:, :128]):
+        with pytest.raises(ValueError, match="workspace"):
+            call(ws)
+    assert not fake.seen
