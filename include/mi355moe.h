@@ -418,7 +418,8 @@ size_t mi_mlp_many_workspace(int32_t B, int32_t D, int32_t I);
  * The last group and block may be partial.  K (n_in, D, I) % 16 == 0 and R, K <= 2^16; x and the weights 16-byte
  * aligned; rows * K < 2^31, at most 2^22 rows.
  *
- * mi_fp8_quantize: n rows of K bf16 or f32 values, row stride x_stride elements (a multiple of 8) -> q, s:
+ * mi_fp8_quantize: n rows of K bf16 or f32 values, row stride x_stride elements (a multiple of 8), n * ceil(K / 128) < 2^28
+ * (rows * K may be more) -> q, s:
  *   a = max |x| of the group's finite values, s = 2^e with the least e >= -100 such that a <= 448 * 2^e,
  *   q = e4m3(x / s) rounded to nearest even; infinities and NaN become NaN.
  *   The scale is a power of two: x / s is exact, each value is rounded once.

@@ -505,6 +505,7 @@ extern "C" int mi_fp8_quantize(const void *x, int32_t x_dtype, int32_t n, int32_
     if (x_dtype != MI_X_BF16 && x_dtype != MI_X_F32) return MI_ERR_ARG;
     if (n <= 0 || n > kFp8MaxRows) return MI_ERR_TOKENS;
     if (!fp8_cols_ok(K)) return MI_ERR_SHAPE;
+    if ((long long)n * fp8_groups(K) >= (1ll << 28)) return MI_ERR_TOKENS;         // 16 threads each: a grid's 2^32
     if (x_stride < K || x_stride % 8 || x_stride > (1ll << 40)) return MI_ERR_ARG;
     if (!aligned16(x) || !aligned16(q) || !aligned4(s)) return MI_ERR_ARG;
     return fp8_launch_quantize(x, x_dtype, n, K, x_stride, nullptr, q, s, (hipStream_t)stream);
