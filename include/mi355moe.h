@@ -412,7 +412,14 @@ size_t mi_mlp_many_workspace(int32_t B, int32_t D, int32_t I);
  * group of 128 columns; weights: e4m3 with one f32 scale per 128 x 128 block, the layout of fp8 checkpoints
  * (checkpoint.py:202), which the reference dequantises:
  *   wq [E, R, K] row-major, ws f32 [E, ceil(R / 128), ceil(K / 128)];  xq [rows, K], xs f32 [rows, ceil(K / 128)]
- *   y[b, o] = sum_c xs[b, c] ws[o / 128, c] sum_{i in group c} xq[b, i] wq[o, i]     exact products, f32 sums
+ *   y[b, o] = sum_c xs[b, c] ws[o / 128, c] sum_{i in group c} xq[b, i] wq[o, i]
+ * The products are exact.  The fp8 matrix instruction adds those of 8 consecutive columns on a grid of 2^-13 of the
+ * largest one's power of two and cuts what is below; these sums, a group's, the groups' and the splits' are added in f32.
+ * So y, y_f32 too, is off by at most 7 * 2^-13 of the largest product per 8 columns besides f32 roundings: 1.3e-5 of the
+ * result (root mean square) on ordinary values.  Gate and up of mi_fp8_mlp with B <= 128 and of mi_fp8_moe with
+ * T * k / E <= 96 (or T * k <= 16) add every product in f32 instead, because h is quantised again and a last bit there may
+ * move a value by a step of e4m3; of larger calls they do not.  A row's result may therefore differ, within these bounds, with
+ * the number of rows in its call.
  * Weight scales may be any f32, xs 2^-100 to 2^120 as mi_fp8_quantize makes them: a product of the two that leaves f32 does
  * not make the scaled sum wrong.
  * The last group and block may be partial.  K (n_in, D, I) % 16 == 0 and R, K <= 2^16; x and the weights 16-byte
@@ -430,7 +437,7 @@ int mi_fp8_quantize(const void *x, int32_t x_dtype, int32_t n, int32_t K, int64_
 
 /*
  * Dense block-scaled product, 1 <= B tokens: x bf16 or f32 [B, n_in] (quantised as by mi_fp8_quantize; xs NULL) or
- * MI_X_FP8 values with their scales xs.  y_bf16 (one rounding of the f32 sum) and/or y_f32 [B, n_out], any n_out.
+ * MI_X_FP8 values with their scales xs.  y_bf16 (y_f32 rounded once) and/or y_f32 [B, n_out], any n_out.
  * Workspace: mi_fp8_project_workspace bytes, 16-byte aligned, no initialisation; its size serves every smaller B.  Up to
  * 32 rows need none (the size is 0, as for a shape that the call refuses).
  */
@@ -441,8 +448,8 @@ size_t mi_fp8_project_workspace(int32_t B, int32_t n_in, int32_t n_out);
 
 /*
  * mlp_partial (model.py:125-127) over block-scaled leaves: g, u = x Wg^T, x Wu^T (f32, not rounded),
- * h = silu(min(g, L)) * clip(u, -L, L) in f32, quantised as by mi_fp8_quantize, y = h Wd^T.  gate, up [I, D], down [D, I].
- * x and the workspace as for mi_fp8_project.
+ * h = silu(min(g, L)) * clip(u, -L, L) in f32, L > 0, quantised as by mi_fp8_quantize, y = h Wd^T.  gate, up [I, D], down
+ * [D, I].  x and the workspace as for mi_fp8_project.
  */
 int mi_fp8_mlp(const void *x, int32_t x_dtype, const float *xs, int32_t B, int32_t D, int32_t I,
                const uint8_t *gate_q, const float *gate_s, const uint8_t *up_q, const float *up_s,
@@ -464,7 +471,7 @@ size_t mi_fp8_grouped_workspace(int32_t rows, int32_t K, int32_t R);
 
 /*
  * The routed experts of one layer (ResidentFetch.apply's composition, resident.py:100-120) over block-scaled weights:
- *   out[t] = sum_j w[t, j] MLP_{idx[t, j]}(x[t])      MLP as mi_fp8_mlp, its y and the sum in f32, columns in order
+ *   out[t] = sum_j w[t, j] MLP_{idx[t, j]}(x[t])      MLP as mi_fp8_mlp, its y kept in f32, the sum in f32, columns in order
  * x bf16 or f32 [T, D], idx int32 [T, k], w f32 [T, k]; out_f32 and/or out_bf16 [T, D].  A slot whose expert id is
  * outside [0, E) adds nothing.  E <= 1024, T * k <= 2^22.  Workspace as for mi_fp8_project.
  */
@@ -481,7 +488,7 @@ size_t mi_fp8_moe_workspace(int32_t T, int32_t k, int32_t E, int32_t D, int32_t 
  *   mi_moe_dispatch      xs[row_slot[t, j]] = x[t], zeros on all other rows
  *   mi_moe_combine       out[t] = sum_j w[t, j] y[row_slot[t, j]]; w NULL: weights 1 (dispatch's gradient)
  *   mi_moe_combine_grad  dy[row_slot[t, j]] = w[t, j] dout[t], zeros on all others; dw[t, j] = <dout[t], y[row_slot[t, j]]>
- * tok_row[row_slot[t, j]] is t, as the plan has it.  A slot without a row (row_slot -1: an expert id outside [0, E), or
+ * At least one token.  tok_row[row_slot[t, j]] is t, as the plan has it, and no two slots share a row.  A slot without a row (row_slot -1: an expert id outside [0, E), or
  * taken out by the caller) adds nothing and gets dw 0.
  */
 int mi_moe_dispatch(const void *x, int32_t dtype, int32_t T, int32_t k, int32_t D, const int32_t *row_slot,
@@ -502,8 +509,8 @@ int mi_moe_combine_grad(const void *dout, const void *y, int32_t dtype, int32_t 
  * splits and token tile (DG_S1, DG_S2, DG_NT), the prefill's wide blocks (PF_WIDE), the dense fp8 product's tile and
  * splits (F8_TW, F8_TT, F8_S) and the fp8 routed layer's streaming limit and rows per block (F8_STREAM, F8_TM).
  * Overrides change launch shapes and summation orders, never the result beyond f32 rounding (of the fp8 MLP and routed
- * layer: beyond that of h before it is rounded to e4m3); workspace sizes follow them, so set them before sizing a
- * workspace.  Not synchronised with calls running on other host threads.
+ * layer: beyond what that moves of h when it is rounded to e4m3, and F8_TM or F8_TT above 128 takes gate and up from f32
+ * sums to the fp8 instruction's); workspace sizes follow them, so set them before sizing a workspace.  Not synchronised with calls running on other host threads.
  */
 int mi_tuning_set(const char *name, int32_t value);
 void mi_tuning_reset(void);

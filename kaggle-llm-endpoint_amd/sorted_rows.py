@@ -9,6 +9,10 @@ Both record gradients (x; y and w), first order and reverse mode only (a forward
 copies: the rows a backward pass reads are the forward's own inputs.  Deterministic: no atomics, sums in f32 in column
 order, one rounding.  A captured backward pass needs leaves of its own (``x.detach().requires_grad_()`` inside the
 capture): an eager graph that still holds the same leaves has bound their gradients to another stream.
+
+The products of this package have no gradient with respect to the rows (fp8_grouped refuses rows that require one), so a
+gradient of x, or of y, flows through products of the caller's own between the two; that of w needs none.  A plan has at
+least one token, and no two of its slots share a row.
 """
 import torch
 from torch.autograd.function import once_differentiable
