@@ -252,7 +252,7 @@ def fp8_grouped(xs, plan, leaf, want_f32=False, y_bf16=None, y_f32=None, workspa
 def fp8_moe(gate, up, down, x, idx, w, limit, want_f32=True, want_bf16=False, out_f32=None, out_bf16=None,
             workspace=None):
     """The routed experts of one layer over block-scaled weights, for one token or a whole prompt piece: out[t] =
-    sum_j w[t, j] * MLP_{idx[t, j]}(x[t]) with the MLP of fp8_mlp, whose y stays f32 until the sum is rounded.  gate, up [E, I, D], down [E, D, I] (Fp8Leaf); x bf16 or f32 [T, D]; idx int32 [T, k]; w f32 [T, k] ->
+    sum_j w[t, j] * MLP_{idx[t, j]}(x[t]) with the MLP of fp8_mlp, whose y stays f32 until the sum is rounded.  gate, up [E, I, D], down [E, D, I] (Fp8Leaf); x bf16 or f32 [T, D]; idx int32 (or int64) [T, k]; w f32 [T, k] ->
     (out_f32 [T, D] or None, out_bf16 [T, D] or None).  A slot whose expert id is outside [0, E) adds nothing.
     Preallocated outputs and ``workspace`` (mi_fp8_moe_workspace bytes) make the call allocation-free."""
     E, I, D = _mlp_dims(gate, up, down, "fp8_moe")
@@ -264,6 +264,8 @@ def fp8_moe(gate, up, down, x, idx, w, limit, want_f32=True, want_bf16=False, ou
     if idx.dim() != 2 or w.shape != idx.shape or idx.shape[0] != x.shape[0]:
         raise ValueError("fp8_moe: idx and w must be [T, k] for the %d tokens of x" % x.shape[0])
     _no_grad("fp8_moe", w)
+    if idx.dtype == torch.int64:
+        idx = idx.clamp(-1, E)                    # (an id outside the range must not wrap into it)
     idx, w = _as(idx, torch.int32), _as(w, torch.float32)
     T, k = idx.shape
     of, ob = out_f32, out_bf16
