@@ -252,9 +252,10 @@ def fp8_grouped(xs, plan, leaf, want_f32=False, y_bf16=None, y_f32=None, workspa
 def fp8_moe(gate, up, down, x, idx, w, limit, want_f32=True, want_bf16=False, out_f32=None, out_bf16=None,
             workspace=None):
     """The routed experts of one layer over block-scaled weights, for one token or a whole prompt piece: out[t] =
-    sum_j w[t, j] * MLP_{idx[t, j]}(x[t]) with the MLP of fp8_mlp, whose y stays f32 until the sum is rounded.  gate, up [E, I, D], down [E, D, I] (Fp8Leaf); x bf16 or f32 [T, D]; idx int32 (or int64) [T, k]; w f32 [T, k] ->
-    (out_f32 [T, D] or None, out_bf16 [T, D] or None).  A slot whose expert id is outside [0, E) adds nothing.
-    Preallocated outputs and ``workspace`` (mi_fp8_moe_workspace bytes) make the call allocation-free."""
+    sum_j w[t, j] * MLP_{idx[t, j]}(x[t]) with the MLP of fp8_mlp, whose y stays f32 until the sum is rounded.  gate, up
+    [E, I, D], down [E, D, I] (Fp8Leaf); x bf16 or f32 [T, D]; idx int32 (or int64) [T, k]; w f32 [T, k] -> (out_f32 [T, D]
+    or None, out_bf16 [T, D] or None).  A slot whose expert id is outside [0, E) adds nothing.  Preallocated outputs and
+    ``workspace`` (mi_fp8_moe_workspace bytes) make the call allocation-free."""
     E, I, D = _mlp_dims(gate, up, down, "fp8_moe")
     if not E:
         raise ValueError("fp8_moe: gate, up and down must be [E, ..] experts")
