@@ -488,6 +488,7 @@ size_t mi_fp8_moe_workspace(int32_t T, int32_t k, int32_t E, int32_t D, int32_t 
  *   mi_moe_dispatch      xs[row_slot[t, j]] = x[t], zeros on all other rows
  *   mi_moe_combine       out[t] = sum_j w[t, j] y[row_slot[t, j]]; w NULL: weights 1 (dispatch's gradient)
  *   mi_moe_combine_grad  dy[row_slot[t, j]] = w[t, j] dout[t], zeros on all others; dw[t, j] = <dout[t], y[row_slot[t, j]]>
+ *                        dw NULL: dy alone, y is not read and may be NULL
  * At least one token.  tok_row[row_slot[t, j]] is t, as the plan has it, and no two slots share a row.  A slot without a row (row_slot -1: an expert id outside [0, E), or
  * taken out by the caller) adds nothing and gets dw 0.
  */

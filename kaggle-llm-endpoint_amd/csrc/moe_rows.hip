@@ -123,9 +123,9 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(const void *__restrict
     }
 }
 
-// The first workgroups zero the rows without a slot, the others take one token each (302 us forward and backward of 4096
+// DW: the gradient of w too, which y is read for.  The first workgroups zero the rows without a slot, the others take one token each (302 us forward and backward of 4096
 // tokens with the zeros last, 297 with them first; dispatch takes 101 and 105: last there).
-template <int XD>
+template <int XD, bool DW>
 __global__ void __launch_bounds__(256) moe_combine_grad_kernel(const void *__restrict__ dout, const void *__restrict__ y,
                                                                const int32_t *__restrict__ row_slot,
                                                                const int32_t *__restrict__ tok_row,
@@ -145,15 +145,16 @@ __global__ void __launch_bounds__(256) moe_combine_grad_kernel(const void *__res
             for (int c = threadIdx.x * 8; c < D; c += 2048) {
                 Row8<XD> g, v;
                 g.load(dout, (size_t)t * D + c);
-                v.load(y, (size_t)r * D + c);
+                if constexpr (DW) v.load(y, (size_t)r * D + c);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    dot = fmaf(g.v[i], v.v[i], dot);
+                    if constexpr (DW) dot = fmaf(g.v[i], v.v[i], dot);
                     g.v[i] *= wt;
                 }
                 g.store(dy, (size_t)r * D + c);
             }
         }
+        if constexpr (!DW) continue;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) dot += __shfl_xor(dot, m, 64);
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
@@ -206,11 +207,12 @@ extern "C" int mi_moe_combine(const void *y, int32_t dtype, int32_t T, int32_t k
 extern "C" int mi_moe_combine_grad(const void *dout, const void *y, int32_t dtype, int32_t T, int32_t k, int32_t D,
                                    const int32_t *row_slot, const int32_t *tok_row, const float *w, int32_t rows,
                                    void *dy, float *dw, void *stream) {
-    if (!dout || !y || !row_slot || !tok_row || !w || !dy || !dw) return MI_ERR_NULL;
+    if (!dout || (dw && !y) || !row_slot || !tok_row || !w || !dy) return MI_ERR_NULL;
     const int rc = moe_rows_check(dtype, T, k, D, rows);
     if (rc != MI_OK) return rc;
     if (!moe_rows_aligned(dout, y, dy) || !words_aligned(row_slot, tok_row, w) || !words_aligned(dw)) return MI_ERR_ARG;
-    auto kern = dtype == MI_X_BF16 ? moe_combine_grad_kernel<MI_X_BF16> : moe_combine_grad_kernel<MI_X_F32>;
+    auto kern = dtype == MI_X_BF16 ? dw ? moe_combine_grad_kernel<MI_X_BF16, true> : moe_combine_grad_kernel<MI_X_BF16, false>
+                                   : dw ? moe_combine_grad_kernel<MI_X_F32, true> : moe_combine_grad_kernel<MI_X_F32, false>;
     hipLaunchKernelGGL(kern, dim3(T + (rows + kPadRows - 1) / kPadRows), dim3(256), 0, (hipStream_t)stream, dout, y,
                        row_slot, tok_row, w, T, k, D,
                        rows, dy, dw);

@@ -6,9 +6,10 @@ combine around the ragged products (resident.py:153-165), with their gradients:
     out  = moe_combine(y, plan, w)          [T, D]
 
 Both record gradients (x; y and w), first order and reverse mode only (a forward-mode tangent is refused), and save no
-copies: the rows a backward pass reads are the forward's own inputs.  Deterministic: no atomics, sums in f32 in column
-order, one rounding.  A captured backward pass needs leaves of its own (``x.detach().requires_grad_()`` inside the
-capture): an eager graph that still holds the same leaves has bound their gradients to another stream.
+copies: the rows a backward pass reads are the forward's own inputs (y only where w requires a gradient).  Deterministic:
+no atomics, sums in f32 in column order, one rounding.  A captured backward pass needs leaves of its own
+(``x.detach().requires_grad_()`` inside the capture): an eager graph that still holds the same leaves has bound their
+gradients to another stream.
 
 The products of this package have no gradient with respect to the rows (fp8_grouped refuses rows that require one), so a
 gradient of x, or of y, flows through products of the caller's own between the two; that of w needs none.  A plan has at
@@ -70,7 +71,7 @@ class _Dispatch(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, w, tok, slot):
-        ctx.save_for_backward(y, w, tok, slot)
+        ctx.save_for_backward(y if ctx.needs_input_grad[1] else None, w, tok, slot)     # only dw is made of y
         return _combine(y, slot, w)
 
     @staticmethod
@@ -80,10 +81,12 @@ class _Combine(torch.autograd.Function):
         _no_tangent("moe_combine's gradient", gout)
         gout = _aligned(gout)
         T, k = slot.shape
-        dy, dw = torch.empty_like(y), torch.empty_like(w)
+        rows, D = tok.numel(), gout.shape[1]
+        dy = torch.empty((rows, D), dtype=gout.dtype, device=gout.device)
+        dw = torch.empty_like(w) if y is not None else None
         check("mi_moe_combine_grad",
-              lib().mi_moe_combine_grad(_ptr(gout), _ptr(y), _DTYPES[y.dtype], T, k, y.shape[1], _ptr(slot), _ptr(tok),
-                                        _ptr(w), y.shape[0], _ptr(dy), _ptr(dw), _stream()))
+              lib().mi_moe_combine_grad(_ptr(gout), _ptr(y), _DTYPES[gout.dtype], T, k, D, _ptr(slot), _ptr(tok), _ptr(w),
+                                        rows, _ptr(dy), _ptr(dw), _stream()))
         return dy, dw, None, None
 
 
