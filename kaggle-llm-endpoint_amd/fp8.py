@@ -88,9 +88,11 @@ def _no_tangent(who, *tensors):
 
 
 def _no_grad(who, *tensors):
-    _no_tangent(who, *tensors)
-    if any([t.requires_grad for t in tensors]) and torch.is_grad_enabled():
-        raise RuntimeError("%s has no gradient: detach its inputs or call it under torch.no_grad()" % who)
+    if forward_ad._current_level >= 0:
+        _no_tangent(who, *tensors)
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("%s has no gradient: detach its inputs or call it under torch.no_grad()" % who)
 
 
 def _aligned(t):
