@@ -404,7 +404,9 @@ static int fp8_launch_dense_pair(Fp8Gemm a, float limit, uint8_t *hq, float *hs,
 }
 
 // ---- the streaming product
-constexpr int kFp8StreamRows = 32;               // rows that the dense streaming kernels take
+// Rows that the dense streaming kernels take.  6144 x 6144: 24 / 32 bf16 rows streamed 18.0 / 20.1 us, 40 tiled 18.5; an MLP of
+// 6144 / 2048: 32 rows streamed 32.5, 33 tiled 34.1.
+constexpr int kFp8StreamRows = 32;
 
 template <int XD, int NT, int RW, bool PAIR, bool SLOTS, int W, int U, int OCC>
 static int fp8_launch_stream_as(const Fp8Stream &a, hipStream_t st) {

@@ -5,9 +5,13 @@
 // row is 32 values in each of 4 lanes: two exchanges give its maximum) and multiplies with one instruction per group and
 // tile; the W sums are added through LDS in wavefront order.
 //
-// Memory bounds it: one token's 8 experts of 6144 / 2048 take 38 us for gate and up (201 MB, 5.3 TB/s) and 21 us for down
-// (101 MB), a 6144 x 6144 matrix one row 9 us (4.1 TB/s, most of the rest its start).  The rows are quantised once in each
-// workgroup, which costs no pass over memory and, with several row tiles to serve, no time that the stream does not cover.
+// Memory bounds it: one token's 8 experts of 6144 / 2048 take 38 us for gate and up (201 MB, 5.3 TB/s) and 22 us for down
+// (101 MB), a 6144 x 6144 matrix one row 9.5 us (4.0 TB/s, most of the rest its start; 11.5 if none of it is in the
+// last-level cache).  The rows are quantised once in each workgroup, which costs no pass over memory and, with several row
+// tiles to serve, no time that the stream does not cover.
+//
+// Scales that need a shift (fp8_scale_shift) are found as they go by, and the wavefront's groups are then taken a second
+// time.  (Its scales looked through beforehand, from loads ahead of the ring's, cost one row's MLP 0.8 us of 17, this 0.5.)
 #pragma once
 #include "fp8.h"
 
