@@ -24,6 +24,7 @@
  *                                                                                   mi_bf16_project
  *   fp8 checkpoint weights (dequant_fp8_device)            checkpoint.py:202     -> mi_fp8_project, mi_fp8_mlp, mi_fp8_moe
  *   gather and combine around the ragged products          resident.py:153-165   -> mi_moe_dispatch, mi_moe_combine
+ *   routing from logits, with groups and a gradient        (moe_route's selection, model.py:798-808) -> mi_moe_gate
  */
 #ifndef MI355MOE_H
 #define MI355MOE_H
@@ -499,6 +500,50 @@ int mi_moe_combine(const void *y, int32_t dtype, int32_t T, int32_t k, int32_t D
 int mi_moe_combine_grad(const void *dout, const void *y, int32_t dtype, int32_t T, int32_t k, int32_t D,
                         const int32_t *row_slot, const int32_t *tok_row, const float *w, int32_t rows, void *dy,
                         float *dw, void *stream);
+
+/*
+ * Root-mean-square norm of T rows of D values (bf16 or f32, dtype; D % 8 == 0, D <= 32768, T <= 2^22), with the residual's
+ * addition before it (the norms around the blocks whose products are above):
+ *   s = x + residual, rounded to dtype (s = x where residual is NULL; else written to stream_out, if that is given)
+ *   r = f32(1 / sqrt(mean(s^2) + eps)), the squares added in 64 bits, 0 <= eps <= 1e30
+ *   y = (s * r) * w, each product rounded to f32
+ * y to dtype and/or q, qs as mi_fp8_quantize makes them of the f32 values (both or neither; D % 16 == 0 then); rstd: r [T],
+ * for the gradient, or NULL.  w [D] of w_dtype (bf16 or f32).  x and residual have row strides in elements (multiples of 8),
+ * the outputs are contiguous.  Rows 16-byte aligned.
+ *
+ * mi_rms_norm_grad: s the rows that were normalised, dstream the gradient of stream_out (NULL: none), g = dy * w, n = s * r:
+ *   dx = r * (g - n * mean(g * n)) + dstream (x's and the residual's), dw = sum_t dy[t] * n[t] of w_dtype, NULL: not asked.
+ * Sums in f32 in a fixed order.  Workspace (with dw): mi_rms_norm_grad_workspace bytes, 16-byte aligned, no initialisation.
+ */
+int mi_rms_norm(const void *x, int32_t dtype, int64_t x_stride, const void *residual, int64_t residual_stride,
+                const void *w, int32_t w_dtype, int32_t T, int32_t D, double eps, void *y, void *stream_out, float *rstd,
+                uint8_t *q, float *qs, void *stream);
+int mi_rms_norm_grad(const void *dy, const void *s, int32_t dtype, int64_t s_stride, const void *dstream, const void *w,
+                     int32_t w_dtype, const float *rstd, int32_t T, int32_t D, void *dx, void *dw, void *workspace,
+                     size_t workspace_bytes, void *stream);
+size_t mi_rms_norm_grad_workspace(int32_t T, int32_t D);
+
+/*
+ * A router's logits [T, E] (bf16 or f32, row stride in elements) to the experts of each token: E <= 1024, 1 <= k <= 32,
+ * k <= E / n_group * topk_group, T <= 2^22.
+ *   s = sigmoid(l) (MI_GATE_SIGMOID) or softmax(l) over the row (MI_GATE_SOFTMAX)
+ *   c = s + bias (bias f32 [E] or NULL); an expert whose logit is -inf is out of service: c = -inf
+ *   n_group > 1 (a power of two, up to 32, that divides E): of the groups of E / n_group consecutive experts the topk_group
+ *     best stay, by the sum of their group_top (1 or 2) largest c; the others' experts are out
+ *   idx = the k largest c, equal ones by the lower id, w = s[idx], with norm_topk divided by (their sum + 1e-20), * scaling
+ * A slot that no expert is left for gets id -1 and weight 0.  Choices are compared in 64 bits, those within 2^-42 of each
+ * other's size as equal; without a bias experts of kept groups are ordered by their logits.  A choice that is no number
+ * counts as the largest.
+ *
+ * mi_moe_gate_grad: dlogits [T, E] (dtype, contiguous) of dw [T, k], for the idx that mi_moe_gate wrote.
+ */
+#define MI_GATE_SIGMOID 0
+#define MI_GATE_SOFTMAX 1
+int mi_moe_gate(const void *logits, int32_t dtype, int64_t stride, const float *bias, int32_t T, int32_t E, int32_t k,
+                int32_t scores, int32_t n_group, int32_t topk_group, int32_t group_top, int32_t norm_topk, float scaling,
+                int32_t *idx, float *w, void *stream);
+int mi_moe_gate_grad(const void *logits, int32_t dtype, int64_t stride, const int32_t *idx, const float *dw, int32_t T,
+                     int32_t E, int32_t k, int32_t scores, int32_t norm_topk, float scaling, void *dlogits, void *stream);
 
 /*
  * Launch-plan overrides, for tests and measurement runs only (no counterpart in the reference).  The library reads

@@ -26,6 +26,8 @@ I8_CTR_BYTES = 2 * 1024 * 128   # counters at the start of every int8 / bf16 str
 MI_W_BF16 = 3                # mi_mlp_many: bf16 weights
 MI_I8_COL_AFTER = 2          # s [n_out] applied after the dot (the int8 lm_head)
 MI_I8_TILED = 0x100          # OR'ed into scale_axis: qT in the tiled layout of mi_int8_tile
+MI_GATE_SIGMOID = 0          # mi_moe_gate's scores
+MI_GATE_SOFTMAX = 1
 MI_COMBINE_MATMUL = 0
 MI_COMBINE_GATHER = 1
 MI_COMBINE_SWEEP = 2         # the dense sweep's rounding points (sweep_mode="dense")
@@ -51,7 +53,8 @@ EXPORTS = ("mi_matvec", "mi_matvec_workspace", "mi_moe_decode", "mi_moe_decode_f
            "mi_bf16_mlp", "mi_mlp_many", "mi_mlp_many_workspace", "mi_bf16_mlp_workspace", "mi_tuning_set", "mi_tuning_reset",
            "mi_fp8_quantize", "mi_fp8_project", "mi_fp8_project_workspace", "mi_fp8_mlp", "mi_fp8_mlp_workspace",
            "mi_fp8_grouped", "mi_fp8_grouped_workspace", "mi_fp8_moe", "mi_fp8_moe_workspace", "mi_moe_dispatch",
-           "mi_moe_combine", "mi_moe_combine_grad", "mi_strerror", "mi_version")
+           "mi_moe_combine", "mi_moe_combine_grad", "mi_rms_norm", "mi_rms_norm_grad", "mi_rms_norm_grad_workspace",
+           "mi_moe_gate", "mi_moe_gate_grad", "mi_strerror", "mi_version")
 
 
 class MiTable(ctypes.Structure):
@@ -83,7 +86,7 @@ def lib():
                            "(or __graft_entry__.build()) first")
     L = ctypes.CDLL(LIB_PATH)
     P, I, Z, F = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t, ctypes.c_float
-    T = ctypes.POINTER(MiTable)
+    L64, T = ctypes.c_int64, ctypes.POINTER(MiTable)
     sig = {
         "mi_matvec": (I, [T, P, I, P, I, I, P, P, Z, P]),
         "mi_matvec_workspace": (Z, [T, I]),
@@ -128,6 +131,11 @@ def lib():
         "mi_moe_dispatch": (I, [P, I, I, I, I, P, P, I, P, P]),
         "mi_moe_combine": (I, [P, I, I, I, I, P, P, I, P, P]),
         "mi_moe_combine_grad": (I, [P, P, I, I, I, I, P, P, P, I, P, P, P]),
+        "mi_rms_norm": (I, [P, I, L64, P, L64, P, I, I, I, ctypes.c_double, P, P, P, P, P, P]),
+        "mi_rms_norm_grad": (I, [P, P, I, L64, P, P, I, P, I, I, P, P, P, Z, P]),
+        "mi_rms_norm_grad_workspace": (Z, [I, I]),
+        "mi_moe_gate": (I, [P, I, L64, P, I, I, I, I, I, I, I, I, F, P, P, P]),
+        "mi_moe_gate_grad": (I, [P, I, L64, P, P, I, I, I, I, I, F, P, P]),
         "mi_tuning_set": (I, [ctypes.c_char_p, I]),
         "mi_tuning_reset": (None, []),
         "mi_strerror": (ctypes.c_char_p, [I]),

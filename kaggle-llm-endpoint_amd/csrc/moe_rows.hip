@@ -6,43 +6,11 @@
 //   combine_grad    dy[row_slot[t, j]] = w[t, j] dout[t], 0 on all others;    dw[t, j] = <dout[t], y[row_slot[t, j]]>
 // No atomics: every output element has one writer and a fixed order of summation.  Rows and tokens outside the
 // buffers count as none.
-#include "common.h"
+#include "rows8.h"
 
 namespace mi {
 
 constexpr int kMoeRowsMax = 1 << 22;
-
-// Eight consecutive elements of a row.
-template <int XD>
-struct Row8 {
-    float v[8];
-    __device__ __forceinline__ void load(const void *p, size_t at) {
-        if constexpr (XD == MI_X_BF16) {
-            const uint4 u = *(const uint4 *)((const uint16_t *)p + at);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[2 * j] = __uint_as_float(w[j] << 16);
-                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-            }
-        } else {
-            const float4 a = *(const float4 *)((const float *)p + at), b = *(const float4 *)((const float *)p + at + 4);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        }
-    }
-    __device__ __forceinline__ void store(void *p, size_t at) const {
-        if constexpr (XD == MI_X_BF16) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16_rne(v[2 * j]) | (f32_to_bf16_rne(v[2 * j + 1]) << 16);
-            *(uint4 *)((uint16_t *)p + at) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-            *(float4 *)((float *)p + at) = make_float4(v[0], v[1], v[2], v[3]);
-            *(float4 *)((float *)p + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        }
-    }
-};
 
 constexpr int kPadRows = 16;                     // rows that one of the padding workgroups looks at: 16 lanes each
 

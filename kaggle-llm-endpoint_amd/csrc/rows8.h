@@ -1,0 +1,38 @@
+// Eight consecutive elements of a row of bf16 or f32 values, as f32: one 16-byte access (two for f32).
+#pragma once
+#include "common.h"
+
+namespace mi {
+
+template <int XD>
+struct Row8 {
+    float v[8];
+    __device__ __forceinline__ void load(const void *p, size_t at) {
+        if constexpr (XD == MI_X_BF16) {
+            const uint4 u = *(const uint4 *)((const uint16_t *)p + at);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[2 * j] = __uint_as_float(w[j] << 16);
+                v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            }
+        } else {
+            const float4 a = *(const float4 *)((const float *)p + at), b = *(const float4 *)((const float *)p + at + 4);
+            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+            v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        }
+    }
+    __device__ __forceinline__ void store(void *p, size_t at) const {
+        if constexpr (XD == MI_X_BF16) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16_rne(v[2 * j]) | (f32_to_bf16_rne(v[2 * j + 1]) << 16);
+            *(uint4 *)((uint16_t *)p + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            *(float4 *)((float *)p + at) = make_float4(v[0], v[1], v[2], v[3]);
+            *(float4 *)((float *)p + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    }
+};
+
+}  // namespace mi
