@@ -12,6 +12,7 @@ from .resident import (Bf16Leaf, ExpertTable, ResidentFetch, bf16_leaf, bf16_mlp
                        random_iq3s_table, random_iq4xs_table, random_kq_table, route, to_device_planes, tuning)
 from .fp8 import Fp8Leaf, fp8_grouped, fp8_leaf, fp8_mlp, fp8_moe, fp8_project, fp8_quantize  # noqa: F401
 from .gating import moe_gate  # noqa: F401
+from .linear import bf16_linear  # noqa: F401
 from .norms import fp8_rms_norm, rms_norm  # noqa: F401
 from .sorted_rows import moe_combine, moe_dispatch  # noqa: F401
 
@@ -23,4 +24,4 @@ __all__ = ["Bf16Leaf", "ExpertTable", "ResidentFetch", "bf16_leaf", "bf16_mlp", 
            "moe_prefill", "moe_route", "pack_planes_device", "prefill_workspace_bytes", "ragged_plan", "route", "gguf", "random_cb3_table", "random_iq2s_table", "random_iq3s_table",
            "random_iq4xs_table", "random_kq_table", "to_device_planes", "tuning", "formats",
            "Fp8Leaf", "fp8_leaf", "fp8_quantize", "fp8_project", "fp8_mlp", "fp8_grouped", "fp8_moe", "moe_dispatch",
-           "moe_combine", "moe_gate", "rms_norm", "fp8_rms_norm"]
+           "moe_combine", "moe_gate", "rms_norm", "fp8_rms_norm", "bf16_linear"]

@@ -28,6 +28,11 @@ MI_I8_COL_AFTER = 2          # s [n_out] applied after the dot (the int8 lm_head
 MI_I8_TILED = 0x100          # OR'ed into scale_axis: qT in the tiled layout of mi_int8_tile
 MI_GATE_SIGMOID = 0          # mi_moe_gate's scores
 MI_GATE_SOFTMAX = 1
+MI_ACT_NONE = 0              # mi_bf16_linear's activations
+MI_ACT_SILU = 1
+MI_ACT_GELU = 2
+MI_ACT_GELU_TANH = 3
+MI_ACT_RELU = 4
 MI_COMBINE_MATMUL = 0
 MI_COMBINE_GATHER = 1
 MI_COMBINE_SWEEP = 2         # the dense sweep's rounding points (sweep_mode="dense")
@@ -54,7 +59,8 @@ EXPORTS = ("mi_matvec", "mi_matvec_workspace", "mi_moe_decode", "mi_moe_decode_f
            "mi_fp8_quantize", "mi_fp8_project", "mi_fp8_project_workspace", "mi_fp8_mlp", "mi_fp8_mlp_workspace",
            "mi_fp8_grouped", "mi_fp8_grouped_workspace", "mi_fp8_moe", "mi_fp8_moe_workspace", "mi_moe_dispatch",
            "mi_moe_combine", "mi_moe_combine_grad", "mi_rms_norm", "mi_rms_norm_grad", "mi_rms_norm_grad_workspace",
-           "mi_moe_gate", "mi_moe_gate_grad", "mi_strerror", "mi_version")
+           "mi_moe_gate", "mi_moe_gate_grad", "mi_bf16_linear", "mi_bf16_linear_workspace", "mi_bf16_linear_grad",
+           "mi_bf16_linear_grad_workspace", "mi_strerror", "mi_version")
 
 
 class MiTable(ctypes.Structure):
@@ -136,6 +142,10 @@ def lib():
         "mi_rms_norm_grad_workspace": (Z, [I, I]),
         "mi_moe_gate": (I, [P, I, L64, P, I, I, I, I, I, I, I, I, F, P, P, P]),
         "mi_moe_gate_grad": (I, [P, I, L64, P, P, I, I, I, I, I, F, P, P]),
+        "mi_bf16_linear": (I, [P, L64, I, P, I, I, P, I, P, I, P, P, P, Z, P]),
+        "mi_bf16_linear_workspace": (Z, [I, I, I]),
+        "mi_bf16_linear_grad": (I, [P, I, P, I, P, L64, I, P, I, I, P, P, P, P, Z, P]),
+        "mi_bf16_linear_grad_workspace": (Z, [I, I, I]),
         "mi_tuning_set": (I, [ctypes.c_char_p, I]),
         "mi_tuning_reset": (None, []),
         "mi_strerror": (ctypes.c_char_p, [I]),

@@ -37,7 +37,8 @@ UNITS = [("moe_decode.hip", [], "moe_decode"), ("int8_project.hip", [], "int8_pr
          ("pack.hip", [], "pack"), ("tuning.hip", [], "tuning"),
          # matrix results straight into vector registers, where they are scaled, instead of by way of accumulation ones
          ("fp8.hip", ["-mllvm", "-amdgpu-mfma-vgpr-form=1"], "fp8"),
-         ("moe_rows.hip", [], "moe_rows"), ("norm.hip", [], "norm"), ("gate.hip", [], "gate")]
+         ("moe_rows.hip", [], "moe_rows"), ("norm.hip", [], "norm"), ("gate.hip", [], "gate"),
+         ("linear.hip", [], "linear")]
 UNITS += [("k_grouped.hip", ["-DMI_KMODE=%d" % m, "-DMI_KQT=%d" % q], "k_grouped_%d_%d" % (m, q))
           for m in (0, 1, 2) for q in (1, 2, 3, 4, 5, 6)]
 UNITS += [("k_fused.hip", [], "k_fused")]

@@ -1,0 +1,270 @@
+// Products over bf16 weights with bias, activation and residual, for any number of rows, and their gradients
+// (linear_gemm.h), behind the C ABI.
+#include <algorithm>
+
+#include "linear_gemm.h"
+#include "rows8.h"
+#include "tuning.h"
+
+namespace mi {
+
+// The split sums of a product, added in split order, then its epilogue: four outputs a thread.
+__global__ void __launch_bounds__(256) lin_reduce_kernel(LinGemm p) {
+    const int quads = (p.R + 3) / 4;
+    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= (long long)p.rows * quads) return;
+    const int row = (int)(at / quads), o = 4 * (int)(at - (long long)row * quads);
+    const size_t n = (size_t)p.rows * p.R;
+    const float *f = p.part + (size_t)row * p.R + o;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.S; ++s, f += n) {
+        if ((p.R & 3) == 0) {
+            v += *(const f32x4 *)f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (o + j < p.R) v[j] += f[j];
+        }
+    }
+    lin_out(p, LinQuads(p), row, o, v);
+}
+
+// dz = dy act'(z), rounded to bf16 for the products (2^-9 of each term), in rows of ldz columns whose last ones are zeros,
+// and each workgroup's sums of dz (before their rounding) over its rows, for the bias.  A workgroup takes 256 columns, 32
+// lanes of 8, and rows blockIdx.y * 8 + .., 8 at a time.
+struct LinDz {
+    const void *dy;             // [B, N]
+    int f32, act, B, N;
+    const uint16_t *z;          // [B, ldz] (act)
+    long long ldz;
+    uint16_t *dz;               // [B, ldz] or NULL
+    float *part;                // [gridDim.y, N] or NULL
+};
+__global__ void __launch_bounds__(256) lin_dz_kernel(LinDz p) {
+    __shared__ float sum[8][256];
+    const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5;
+    const int c = blockIdx.x * 256 + 8 * lane;
+    const bool whole = p.N % 8 == 0 && ((uintptr_t)p.dy & 15) == 0;
+    float acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+    if (c < p.N) {
+        for (int row = blockIdx.y * 8 + sub; row < p.B; row += gridDim.y * 8) {
+            const size_t at = (size_t)row * p.N + c;
+            Row8<MI_X_F32> g;
+            if (whole) {
+                if (p.f32) {
+                    g.load(p.dy, at);
+                } else {
+                    Row8<MI_X_BF16> b;
+                    b.load(p.dy, at);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) g.v[j] = b.v[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    g.v[j] = c + j >= p.N ? 0.0f : p.f32 ? ((const float *)p.dy)[at + j] : bf16_to_f32(((const uint16_t *)p.dy)[at + j]);
+            }
+            if (p.act) {
+                Row8<MI_X_BF16> z;
+                z.load(p.z, (size_t)row * p.ldz + c);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g.v[j] = c + j >= p.N ? 0.0f : g.v[j] * lin_act_grad(z.v[j], p.act);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] += g.v[j];
+            if (p.dz) {
+                Row8<MI_X_BF16> o;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o.v[j] = g.v[j];
+                o.store(p.dz, (size_t)row * p.ldz + c);
+            }
+        }
+    }
+    if (!p.part) return;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[sub][8 * lane + j] = acc[j];
+    __syncthreads();
+    const int o = blockIdx.x * 256 + threadIdx.x;
+    if (o >= p.N) return;
+    float v = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += sum[k][threadIdx.x];
+    p.part[(size_t)blockIdx.y * p.N + o] = v;
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+constexpr int kLinMaxCols = 1 << 16;             // n_in, n_out
+constexpr int kLinMaxRows = 1 << 20;
+constexpr int kLinCus = 256;
+constexpr int kLinStreamRows = 32;
+
+static bool lin_shape_ok(int n_in, int n_out) {
+    return n_in > 0 && n_in % 8 == 0 && n_in <= kLinMaxCols && n_out > 0 && n_out <= kLinMaxCols;
+}
+static size_t lin_up(size_t n) { return (n + 255) & ~(size_t)255; }
+static bool lin_aligned(const void *a, int n) { return ((uintptr_t)a & (n - 1)) == 0; }
+static int lin_ok() { return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH; }
+
+template <int TW, int TT, int WM, int WN, int NST>
+static int lin_launch_tile(LinGemm p, bool slow_a, bool slow_b, hipStream_t st) {
+    p.nw = (p.R + TW - 1) / TW;
+    p.nb = (p.rows + TT - 1) / TT;
+    const long long total = (long long)p.nw * p.nb * p.S, grid = (total + 7) / 8 * 8;
+    if (grid >= (1ll << 31) / (64 * WM * WN)) return MI_ERR_TOKENS;
+    auto kern = slow_b ? lin_gemm_kernel<TW, TT, WM, WN, NST, true, true>
+              : slow_a ? lin_gemm_kernel<TW, TT, WM, WN, NST, true, false> : lin_gemm_kernel<TW, TT, WM, WN, NST, false, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, p);
+    return lin_ok();
+}
+
+struct LinPlan {
+    int tw, tt, S;
+};
+constexpr int kLinMaxSplits = 8;
+constexpr size_t kLinSplitTiles = 512;           // tiles of 128 x 128 of all splits together, at most
+
+// Floats of split sums of a product of R outputs and any number of rows.
+static size_t lin_split_floats(int R) {
+    const size_t n = (size_t)(R + 127) / 128;
+    return std::max<size_t>(kLinSplitTiles / n, 1) * 128 * R;
+}
+
+static LinPlan lin_plan(int rows, int R, int K) {
+    LinPlan best{128, 128, 1};
+    const int steps = (K + kLinCols - 1) / kLinCols;
+    const long long big = (long long)((R + 255) / 256) * ((rows + 255) / 256);
+    if (big >= kLinCus / 2) best = {256, 256, 1};
+    const long long tiles = (long long)((R + 127) / 128) * ((rows + 127) / 128);
+    if (best.tw == 128)
+        while (best.S < kLinMaxSplits && tiles * best.S * 2 <= 2 * kLinCus && steps / (2 * best.S) >= 4 &&
+               (size_t)best.S * 2 * rows * R <= lin_split_floats(R))
+            best.S *= 2;
+    const int tw = tuning(kTuneLinTw, 0), tt = tuning(kTuneLinTt, 0), S = tuning(kTuneLinS, 0);
+    if (tw) best.tw = tw;
+    if (tt) best.tt = tt;
+    if (S && S <= steps && (S == 1 || (size_t)S * rows * R <= lin_split_floats(R))) best.S = S;
+    return best;
+}
+
+static int lin_launch(LinGemm p, bool slow_a, bool slow_b, float *part, hipStream_t st) {
+    const LinPlan pl = lin_plan(p.rows, p.R, p.K);
+    p.S = pl.S;
+    p.part = part;
+    int rc;
+    if (pl.tw == 256 && pl.tt == 256) rc = lin_launch_tile<256, 256, 2, 4, 2>(p, slow_a, slow_b, st);
+    else rc = lin_launch_tile<128, 128, 2, 2, 2>(p, slow_a, slow_b, st);
+    if (rc != MI_OK || p.S == 1) return rc;
+    const long long n = (long long)p.rows * ((p.R + 3) / 4);
+    hipLaunchKernelGGL(lin_reduce_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p);
+    return lin_ok();
+}
+
+template <int NT>
+static int lin_launch_stream(const LinGemm &p, hipStream_t st) {
+    hipLaunchKernelGGL((lin_stream_kernel<NT, 1, 4, 4>), dim3((p.R + 15) / 16), dim3(256), 0, st, p);
+    return lin_ok();
+}
+
+static int lin_check(int B, int n_in, int n_out, int64_t x_stride, int act) {
+    if (B <= 0 || B > kLinMaxRows) return MI_ERR_TOKENS;
+    if (!lin_shape_ok(n_in, n_out)) return MI_ERR_SHAPE;
+    if (x_stride < n_in || x_stride % 8 || x_stride > (1 << 20)) return MI_ERR_ARG;
+    return act >= MI_ACT_NONE && act <= MI_ACT_RELU ? MI_OK : MI_ERR_ARG;
+}
+
+static long long lin_pad(int n) { return (n + 7) & ~7; }
+// Workgroups along the rows of lin_dz_kernel.
+static int lin_dz_wgs(int B) { return std::min((B + 7) / 8, 64); }
+
+}  // namespace mi
+
+using namespace mi;
+
+extern "C" size_t mi_bf16_linear_workspace(int32_t B, int32_t n_in, int32_t n_out) {
+    if (lin_check(B, n_in, n_out, n_in, 0) != MI_OK || B <= kLinStreamRows) return 0;
+    return lin_up(lin_split_floats(n_out) * sizeof(float));
+}
+
+extern "C" int mi_bf16_linear(const uint16_t *x, int64_t x_stride, int32_t B, const uint16_t *wT, int32_t n_in, int32_t n_out,
+                              const uint16_t *bias, int32_t act, const void *residual, int32_t y_dtype, void *y, uint16_t *z,
+                              void *workspace, size_t workspace_bytes, void *stream) {
+    if (!x || !wT || !y) return MI_ERR_NULL;
+    const int rc = lin_check(B, n_in, n_out, x_stride, act);
+    if (rc != MI_OK) return rc;
+    if (y_dtype != MI_X_BF16 && y_dtype != MI_X_F32) return MI_ERR_ARG;
+    const int el = y_dtype == MI_X_F32 ? 4 : 2;
+    if (!lin_aligned(x, 16) || !lin_aligned(wT, 16) || !lin_aligned(bias, 2) || !lin_aligned(residual, el) ||
+        !lin_aligned(y, el) || !lin_aligned(z, 16) || !lin_aligned(workspace, 16))
+        return MI_ERR_ARG;
+    const size_t need = mi_bf16_linear_workspace(B, n_in, n_out);
+    if (need && (!workspace || workspace_bytes < need)) return MI_ERR_WORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    LinGemm p = {};
+    p.a = wT, p.lda = n_in;
+    p.b = x, p.ldb = x_stride;
+    p.R = n_out, p.rows = B, p.K = p.Ks = n_in;
+    p.bias = bias, p.act = act, p.res = residual;
+    p.f32 = y_dtype == MI_X_F32;
+    p.y = y, p.z = z, p.ldz = lin_pad(n_out);
+    if (B <= 16) return lin_launch_stream<1>(p, st);
+    if (B <= kLinStreamRows) return lin_launch_stream<2>(p, st);
+    return lin_launch(p, false, false, (float *)workspace, st);
+}
+
+extern "C" size_t mi_bf16_linear_grad_workspace(int32_t B, int32_t n_in, int32_t n_out) {
+    if (lin_check(B, n_in, n_out, n_in, 0) != MI_OK) return 0;
+    return lin_up((size_t)B * lin_pad(n_out) * 2) + lin_up((size_t)lin_dz_wgs(B) * n_out * sizeof(float)) +
+           lin_up(lin_split_floats(n_in) * sizeof(float));
+}
+
+extern "C" int mi_bf16_linear_grad(const void *dy, int32_t dy_dtype, const uint16_t *z, int32_t act, const uint16_t *x,
+                                   int64_t x_stride, int32_t B, const uint16_t *wT, int32_t n_in, int32_t n_out, uint16_t *dx,
+                                   uint16_t *dw, uint16_t *dbias, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!dy || (act && !z) || (dx && !wT) || (dw && !x) || (!dx && !dw && !dbias)) return MI_ERR_NULL;
+    int rc = lin_check(B, n_in, n_out, dw ? x_stride : n_in, act);
+    if (rc != MI_OK) return rc;
+    if (dy_dtype != MI_X_BF16 && dy_dtype != MI_X_F32) return MI_ERR_ARG;
+    if (!lin_aligned(dy, dy_dtype == MI_X_F32 ? 4 : 2) || !lin_aligned(z, 16) || !lin_aligned(x, 16) || !lin_aligned(wT, 16) ||
+        !lin_aligned(dx, 2) || !lin_aligned(dw, 2) || !lin_aligned(dbias, 2) || !lin_aligned(workspace, 16))
+        return MI_ERR_ARG;
+    if (!workspace || workspace_bytes < mi_bf16_linear_grad_workspace(B, n_in, n_out)) return MI_ERR_WORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    char *ws = (char *)workspace;
+    uint16_t *dz = (uint16_t *)ws;
+    ws += lin_up((size_t)B * lin_pad(n_out) * 2);
+    float *sums = (float *)ws;
+    ws += lin_up((size_t)lin_dz_wgs(B) * n_out * sizeof(float));
+    float *part = (float *)ws;
+    // dy itself where it is dz already, in rows that the products can load
+    const bool as_is = act == MI_ACT_NONE && dy_dtype == MI_X_BF16 && n_out % 8 == 0 && lin_aligned(dy, 16);
+    if (!as_is || dbias) {
+        const LinDz d = {dy, dy_dtype == MI_X_F32, act, B, n_out, z, lin_pad(n_out), as_is || !(dx || dw) ? nullptr : dz,
+                         dbias ? sums : nullptr};
+        const int n = lin_dz_wgs(B);
+        hipLaunchKernelGGL(lin_dz_kernel, dim3((n_out + 255) / 256, n), dim3(256), 0, st, d);
+        if ((rc = lin_ok()) != MI_OK) return rc;
+        if (dbias) {
+            hipLaunchKernelGGL(column_sums_kernel, dim3((n_out + 31) / 32), dim3(256), 0, st, sums, n, n_out, 0, (void *)dbias);
+            if ((rc = lin_ok()) != MI_OK) return rc;
+        }
+    }
+    LinGemm p = {};
+    p.b = as_is ? (const uint16_t *)dy : dz;
+    p.ldb = lin_pad(n_out);
+    p.R = n_in;
+    if (dx) {                                    // dx[t, k] = sum_n dz[t, n] w[n, k]
+        p.a = wT, p.lda = n_in;
+        p.rows = B, p.K = (int)lin_pad(n_out), p.Ks = n_out;
+        p.y = dx;
+        if ((rc = lin_launch(p, true, false, part, st)) != MI_OK) return rc;
+    }
+    if (dw) {                                    // dw[n, k] = sum_t dz[t, n] x[t, k]
+        p.a = x, p.lda = x_stride;
+        p.rows = n_out, p.K = p.Ks = B;
+        p.y = dw;
+        if ((rc = lin_launch(p, true, true, part, st)) != MI_OK) return rc;
+    }
+    return MI_OK;
+}

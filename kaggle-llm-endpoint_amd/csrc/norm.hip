@@ -224,24 +224,6 @@ __global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) rms_norm_grad_kerne
     }
 }
 
-// dw: the workgroups' sums added in order within 8 pieces, then the pieces; 32 columns a workgroup.
-__global__ void __launch_bounds__(256) rms_norm_dw_kernel(const float *__restrict__ part, int n, int D, int w_f32, void *dw) {
-    __shared__ float sum[8][32];
-    const int lane = threadIdx.x & 31, piece = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    float a = 0.0f;
-    if (c < D)
-        for (int k = piece; k < n; k += 8) a += part[(size_t)k * D + c];
-    sum[piece][lane] = a;
-    __syncthreads();
-    if (piece || c >= D) return;
-#pragma unroll
-    for (int k = 1; k < 8; ++k) a += sum[k][lane];
-    if (w_f32)
-        ((float *)dw)[c] = a;
-    else
-        ((uint16_t *)dw)[c] = (uint16_t)f32_to_bf16_rne(a);
-}
-
 // ------------------------------------------------------------------------------------------------ host side
 // f(lanes, values / 8) of the least number of values that holds a row.
 template <class F>
@@ -319,6 +301,6 @@ extern "C" int mi_rms_norm_grad(const void *dy, const void *s, int32_t dtype, in
         return hipGetLastError() == hipSuccess ? (int)MI_OK : (int)MI_ERR_LAUNCH;
     });
     if (launched != MI_OK || !dw) return launched;
-    hipLaunchKernelGGL(rms_norm_dw_kernel, dim3((D + 31) / 32), dim3(256), 0, st, part, n, D, (int)(w_dtype == MI_X_F32), dw);
+    hipLaunchKernelGGL(column_sums_kernel, dim3((D + 31) / 32), dim3(256), 0, st, part, n, D, (int)(w_dtype == MI_X_F32), dw);
     return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH;
 }

@@ -1,4 +1,4 @@
-// Eight consecutive elements of a row of bf16 or f32 values, as f32: one 16-byte access (two for f32).
+// Rows of bf16 or f32 values: eight consecutive elements as f32, one 16-byte access (two for f32), and sums of columns.
 #pragma once
 #include "common.h"
 
@@ -34,5 +34,23 @@ struct Row8 {
         }
     }
 };
+
+// Sums over the n rows of part [n, D]: in order within 8 pieces, then the pieces; 32 columns a workgroup.
+static __global__ void __launch_bounds__(256) column_sums_kernel(const float *__restrict__ part, int n, int D, int f32, void *out) {
+    __shared__ float sum[8][32];
+    const int lane = threadIdx.x & 31, piece = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    float a = 0.0f;
+    if (c < D)
+        for (int k = piece; k < n; k += 8) a += part[(size_t)k * D + c];
+    sum[piece][lane] = a;
+    __syncthreads();
+    if (piece || c >= D) return;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) a += sum[k][lane];
+    if (f32)
+        ((float *)out)[c] = a;
+    else
+        ((uint16_t *)out)[c] = (uint16_t)f32_to_bf16_rne(a);
+}
 
 }  // namespace mi
