@@ -550,10 +550,10 @@ int mi_moe_gate_grad(const void *logits, int32_t dtype, int64_t stride, const in
  *   z = x W + bias in f32 (bf16 products, exact; f32 sums), y = act(z) + residual, rounded once to y_dtype
  * x bf16 [B, n_in], row stride x_stride elements (a multiple of 8, up to 2^20); wT bf16 [n_out, n_in] (the reference's leaf
  * transposed once, as for mi_bf16_project); bias bf16 [n_out] or NULL; residual [B, n_out] of y_dtype (MI_X_BF16 or
- * MI_X_F32) or NULL; act MI_ACT_*: silu z sigmoid(z), gelu z Phi(z), its tanh form, relu.  z (may be NULL): bf16(z) in rows
+ * MI_X_F32) or NULL; act MI_ACT_*: silu z sigmoid(z), gelu z Phi(z), its tanh form, relu.  z (may be NULL): z in f32, rows
  * of n_out rounded up to 8 columns, for the gradient.  1 <= B <= 2^20, n_in % 8 == 0, n_in and n_out <= 2^16.  x, wT, z and
- * the workspace 16-byte aligned.  Workspace: mi_bf16_linear_workspace bytes, no initialisation; its size serves every B.
- * Up to 32 rows need none (the size is 0, as for a shape that the call refuses).
+ * the workspace 16-byte aligned.  Workspace: mi_bf16_linear_workspace bytes, no initialisation; its size serves every smaller B.
+ * Calls of few rows that stream the weights need none (the size is 0, as for a shape that the call refuses).
  *
  * mi_bf16_linear_grad: dz = dy act'(z) from the z that was kept (NULL without an activation), rounded to bf16 for
  *   dx = dz W^T [B, n_in], dw = dz^T x [n_out, n_in] (bf16, contiguous), and summed unrounded for dbias [n_out] (bf16)
@@ -566,10 +566,10 @@ int mi_moe_gate_grad(const void *logits, int32_t dtype, int64_t stride, const in
 #define MI_ACT_GELU_TANH 3
 #define MI_ACT_RELU      4
 int mi_bf16_linear(const uint16_t *x, int64_t x_stride, int32_t B, const uint16_t *wT, int32_t n_in, int32_t n_out,
-                   const uint16_t *bias, int32_t act, const void *residual, int32_t y_dtype, void *y, uint16_t *z,
+                   const uint16_t *bias, int32_t act, const void *residual, int32_t y_dtype, void *y, float *z,
                    void *workspace, size_t workspace_bytes, void *stream);
 size_t mi_bf16_linear_workspace(int32_t B, int32_t n_in, int32_t n_out);
-int mi_bf16_linear_grad(const void *dy, int32_t dy_dtype, const uint16_t *z, int32_t act, const uint16_t *x,
+int mi_bf16_linear_grad(const void *dy, int32_t dy_dtype, const float *z, int32_t act, const uint16_t *x,
                         int64_t x_stride, int32_t B, const uint16_t *wT, int32_t n_in, int32_t n_out, uint16_t *dx,
                         uint16_t *dw, uint16_t *dbias, void *workspace, size_t workspace_bytes, void *stream);
 size_t mi_bf16_linear_grad_workspace(int32_t B, int32_t n_in, int32_t n_out);
@@ -583,7 +583,7 @@ size_t mi_bf16_linear_grad_workspace(int32_t B, int32_t n_in, int32_t n_out);
  * one-launch decode's poll limit (SPIN_LIMIT), the int8 split plan (I8S, I8_WAVES, I8_FUSE) and the many-token MLP's
  * splits and token tile (DG_S1, DG_S2, DG_NT), the prefill's wide blocks (PF_WIDE), the dense fp8 product's tile and
  * splits (F8_TW, F8_TT, F8_S) and the fp8 routed layer's streaming limit and rows per block (F8_STREAM, F8_TM), the tile and splits of the bf16 product with an
- * epilogue (LIN_TW, LIN_TT, LIN_S).
+ * epilogue and its streaming limit (LIN_TW, LIN_TT, LIN_S, LIN_STREAM).
  * Overrides change launch shapes and summation orders, never the result beyond f32 rounding (of the fp8 MLP and routed
  * layer: beyond what that moves of h when it is rounded to e4m3, and F8_TM or F8_TT above 128 takes gate and up from f32
  * sums to the fp8 instruction's); workspace sizes follow them, so set them before sizing a workspace.  Not synchronised with calls running on other host threads.

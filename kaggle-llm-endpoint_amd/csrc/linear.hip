@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(256) lin_reduce_kernel(LinGemm p) {
                 if (o + j < p.R) v[j] += f[j];
         }
     }
-    lin_out(p, LinQuads(p), row, o, v);
+    lin_out(p, row, o, v);
 }
 
 // dz = dy act'(z), rounded to bf16 for the products (2^-9 of each term), in rows of ldz columns whose last ones are zeros,
@@ -35,7 +35,7 @@ __global__ void __launch_bounds__(256) lin_reduce_kernel(LinGemm p) {
 struct LinDz {
     const void *dy;             // [B, N]
     int f32, act, B, N;
-    const uint16_t *z;          // [B, ldz] (act)
+    const float *z;             // [B, ldz] (act)
     long long ldz;
     uint16_t *dz;               // [B, ldz] or NULL
     float *part;                // [gridDim.y, N] or NULL
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) lin_dz_kernel(LinDz p) {
                     g.v[j] = c + j >= p.N ? 0.0f : p.f32 ? ((const float *)p.dy)[at + j] : bf16_to_f32(((const uint16_t *)p.dy)[at + j]);
             }
             if (p.act) {
-                Row8<MI_X_BF16> z;
+                Row8<MI_X_F32> z;
                 z.load(p.z, (size_t)row * p.ldz + c);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) g.v[j] = c + j >= p.N ? 0.0f : g.v[j] * lin_act_grad(z.v[j], p.act);
@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(256) lin_dz_kernel(LinDz p) {
 constexpr int kLinMaxCols = 1 << 16;             // n_in, n_out
 constexpr int kLinMaxRows = 1 << 20;
 constexpr int kLinCus = 256;
-constexpr int kLinStreamRows = 32;
+constexpr int kLinStreamRows = 16;              // rows of one matrix instruction
+constexpr long long kLinStreamWeights = 1 << 24;
 
 static bool lin_shape_ok(int n_in, int n_out) {
     return n_in > 0 && n_in % 8 == 0 && n_in <= kLinMaxCols && n_out > 0 && n_out <= kLinMaxCols;
@@ -107,14 +108,18 @@ static size_t lin_up(size_t n) { return (n + 255) & ~(size_t)255; }
 static bool lin_aligned(const void *a, int n) { return ((uintptr_t)a & (n - 1)) == 0; }
 static int lin_ok() { return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH; }
 
-template <int TW, int TT, int WM, int WN, int NST>
+// FAST: for a product of two fast operands only.
+template <int TW, int TT, int WM, int WN, int NST, bool FAST = false>
 static int lin_launch_tile(LinGemm p, bool slow_a, bool slow_b, hipStream_t st) {
     p.nw = (p.R + TW - 1) / TW;
     p.nb = (p.rows + TT - 1) / TT;
     const long long total = (long long)p.nw * p.nb * p.S, grid = (total + 7) / 8 * 8;
     if (grid >= (1ll << 31) / (64 * WM * WN)) return MI_ERR_TOKENS;
-    auto kern = slow_b ? lin_gemm_kernel<TW, TT, WM, WN, NST, true, true>
-              : slow_a ? lin_gemm_kernel<TW, TT, WM, WN, NST, true, false> : lin_gemm_kernel<TW, TT, WM, WN, NST, false, false>;
+    auto kern = lin_gemm_kernel<TW, TT, WM, WN, NST, false, false>;
+    if constexpr (!FAST) {
+        if (slow_b) kern = lin_gemm_kernel<TW, TT, WM, WN, NST, true, true>;
+        else if (slow_a) kern = lin_gemm_kernel<TW, TT, WM, WN, NST, true, false>;
+    }
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, p);
     return lin_ok();
 }
@@ -123,7 +128,7 @@ struct LinPlan {
     int tw, tt, S;
 };
 constexpr int kLinMaxSplits = 8;
-constexpr size_t kLinSplitTiles = 512;           // tiles of 128 x 128 of all splits together, at most
+constexpr size_t kLinSplitTiles = 512;           // 128 x 128 pieces of all splits' sums together, at most
 
 // Floats of split sums of a product of R outputs and any number of rows.
 static size_t lin_split_floats(int R) {
@@ -131,40 +136,62 @@ static size_t lin_split_floats(int R) {
     return std::max<size_t>(kLinSplitTiles / n, 1) * 128 * R;
 }
 
-static LinPlan lin_plan(int rows, int R, int K) {
-    LinPlan best{128, 128, 1};
+// The tile and the splits of the contraction: the pair of least estimated time.  A stage of 64 columns of a tile takes `one`
+// us in a launch of at most one workgroup per CU, `more` in each round of `slots` workgroups otherwise, its start and epilogue
+// as much as `ends` stages; a split adds a launch and a pass over its sums.  The times are those of operands from memory:
+// 6144 x 6144, 37 / 48 / 128 / 256 / 517 / 2048 / 4096 rows take 18 (of 2051 outputs), 23, 29, 40, 53, 135 and 260 us with
+// the tiles that this chooses; all with 256 x 256 would take 140 to 158 up to 2048 rows and 284.
+static LinPlan lin_plan(int rows, int R, int K, bool fast) {
+    struct Tile {
+        int tw, tt, slots;
+        float one, more;
+        int ends;
+    };
+    static const Tile tiles[] = {{128, 64, 2 * kLinCus, 0.50f, 0.70f, 8}, {128, 128, kLinCus, 0.54f, 0.56f, 8},
+                                 {256, 128, kLinCus, 0.74f, 0.83f, 9}, {256, 256, kLinCus, 1.52f, 1.38f, 8},
+                                 {192, 256, kLinCus, 1.31f, 1.27f, 7}};
     const int steps = (K + kLinCols - 1) / kLinCols;
-    const long long big = (long long)((R + 255) / 256) * ((rows + 255) / 256);
-    if (big >= kLinCus / 2) best = {256, 256, 1};
-    const long long tiles = (long long)((R + 127) / 128) * ((rows + 127) / 128);
-    if (best.tw == 128)
-        while (best.S < kLinMaxSplits && tiles * best.S * 2 <= 2 * kLinCus && steps / (2 * best.S) >= 4 &&
-               (size_t)best.S * 2 * rows * R <= lin_split_floats(R))
-            best.S *= 2;
-    const int tw = tuning(kTuneLinTw, 0), tt = tuning(kTuneLinTt, 0), S = tuning(kTuneLinS, 0);
-    if (tw) best.tw = tw;
-    if (tt) best.tt = tt;
-    if (S && S <= steps && (S == 1 || (size_t)S * rows * R <= lin_split_floats(R))) best.S = S;
+    const int tw = tuning(kTuneLinTw, 0), tt = tuning(kTuneLinTt, 0), fs = tuning(kTuneLinS, 0);
+    LinPlan best{128, 128, 1};
+    float least = 1e30f;
+    for (const Tile &c : tiles) {
+        if ((c.tw == 192 && !fast) || (tw && c.tw != tw) || (tt && c.tt != tt)) continue;
+        const long long n = (long long)((R + c.tw - 1) / c.tw) * ((rows + c.tt - 1) / c.tt);
+        for (int S = 1; S <= std::min(kLinMaxSplits, steps); ++S) {
+            if (S > 1 && (n * S > c.slots || (size_t)S * rows * R > lin_split_floats(R))) break;
+            if (fs && S != fs) continue;
+            const long long wgs = n * S;
+            const float step = wgs <= kLinCus ? c.one : (float)((wgs + c.slots - 1) / c.slots) * c.more;
+            const float us = step * ((steps + S - 1) / S + c.ends) +
+                             (S > 1 ? 3.0f + (float)((double)S * rows * R * 8 / 3.5e6) : 0.0f);
+            if (us < least) least = us, best = LinPlan{c.tw, c.tt, S};
+        }
+    }
     return best;
 }
 
 static int lin_launch(LinGemm p, bool slow_a, bool slow_b, float *part, hipStream_t st) {
-    const LinPlan pl = lin_plan(p.rows, p.R, p.K);
+    const LinPlan pl = lin_plan(p.rows, p.R, p.K, !slow_a && !slow_b);
     p.S = pl.S;
     p.part = part;
     int rc;
-    if (pl.tw == 256 && pl.tt == 256) rc = lin_launch_tile<256, 256, 2, 4, 2>(p, slow_a, slow_b, st);
-    else rc = lin_launch_tile<128, 128, 2, 2, 2>(p, slow_a, slow_b, st);
+    if (pl.tw == 192) rc = lin_launch_tile<192, 256, 2, 4, 2, true>(p, slow_a, slow_b, st);
+    else if (pl.tt == 256) rc = lin_launch_tile<256, 256, 2, 4, 2>(p, slow_a, slow_b, st);
+    else if (pl.tw == 256) rc = lin_launch_tile<256, 128, 4, 2, 3>(p, slow_a, slow_b, st);
+    else if (pl.tt == 128) rc = lin_launch_tile<128, 128, 2, 2, 4>(p, slow_a, slow_b, st);
+    else rc = lin_launch_tile<128, 64, 2, 2, 3>(p, slow_a, slow_b, st);
     if (rc != MI_OK || p.S == 1) return rc;
     const long long n = (long long)p.rows * ((p.R + 3) / 4);
     hipLaunchKernelGGL(lin_reduce_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p);
     return lin_ok();
 }
 
-template <int NT>
-static int lin_launch_stream(const LinGemm &p, hipStream_t st) {
-    hipLaunchKernelGGL((lin_stream_kernel<NT, 1, 4, 4>), dim3((p.R + 15) / 16), dim3(256), 0, st, p);
-    return lin_ok();
+// Whether a product of B rows streams the weights: every workgroup reads all rows again, which costs more the more they are
+// (6144 x 6144: 1 / 4 / 8 / 16 rows 18 / 20 / 22 / 27 us, tiled with 4 splits 20 to 21; 2051 outputs of 6144 columns: 16 rows
+// 14.4, tiled 19.3; 2048 x 2048: 5.3 and 8.8).
+static bool lin_streams(int B, int K, int R) {
+    return B <= tuning(kTuneLinStream, B <= 4 || (long long)K * R <= kLinStreamWeights ? kLinStreamRows : 0) &&
+           B <= kLinStreamRows;
 }
 
 static int lin_check(int B, int n_in, int n_out, int64_t x_stride, int act) {
@@ -183,12 +210,12 @@ static int lin_dz_wgs(int B) { return std::min((B + 7) / 8, 64); }
 using namespace mi;
 
 extern "C" size_t mi_bf16_linear_workspace(int32_t B, int32_t n_in, int32_t n_out) {
-    if (lin_check(B, n_in, n_out, n_in, 0) != MI_OK || B <= kLinStreamRows) return 0;
+    if (lin_check(B, n_in, n_out, n_in, 0) != MI_OK || lin_streams(B, n_in, n_out)) return 0;
     return lin_up(lin_split_floats(n_out) * sizeof(float));
 }
 
 extern "C" int mi_bf16_linear(const uint16_t *x, int64_t x_stride, int32_t B, const uint16_t *wT, int32_t n_in, int32_t n_out,
-                              const uint16_t *bias, int32_t act, const void *residual, int32_t y_dtype, void *y, uint16_t *z,
+                              const uint16_t *bias, int32_t act, const void *residual, int32_t y_dtype, void *y, float *z,
                               void *workspace, size_t workspace_bytes, void *stream) {
     if (!x || !wT || !y) return MI_ERR_NULL;
     const int rc = lin_check(B, n_in, n_out, x_stride, act);
@@ -208,8 +235,10 @@ extern "C" int mi_bf16_linear(const uint16_t *x, int64_t x_stride, int32_t B, co
     p.bias = bias, p.act = act, p.res = residual;
     p.f32 = y_dtype == MI_X_F32;
     p.y = y, p.z = z, p.ldz = lin_pad(n_out);
-    if (B <= 16) return lin_launch_stream<1>(p, st);
-    if (B <= kLinStreamRows) return lin_launch_stream<2>(p, st);
+    if (lin_streams(B, n_in, n_out)) {
+        hipLaunchKernelGGL((lin_stream_kernel<4, 4>), dim3((n_out + 15) / 16), dim3(256), 0, st, p);
+        return lin_ok();
+    }
     return lin_launch(p, false, false, (float *)workspace, st);
 }
 
@@ -219,7 +248,7 @@ extern "C" size_t mi_bf16_linear_grad_workspace(int32_t B, int32_t n_in, int32_t
            lin_up(lin_split_floats(n_in) * sizeof(float));
 }
 
-extern "C" int mi_bf16_linear_grad(const void *dy, int32_t dy_dtype, const uint16_t *z, int32_t act, const uint16_t *x,
+extern "C" int mi_bf16_linear_grad(const void *dy, int32_t dy_dtype, const float *z, int32_t act, const uint16_t *x,
                                    int64_t x_stride, int32_t B, const uint16_t *wT, int32_t n_in, int32_t n_out, uint16_t *dx,
                                    uint16_t *dw, uint16_t *dbias, void *workspace, size_t workspace_bytes, void *stream) {
     if (!dy || (act && !z) || (dx && !wT) || (dw && !x) || (!dx && !dw && !dbias)) return MI_ERR_NULL;

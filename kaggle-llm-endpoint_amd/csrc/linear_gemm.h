@@ -3,6 +3,8 @@
 // in f32, rounded once.  Forward a is the weight [n_out, n_in] and b the rows [B, n_in]; the gradients take an operand whose
 // contraction index is the slow one ([k, o] in memory) as it lies: its fragments are read from LDS transposed.
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace mi {
@@ -28,7 +30,7 @@ struct LinGemm {
     const void *res;            // [rows, R] of y's type, or NULL
     int f32;                    // y and res are f32, else bf16
     void *y;                    // [rows, R]
-    uint16_t *z;                // bf16(C + bias) [rows, ldz], ldz a multiple of 8 that holds R, or NULL
+    float *z;                   // C + bias [rows, ldz], ldz a multiple of 8 that holds R, or NULL
     long long ldz;
     // ---- tiled launches
     int nw, nb, S;              // weight tiles, token tiles, splits of K
@@ -36,129 +38,179 @@ struct LinGemm {
 };
 
 // ------------------------------------------------------------------------------------------------ activations
-__device__ __forceinline__ float lin_sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+// e^x and 1 / x by the plain instructions: 1 ulp each, besides |x| 2^-24 for the rounding of x log2(e).
+__device__ __forceinline__ float lin_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ float lin_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + lin_exp(-z)); }
 __device__ __forceinline__ float gelu_inner2(float z) {                  // 2 sqrt(2 / pi) (z + 0.044715 z^3)
     return 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
 }
-__device__ __forceinline__ float lin_act(float z, int act) {
-    switch (act) {
-        case MI_ACT_SILU: return z * lin_sigmoid(z);
-        case MI_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.7071067811865476f));
-        case MI_ACT_GELU_TANH: return z * lin_sigmoid(gelu_inner2(z));   // (1 + tanh(u)) / 2 = sigmoid(2 u)
-        case MI_ACT_RELU: return z < 0.0f ? 0.0f : z;                    // (a NaN stays)
-        default: return z;
-    }
+// The normal distribution's Phi(z), and e^(-z^2 / 2): 1 - Phi(|z|) = (a1 t + .. + a5 t^5) e^(-z^2 / 2) / 2 with
+// t = 1 / (1 + p |z| / sqrt 2), Abramowitz and Stegun 7.1.26, off by at most 7.5e-8 (a third of erff's instructions, which
+// took 17 us of a 2048 x 6144 x 6144 product).
+__device__ __forceinline__ float normal_cdf(float z, float &e) {
+    const float u = fabsf(z) * 0.7071067811865476f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, u, 1.0f));
+    float a = fmaf(1.061405429f, t, -1.453152027f);
+    a = fmaf(a, t, 1.421413741f);
+    a = fmaf(a, t, -0.284496736f);
+    a = fmaf(a, t, 0.254829592f) * t;
+    e = lin_exp(-u * u);
+    const float tail = 0.5f * a * e;
+    return z < 0.0f ? tail : 1.0f - tail;
 }
-// The derivative; past |z| = 30 it is 0 or 1 to f32, and the factors below may be no numbers.
+template <int ACT>
+__device__ __forceinline__ float lin_act(float z) {
+    if constexpr (ACT == MI_ACT_SILU) return z * lin_sigmoid(z);
+    if constexpr (ACT == MI_ACT_GELU) {
+        float e;
+        return z * normal_cdf(z, e);
+    }
+    if constexpr (ACT == MI_ACT_GELU_TANH) return z * lin_sigmoid(gelu_inner2(z));   // (1 + tanh(u)) / 2 = sigmoid(2 u)
+    if constexpr (ACT == MI_ACT_RELU) return z < 0.0f ? 0.0f : z;        // (a NaN stays)
+    return z;
+}
+// The derivative; far out it is 0 or 1 to f32, and the factors below may be no numbers.
 __device__ __forceinline__ float lin_act_grad(float z, int act) {
-    if (act != MI_ACT_NONE && fabsf(z) > 30.0f && act != MI_ACT_SILU) return z > 0.0f ? 1.0f : 0.0f;
+    const float far = z > 0.0f ? 1.0f : 0.0f;
     switch (act) {
         case MI_ACT_SILU: {
-            if (fabsf(z) > 120.0f) return z > 0.0f ? 1.0f : 0.0f;
             const float s = lin_sigmoid(z);
-            return s * fmaf(z, lin_sigmoid(-z), 1.0f);
+            return fabsf(z) > 120.0f ? far : s * fmaf(z, lin_sigmoid(-z), 1.0f);
         }
-        case MI_ACT_GELU:
-            return fmaf(z * 0.3989422804014327f, expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.7071067811865476f)));
+        case MI_ACT_GELU: {
+            float e;
+            const float c = normal_cdf(z, e);
+            return fabsf(z) > 30.0f ? far : fmaf(z * 0.3989422804014327f, e, c);
+        }
         case MI_ACT_GELU_TANH: {
-            const float s = lin_sigmoid(gelu_inner2(z));
-            return s + z * s * (1.0f - s) * 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f);
+            const float s = lin_sigmoid(gelu_inner2(z)), r = lin_sigmoid(-gelu_inner2(z));
+            return fabsf(z) > 30.0f ? far : s + z * s * r * 1.5957691216057308f * fmaf(0.134145f * z, z, 1.0f);
         }
-        case MI_ACT_RELU: return z > 0.0f ? 1.0f : z != z ? z : 0.0f;
+        case MI_ACT_RELU: return z != z ? z : far;
         default: return 1.0f;
+    }
+}
+// f(act) with the activation as a constant.
+template <class F>
+__device__ __forceinline__ void lin_with_act(int act, F f) {
+    using std::integral_constant;
+    switch (act) {
+        case MI_ACT_SILU: return f(integral_constant<int, MI_ACT_SILU>{});
+        case MI_ACT_GELU: return f(integral_constant<int, MI_ACT_GELU>{});
+        case MI_ACT_GELU_TANH: return f(integral_constant<int, MI_ACT_GELU_TANH>{});
+        case MI_ACT_RELU: return f(integral_constant<int, MI_ACT_RELU>{});
+        default: return f(integral_constant<int, MI_ACT_NONE>{});
     }
 }
 
 // ------------------------------------------------------------------------------------------------ epilogue
-// Which accesses of four consecutive outputs are whole ones.
-struct LinQuads {
-    bool y, res, bias;
-    __device__ __forceinline__ explicit LinQuads(const LinGemm &p) {
-        const bool q = (p.R & 3) == 0;
-        const int m = p.f32 ? 15 : 7;
-        y = q && ((uintptr_t)p.y & m) == 0;
-        res = q && ((uintptr_t)p.res & m) == 0;
-        bias = q && ((uintptr_t)p.bias & 7) == 0;
-    }
-};
-
 __device__ __forceinline__ f32x4 lin_bf16x4(uint2 u) {
     return (f32x4){__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
                    __uint_as_float(u.y & 0xffff0000u)};
 }
+// To nearest even, by the conversion instruction (two values each).
 __device__ __forceinline__ uint2 lin_pack4(f32x4 v) {
-    return make_uint2(f32_to_bf16_rne(v[0]) | (f32_to_bf16_rne(v[1]) << 16),
-                      f32_to_bf16_rne(v[2]) | (f32_to_bf16_rne(v[3]) << 16));
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(uint2, __builtin_convertvector(v, bf16x4));
 }
 
-// Outputs o .. o + 3 (o a multiple of 4) of one row from their sums.
-__device__ __forceinline__ void lin_out(const LinGemm &p, const LinQuads &quad, int row, int o, f32x4 v) {
-    if (o >= p.R) return;
-    const int n = min(4, p.R - o);
-    const size_t at = (size_t)row * p.R + o;
+// Whether four consecutive outputs are one access each of y, the residual and the bias.
+__device__ __forceinline__ bool lin_quads(const LinGemm &p) {
+    const int m = p.f32 ? 15 : 7;
+    return (p.R & 3) == 0 && (((uintptr_t)p.y | (uintptr_t)p.res) & m) == 0 && ((uintptr_t)p.bias & 7) == 0;
+}
+
+// Outputs o[r] .. o[r] + 3 (multiples of 4) of N places of one row from their sums: whole accesses.  Places past R are
+// computed from the row's last ones and not stored, so that no branch surrounds a load.
+template <int ACT, int N>
+__device__ __forceinline__ void lin_out_quads(const LinGemm &p, int row, const int (&o)[N], const uint2 (&bias)[N],
+                                              f32x4 (&v)[N]) {
+    const bool in = row < p.rows;
+    const size_t at = (size_t)min(row, p.rows - 1) * p.R;
+    f32x4 res[N];
+    if (p.res) {
+        if (p.f32) {
+#pragma unroll
+            for (int r = 0; r < N; ++r) res[r] = *(const f32x4 *)((const float *)p.res + at + min(o[r], p.R - 4));
+        } else {
+            uint2 u[N];
+#pragma unroll
+            for (int r = 0; r < N; ++r) u[r] = *(const uint2 *)((const uint16_t *)p.res + at + min(o[r], p.R - 4));
+#pragma unroll
+            for (int r = 0; r < N; ++r) res[r] = lin_bf16x4(u[r]);
+        }
+    }
     if (p.bias) {
-        if (quad.bias) {
-            const f32x4 b = lin_bf16x4(*(const uint2 *)(p.bias + o));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] += b[j];
+        for (int r = 0; r < N; ++r) v[r] += lin_bf16x4(bias[r]);
+    }
+    if (p.z) {
+#pragma unroll
+        for (int r = 0; r < N; ++r)
+            if (in && o[r] < p.R) *(f32x4 *)(p.z + (size_t)row * p.ldz + o[r]) = v[r];
+    }
+#pragma unroll
+    for (int r = 0; r < N; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[r][j] = lin_act<ACT>(v[r][j]);
+    if (p.res) {
+#pragma unroll
+        for (int r = 0; r < N; ++r) v[r] += res[r];
+    }
+#pragma unroll
+    for (int r = 0; r < N; ++r) {
+        if (!in || o[r] >= p.R) continue;
+        if (p.f32) *(f32x4 *)((float *)p.y + at + o[r]) = v[r];
+        else *(uint2 *)((uint16_t *)p.y + at + o[r]) = lin_pack4(v[r]);
+    }
+}
+
+// The same for four outputs of a row, value by value.
+template <int ACT>
+__device__ __forceinline__ void lin_out_single(const LinGemm &p, int row, int o, f32x4 v) {
+    if (row >= p.rows) return;
+    const size_t at = (size_t)row * p.R + o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (o + j >= p.R) continue;
+        if (p.bias) v[j] += bf16_to_f32(p.bias[o + j]);
+        if (p.z) p.z[(size_t)row * p.ldz + o + j] = v[j];
+        v[j] = lin_act<ACT>(v[j]);
+        if (p.f32) {
+            if (p.res) v[j] += ((const float *)p.res)[at + j];
+            ((float *)p.y)[at + j] = v[j];
         } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < n) v[j] += bf16_to_f32(p.bias[o + j]);
+            if (p.res) v[j] += bf16_to_f32(((const uint16_t *)p.res)[at + j]);
+            ((uint16_t *)p.y)[at + j] = (uint16_t)f32_to_bf16_rne(v[j]);
         }
     }
-    if (p.z) *(uint2 *)(p.z + (size_t)row * p.ldz + o) = lin_pack4(v);
-    if (p.act) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = lin_act(v[j], p.act);
-    }
-    if (p.f32) {
-        float *y = (float *)p.y + at;
-        const float *r = (const float *)p.res + at;
-        if (p.res) {
-            if (quad.res) {
-                const float4 u = *(const float4 *)r;
-                v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < n) v[j] += r[j];
-            }
-        }
-        if (quad.y) {
-            *(f32x4 *)y = v;
+}
+
+// Outputs o .. o + 3 of one row.
+__device__ __forceinline__ void lin_out(const LinGemm &p, int row, int o, f32x4 v) {
+    if (o >= p.R) return;
+    lin_with_act(p.act, [&](auto act) __attribute__((always_inline)) {
+        constexpr int ACT = decltype(act)::value;
+        if (lin_quads(p)) {
+            const int at[1] = {o};
+            const uint2 bias[1] = {p.bias ? *(const uint2 *)(p.bias + o) : make_uint2(0, 0)};
+            f32x4 w[1] = {v};
+            lin_out_quads<ACT, 1>(p, row, at, bias, w);
         } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < n) y[j] = v[j];
+            lin_out_single<ACT>(p, row, o, v);
         }
-    } else {
-        uint16_t *y = (uint16_t *)p.y + at;
-        const uint16_t *r = (const uint16_t *)p.res + at;
-        if (p.res) {
-            if (quad.res) {
-                const f32x4 u = lin_bf16x4(*(const uint2 *)r);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] += u[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < n) v[j] += bf16_to_f32(r[j]);
-            }
-        }
-        if (quad.y) {
-            *(uint2 *)y = lin_pack4(v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (j < n) y[j] = (uint16_t)f32_to_bf16_rne(v[j]);
-        }
-    }
+    });
 }
 
 // ------------------------------------------------------------------------------------------------ tiled product
 __device__ __forceinline__ void lin_lds_load(__amdgpu_buffer_rsrc_t r, uint4 *dst, uint32_t voff) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 16, (int)voff, 0, 0, 0);
+}
+
+// One word of a line into a place in LDS that nobody reads: the line comes into L2.
+template <int AT>
+__device__ __forceinline__ void lin_lds_touch(__amdgpu_buffer_rsrc_t r, uint4 *dst, int voff) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 4, voff, AT, 0, 0);
 }
 
 // A slow operand's row k of a stage: the 32-byte piece u (16 columns) sits at u ^ lin_swizzle(k), so that the 16 pieces of
@@ -170,12 +222,14 @@ __host__ __device__ constexpr int lin_swizzle(int k) { return (k & 3) | ((k >> 1
 template <int T, int W, bool SLOW>
 struct LinOperand {
     static constexpr int N = T / 8 / W;          // 1 KB loads of a wavefront and stage
-    static_assert(T % (8 * W) == 0, "");
+    static_assert(T % (8 * W) == 0 && (!SLOW || (T & (T - 1)) == 0), "");
     const char *base;           // of the tile, stage 0
     long long advance;          // bytes from stage to stage
     uint32_t voff[N];
     int kat;                    // first contraction index of load 0 within the stage
     int frag;                   // byte of this lane's part of fragment 0
+    uint32_t touch_at;          // the line this lane reads ahead, and its contraction index within the stage
+    int touch_k;
 
     __device__ __forceinline__ void init(const uint16_t *m, long long ld, int first, int count, int wave, int lane,
                                          int tile0) {
@@ -211,6 +265,20 @@ struct LinOperand {
             __builtin_amdgcn_make_buffer_rsrc((void *)(base + g * advance), (short)0, 0x7fffffff, kLinWord3);
         lin_lds_load(r, lds + 64 * (j * W + wave), voff[j] | (g * kLinCols + kat + (SLOW ? j * (512 * W / T) : 0) >= k ? kLinOut : 0u));
     }
+    // Reading ahead: this lane takes line n of the T of a stage (128 bytes each), if n is below T.
+    __device__ __forceinline__ void touch_init(long long ld, int first, int count, int n) {
+        constexpr int L = SLOW ? T / 64 : 1;     // lines of a row
+        const int row = n / L, col = 64 * (n % L);
+        touch_k = SLOW ? row : 0;
+        touch_at = n < T && first + (SLOW ? col : row) < count ? (uint32_t)(2 * (row * ld + col)) : kLinOut;
+    }
+    __device__ __forceinline__ void touch(uint4 *lds, int g, int k) const {
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc((void *)(base + g * advance), (short)0, 0x7fffffff, kLinWord3);
+        const int at = (int)(touch_at | (g * kLinCols + (SLOW ? touch_k : 0) >= k ? kLinOut : 0u));
+        lin_lds_touch<0>(r, lds, at);
+        lin_lds_touch<64>(r, lds, at);
+    }
     // fragment of the 16 rows (columns) tile0 + 16 r, contraction indexes 32 half + 8 q .. + 7
     __device__ __forceinline__ lin_bf16x8 read(const uint4 *lds, int r, int half) const {
         if constexpr (SLOW) {
@@ -225,10 +293,22 @@ struct LinOperand {
     }
 };
 
+// A workgroup computes TW weight rows x TT rows, its wavefronts WM x WN of them, 64 columns a stage, NST stages in LDS.
+//
+// What bounds it: of 8 wavefronts of 128 x 64 outputs a stage takes 1.27 us of which the matrix instructions are 0.85 (at 2.4
+// GHz); 24 KB of fragments a wavefront keep LDS about as busy as they keep the matrix cores, then memory under load, tiles
+// that do not fill the last round, and the ends (7 to 9 stages' time).  8192^3 in 790 us (1.39 PFLOP/s), its gradients' products in
+// 810 and 800; a library's product, without an epilogue, takes 740, 820 and 940.  4096 x 6144 x 6144 260, 265, 285 (290, 325, 350).
+//
+// Measured and not kept: 4 wavefronts of 128 x 128 (the accumulators and two sets of fragments do not fit), 2 x 2 wavefronts for
+// 256 x 128 (20 % slower), 128 x 128 with 2 stages and 2 workgroups a CU (10 to 40 % slower than with 4 stages and one).
 template <int TW, int TT, int WM, int WN, int NST, bool SLOWA, bool SLOWB>
 __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(LinGemm p) {
     constexpr int W = WM * WN, RT = TW / WM / 16, CT = TT / WN / 16, ROWS = TW + TT;
+    constexpr bool AHEAD = TW == 192;
+    constexpr int TOUCHES = AHEAD ? 2 : 0;       // loads of a stage that read ahead
     __shared__ uint4 buf0[ROWS * 8], buf1[ROWS * 8], buf2[NST > 2 ? ROWS * 8 : 1], buf3[NST > 3 ? ROWS * 8 : 1];
+    __shared__ uint4 sink[AHEAD ? 16 * W : 1];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -253,9 +333,33 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(Lin
     B.init(p.b, p.ldb, row0, p.rows, wave, lane, wn * (TT / WN));
     constexpr int PER = A.N + B.N;
     const int kend = t1 * kLinCols, ka = min(SLOWA ? p.Ks : p.K, kend), kb = min(SLOWB ? p.Ks : p.K, kend);
+    // The columns are summed in a cycle that starts at another place for every XCD: with all of them at the same columns of
+    // rows 12 KB apart, memory answers more slowly (4096 x 6144 x 6144, tiles of 256 x 256: 325 us from the first column on,
+    // 299 so).
+    const int start = xcd * 3 % 8 * (t1 - t0) / 8;
+    auto stage_at = [&](int g) __attribute__((always_inline)) { return g + start - (g + start >= t1 ? t1 - t0 : 0); };
     auto load_piece = [&](uint4 *buf, int g, int j) __attribute__((always_inline)) {
-        if (j < A.N) A.load(buf, g, ka, wave, j);
-        else B.load(buf + 8 * TW, g, kb, wave, j - A.N);
+        if (j < A.N) A.load(buf, stage_at(g), g < t1 ? ka : 0, wave, j);
+        else B.load(buf + 8 * TW, stage_at(g), g < t1 ? kb : 0, wave, j - A.N);
+    };
+    // A stage's loads have a step to come back, less than memory takes.  So 3 stages ahead of its use a stage's lines are
+    // brought into L2, each by one of the workgroups that share them, both 64-byte halves (one word of a line brings half of it).
+    // 253 us instead of 295 of 4096 x 6144 x 6144, 135 instead of 150 of 2048.  Tiles of 256 x 256 have no registers for it.
+    if constexpr (AHEAD) {
+        const int line = wave * 64 + lane;
+        const bool mine = ((line ^ (int)(blockIdx.x >> 3)) & (kLinNear - 1)) == 0;
+        A.touch_init(p.lda, o0, p.R, mine && line < TW ? line : TW);
+        B.touch_init(p.ldb, row0, p.rows, mine && line >= TW ? line - TW : TT);
+    }
+    auto touch = [&](int g) __attribute__((always_inline)) {
+        if constexpr (AHEAD) {
+            uint4 *const to = sink + 16 * wave;
+            if (wave * 64 < TW) {
+                A.touch(to, stage_at(g), g < t1 ? ka : 0);
+            } else {
+                B.touch(to, stage_at(g), g < t1 ? kb : 0);
+            }
+        }
     };
 
     f32x4 acc[RT][CT];
@@ -286,7 +390,7 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(Lin
                 for (int n = r * READS / BAR; n < (r + 1) * READS / BAR; ++n) read(buf, 1, n);
             }
             if (r == BAR) {
-                vm_wait<(NST - 2) * PER>();
+                vm_wait<(NST - 2) * PER + TOUCHES>();
                 lds_barrier();
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -303,13 +407,15 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(Lin
             multiply(1, r);
             __builtin_amdgcn_sched_barrier(0);
         }
+        touch(g + NST + 1);
     };
     uint4 *const bufs[4] = {buf0, buf1, buf2, buf3};
 #pragma unroll
     for (int st = 0; st < NST; ++st)
 #pragma unroll
         for (int j = 0; j < PER; ++j) load_piece(bufs[st], t0 + st, j);
-    vm_wait<(NST - 1) * PER>();
+    touch(t0 + NST);
+    vm_wait<(NST - 1) * PER + TOUCHES>();
     lds_barrier();
 #pragma unroll
     for (int n = 0; n < READS; ++n) read(buf0, 0, n);
@@ -324,74 +430,84 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(Lin
     vm_wait<0>();
 
     // lane (i, q) holds outputs 4 q .. 4 q + 3 of each row tile for row 16 t + i
-    const LinQuads quad(p);
+    auto row_of = [&](int t) { return row0 + wn * (TT / WN) + 16 * t + i; };
+    auto out_of = [&](int r) { return o0 + wm * (TW / WM) + 16 * r + 4 * q; };
+    if (p.S > 1) {
 #pragma unroll
-    for (int t = 0; t < CT; ++t) {
-        const int row = row0 + wn * (TT / WN) + 16 * t + i;
-        if (row >= p.rows) continue;
+        for (int t = 0; t < CT; ++t) {
+            if (row_of(t) >= p.rows) continue;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const int o = o0 + wm * (TW / WM) + 16 * r + 4 * q;
-            if (p.S == 1) {
-                lin_out(p, quad, row, o, acc[r][t]);
-            } else if (o < p.R) {
-                float *f = p.part + ((size_t)split * p.rows + row) * p.R + o;
+            for (int r = 0; r < RT; ++r) {
+                if (out_of(r) >= p.R) continue;
+                float *f = p.part + ((size_t)split * p.rows + row_of(t)) * p.R + out_of(r);
                 if ((p.R & 3) == 0) {
                     *(f32x4 *)f = acc[r][t];
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        if (o + j < p.R) f[j] = acc[r][t][j];
+                        if (out_of(r) + j < p.R) f[j] = acc[r][t][j];
                 }
             }
         }
+        return;
     }
+    if (!lin_quads(p)) {
+        lin_with_act(p.act, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int r = 0; r < RT; ++r) lin_out_single<decltype(act)::value>(p, row_of(t), out_of(r), acc[r][t]);
+        });
+        return;
+    }
+    int o[RT];
+    uint2 bias[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        o[r] = out_of(r);
+        bias[r] = p.bias ? *(const uint2 *)(p.bias + min(o[r], p.R - 4)) : make_uint2(0, 0);
+    }
+    lin_with_act(SLOWA ? MI_ACT_NONE : p.act, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            f32x4 v[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) v[r] = acc[r][t];
+            lin_out_quads<decltype(act)::value, RT>(p, row_of(t), o, bias, v);
+        }
+    });
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
-// Up to 16 NT rows: the weights are streamed once, from memory into the matrix instructions' registers.  A workgroup takes
-// 16 RW weight rows, its W wavefronts every W-th piece of 32 U columns; their sums meet in LDS.
-template <int NT, int RW, int W, int U>
+// Up to 16 rows: the weights are streamed once, from memory into the matrix instructions' registers.  A workgroup takes 16
+// weight rows, its W wavefronts every W-th piece of 32 U columns; their sums meet in LDS.  One row through 6144 x 6144 takes
+// 17.5 us, 4.3 TB/s (a copy reaches 5.1); 8 or 16 wavefronts, or two row tiles for each, took 0 to 2 us more.
+template <int W, int U>
 __global__ void __launch_bounds__(64 * W) lin_stream_kernel(LinGemm p) {
-    __shared__ f32x4 red[W][RW * NT][64];
+    __shared__ f32x4 red[W][64];
     const int tid = threadIdx.x, lane = tid & 63, i = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int o0 = blockIdx.x * 16 * RW;
+    const int o0 = blockIdx.x * 16;
     const __amdgpu_buffer_rsrc_t ra =
         __builtin_amdgcn_make_buffer_rsrc((void *)(p.a + (size_t)o0 * p.lda), (short)0, 0x7fffffff, kLinWord3);
     const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc((void *)p.b, (short)0, 0x7fffffff, kLinWord3);
-    uint32_t va[RW], vb[NT];
-#pragma unroll
-    for (int r = 0; r < RW; ++r) va[r] = (uint32_t)(2 * (min(16 * r + i, p.R - 1 - o0) * p.lda + 8 * q));
-#pragma unroll
-    for (int t = 0; t < NT; ++t) vb[t] = (uint32_t)(2 * (min(16 * t + i, p.rows - 1) * p.ldb + 8 * q));
-    f32x4 acc[RW][NT];
-#pragma unroll
-    for (int r = 0; r < RW; ++r)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[r][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    lin_bf16x8 fa[2][RW][U], fb[2][NT][U];
+    // rows past the last one read it again: their outputs are not stored
+    const uint32_t va = (uint32_t)(2 * (min(i, p.R - 1 - o0) * p.lda + 8 * q));
+    const uint32_t vb = (uint32_t)(2 * (min(i, p.rows - 1) * p.ldb + 8 * q));
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    lin_bf16x8 fa[2][U], fb[2][U];
     auto load = [&](int s, int g) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = (g * U + u) * 32;
             const uint32_t out = k + 8 * q >= p.K ? kLinOut : 0u;
-#pragma unroll
-            for (int r = 0; r < RW; ++r)
-                fa[s][r][u] = __builtin_bit_cast(lin_bf16x8, __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(va[r] | out), 2 * k, 0));
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-                fb[s][t][u] = __builtin_bit_cast(lin_bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(vb[t] | out), 2 * k, 0));
+            fa[s][u] = __builtin_bit_cast(lin_bf16x8, __builtin_amdgcn_raw_buffer_load_b128(ra, (int)(va | out), 2 * k, 0));
+            fb[s][u] = __builtin_bit_cast(lin_bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rb, (int)(vb | out), 2 * k, 0));
         }
     };
     auto multiply = [&](int s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int r = 0; r < RW; ++r)
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    acc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[s][r][u], fb[s][t][u], acc[r][t], 0, 0, 0);
+        for (int u = 0; u < U; ++u) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[s][u], fb[s][u], acc, 0, 0, 0);
     };
     const int pieces = (p.K + 32 * U - 1) / (32 * U);
     load(0, wave);
@@ -401,19 +517,13 @@ __global__ void __launch_bounds__(64 * W) lin_stream_kernel(LinGemm p) {
         load(0, g + 2 * W);
         multiply(1);
     }
-#pragma unroll
-    for (int r = 0; r < RW; ++r)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) red[wave][r * NT + t][lane] = acc[r][t];
+    red[wave][lane] = acc;
     __syncthreads();
-    const LinQuads quad(p);
-    for (int n = wave; n < RW * NT; n += W) {
-        f32x4 v = red[0][n][lane];
+    if (wave > 0) return;
+    f32x4 v = red[0][lane];
 #pragma unroll
-        for (int w = 1; w < W; ++w) v += red[w][n][lane];
-        const int row = 16 * (n % NT) + i;
-        if (row < p.rows) lin_out(p, quad, row, o0 + 16 * (n / NT) + 4 * q, v);
-    }
+    for (int w = 1; w < W; ++w) v += red[w][lane];
+    if (i < p.rows) lin_out(p, i, o0 + 4 * q, v);
 }
 
 }  // namespace mi

@@ -41,7 +41,13 @@ static __global__ void __launch_bounds__(256) column_sums_kernel(const float *__
     const int lane = threadIdx.x & 31, piece = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float a = 0.0f;
     if (c < D)
-        for (int k = piece; k < n; k += 8) a += part[(size_t)k * D + c];
+        for (int k0 = piece; k0 < n; k0 += 64) { // eight loads at once
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = k0 + 8 * j < n ? part[(size_t)(k0 + 8 * j) * D + c] : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a += v[j];
+        }
     sum[piece][lane] = a;
     __syncthreads();
     if (piece || c >= D) return;

@@ -21,6 +21,7 @@ enum Knob : int {
     kTuneF8Tw, kTuneF8Tt, kTuneF8S,          // dense fp8 product: weight rows and tokens per tile, splits of K
     kTuneF8Stream, kTuneF8Tm,                // fp8 routed layer: most slots that stream, rows per block
     kTuneLinTw, kTuneLinTt, kTuneLinS,       // bf16 product with an epilogue: weight rows and rows per tile, splits
+    kTuneLinStream,                          // its most rows that stream
     kTuneCount
 };
 

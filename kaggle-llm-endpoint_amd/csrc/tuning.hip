@@ -33,7 +33,7 @@ const Entry kNames[] = {
     {"DG_S1", kTuneDgS1}, {"DG_S2", kTuneDgS2}, {"DG_NT", kTuneDgNt},
     {"PF_WIDE", kTunePfWide},
     {"F8_TW", kTuneF8Tw}, {"F8_TT", kTuneF8Tt}, {"F8_S", kTuneF8S}, {"F8_STREAM", kTuneF8Stream}, {"F8_TM", kTuneF8Tm},
-    {"LIN_TW", kTuneLinTw}, {"LIN_TT", kTuneLinTt}, {"LIN_S", kTuneLinS},
+    {"LIN_TW", kTuneLinTw}, {"LIN_TT", kTuneLinTt}, {"LIN_S", kTuneLinS}, {"LIN_STREAM", kTuneLinStream},
 };
 static_assert(sizeof(kNames) / sizeof(kNames[0]) == kTuneCount, "every knob has a name");
 
