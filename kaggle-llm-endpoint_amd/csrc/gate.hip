@@ -106,22 +106,21 @@ __device__ __forceinline__ float sigmoid32(float l) {
     return (l < 0.0f ? e : 1.0f) / (1.0f + e);
 }
 
-__device__ __forceinline__ double gate_key(double c, int id) {
-    c = c >= 0x1p1000 || c != c ? 0x1.fffffffffffffp1023 : c + 0.0;      // +inf and NaN: the largest; -0: 0
-    const uint2 u = __builtin_bit_cast(uint2, c);
-    const uint32_t low = (u.x & ~1023u) | ((int)u.y < 0 ? (uint32_t)id : 1023u - (uint32_t)id);
-    const bool none = u.y == 0xfff00000u;                                // -inf: out
-    return __builtin_bit_cast(double, make_uint2(none ? 0u : low, none ? kGateNone : u.y));
+__device__ __forceinline__ double gate_key(double c, int id, bool none) {
+    // the minimum makes +inf and NaN the largest double, the sum -0 to 0
+    const uint2 u = __builtin_bit_cast(uint2, fmin(c + 0.0, 0x1.fffffffffffffp1023));
+    const uint32_t flip = (uint32_t)((int)u.y >> 31);                    // all ones below 0: the lower id is the larger key
+    return __builtin_bit_cast(double, make_uint2((u.x & ~1023u) | ((1023u - (uint32_t)id) ^ (flip & 1023u)), none ? kGateNone : u.y));
 }
+__device__ __forceinline__ bool gate_out(double key) { return key < -0x1p1000; }
 __device__ __forceinline__ int gate_id(double key) {
     const uint2 u = __builtin_bit_cast(uint2, key);
-    return u.y == kGateNone ? -1 : (int)((int)u.y < 0 ? u.x & 1023u : 1023u - (u.x & 1023u));
+    return gate_out(key) ? -1 : (int)((int)u.y < 0 ? u.x & 1023u : 1023u - (u.x & 1023u));
 }
 __device__ __forceinline__ double gate_drop(double key, bool drop) {
     const uint2 u = __builtin_bit_cast(uint2, key);
     return __builtin_bit_cast(double, make_uint2(u.x, drop ? kGateNone : u.y));
 }
-__device__ __forceinline__ bool gate_out(double key) { return __builtin_bit_cast(uint2, key).y == kGateNone; }
 
 __device__ __forceinline__ double without_id(double key) {
     const uint2 u = __builtin_bit_cast(uint2, key);
@@ -226,10 +225,22 @@ __global__ void __launch_bounds__(256) moe_gate_kernel(GateArgs p) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) c[j] = sigmoid64((double)l[j]);
         }
+        if (p.bias) {
+            const float *b = p.bias + at.id0;
+            if (__ballot(at.n != PER || ((uintptr_t)b & 15)) == 0) {
+#pragma unroll
+                for (int j = 0; j < PER; j += 4) {
+                    const float4 u = *(const float4 *)(b + j);
+                    c[j] += (double)u.x, c[j + 1] += (double)u.y, c[j + 2] += (double)u.z, c[j + 3] += (double)u.w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) c[j] += j < at.n ? (double)b[j] : 0.0;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            if (p.bias && j < at.n) c[j] += (double)p.bias[at.id0 + j];
-            key[j] = gate_key(l[j] == -INFINITY ? -INFINITY : c[j], min(at.id0 + j, kGateMaxE - 1));
+            key[j] = gate_key(c[j], min(at.id0 + j, kGateMaxE - 1), l[j] == -INFINITY || c[j] == -INFINITY);
         }
     }
     if (p.n_group > 1) {
@@ -251,7 +262,7 @@ __global__ void __launch_bounds__(256) moe_gate_kernel(GateArgs p) {
         // the groups' places: a group stays if fewer than topk_group are better
         double g = without_id(a);
         if (p.group_top == 2 && !gate_out(b)) g += without_id(b);
-        g = gate_key(gate_out(a) ? -INFINITY : g, at.group);
+        g = gate_key(g, at.group, gate_out(a));
         int better = 0;
         for (int q = 0; q < p.n_group; ++q) {
             const double o = __shfl(g, (threadIdx.x & 63) / LPR * LPR + q * lanes, 64);
@@ -260,12 +271,12 @@ __global__ void __launch_bounds__(256) moe_gate_kernel(GateArgs p) {
         const bool drop = better >= p.topk_group;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            if (!p.bias) key[j] = gate_key((double)l[j], min(at.id0 + j, kGateMaxE - 1));
+            if (!p.bias) key[j] = gate_key((double)l[j], min(at.id0 + j, kGateMaxE - 1), l[j] == -INFINITY);
             key[j] = gate_drop(key[j], drop);
         }
     } else if (!p.bias) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) key[j] = gate_key((double)l[j], min(at.id0 + j, kGateMaxE - 1));
+        for (int j = 0; j < PER; ++j) key[j] = gate_key((double)l[j], min(at.id0 + j, kGateMaxE - 1), l[j] == -INFINITY);
     }
 
     int id[2] = {-1, -1};                        // of slots lane and 16 + lane (lane % 16)

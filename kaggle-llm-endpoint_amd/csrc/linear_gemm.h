@@ -34,8 +34,11 @@ struct LinGemm {
     long long ldz;
     // ---- tiled launches
     int nw, nb, S;              // weight tiles, token tiles, splits of K
-    float *part;                // S > 1: f32 [S, rows, R]
+    float *part;                // S > 1: f32 [S, rows, lin_part_ld(R)]
 };
+
+// Columns of a row of split sums: whole groups of four.
+__host__ __device__ constexpr int lin_part_ld(int R) { return (R + 3) & ~3; }
 
 // ------------------------------------------------------------------------------------------------ activations
 // e^x and 1 / x by the plain instructions: 1 ulp each, besides |x| 2^-24 for the rounding of x log2(e).
@@ -301,7 +304,8 @@ struct LinOperand {
 // 810 and 800; a library's product, without an epilogue, takes 740, 820 and 940.  4096 x 6144 x 6144 260, 265, 285 (290, 325, 350).
 //
 // Measured and not kept: 4 wavefronts of 128 x 128 (the accumulators and two sets of fragments do not fit), 2 x 2 wavefronts for
-// 256 x 128 (20 % slower), 128 x 128 with 2 stages and 2 workgroups a CU (10 to 40 % slower than with 4 stages and one).
+// 256 x 128 (20 % slower), 128 x 128 with 2 stages and 2 workgroups a CU (10 to 40 % slower than with 4 stages and one), or
+// with 4 wavefronts instead of 8 (517 x 6144 x 6144 57 us instead of 50).
 template <int TW, int TT, int WM, int WN, int NST, bool SLOWA, bool SLOWB>
 __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(LinGemm p) {
     constexpr int W = WM * WN, RT = TW / WM / 16, CT = TT / WN / 16, ROWS = TW + TT;
@@ -438,15 +442,8 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(Lin
             if (row_of(t) >= p.rows) continue;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                if (out_of(r) >= p.R) continue;
-                float *f = p.part + ((size_t)split * p.rows + row_of(t)) * p.R + out_of(r);
-                if ((p.R & 3) == 0) {
-                    *(f32x4 *)f = acc[r][t];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (out_of(r) + j < p.R) f[j] = acc[r][t][j];
-                }
+                const int ld = lin_part_ld(p.R);
+                if (out_of(r) < p.R) *(f32x4 *)(p.part + ((size_t)split * p.rows + row_of(t)) * ld + out_of(r)) = acc[r][t];
             }
         }
         return;

@@ -27,22 +27,24 @@ def _rows(t):
     return t.contiguous(), t.shape[1]
 
 
-def _gate(logits, bias, k, scores, n_group, topk_group, group_top, norm, scaling):
+def _gate(logits, args):
+    bias, k, scores, n_group, topk_group, group_top, norm, scaling = args
     T, E = logits.shape
-    idx = torch.empty((T, k), dtype=torch.int32, device=logits.device)
-    w = torch.empty((T, k), dtype=torch.float32, device=logits.device)
     stream = _stream_of("moe_gate", logits, bias)
+    dev = logits.device
+    idx = torch.empty((T, k), dtype=torch.int32, device=dev)
+    w = torch.empty((T, k), dtype=torch.float32, device=dev)
     if T:
         l, stride = _rows(logits)
-        check("mi_moe_gate", lib().mi_moe_gate(_ptr(l), _DTYPES[l.dtype], stride, _ptr(bias), T, E, k, scores, n_group,
-                                               topk_group, group_top, norm, scaling, _ptr(idx), _ptr(w), stream))
+        check("mi_moe_gate", lib().mi_moe_gate(l.data_ptr(), _DTYPES[l.dtype], stride, _ptr(bias), T, E, k, scores, n_group,
+                                               topk_group, group_top, norm, scaling, idx.data_ptr(), w.data_ptr(), stream))
     return idx, w
 
 
 class _Gate(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, *args):
-        idx, w = _gate(logits, *args)
+    def forward(ctx, logits, args):
+        idx, w = _gate(logits, args)
         ctx.save_for_backward(logits, idx)
         ctx.args = args
         ctx.mark_non_differentiable(idx)
@@ -52,21 +54,20 @@ class _Gate(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, _, gw):
-        nothing = (None,) * len(ctx.args)
         if gw is None:
-            return (None,) + nothing
+            return None, None
         logits, idx = ctx.saved_tensors
         _no_tangent("moe_gate's gradient", gw)
-        k, scores, norm, scaling = ctx.args[1], ctx.args[2], ctx.args[6], ctx.args[7]
+        bias, k, scores, n_group, topk_group, group_top, norm, scaling = ctx.args
         gw = gw.contiguous()
         T, E = logits.shape
         dl = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-        stream = _stream_of("moe_gate's gradient", logits, idx, gw)
+        stream = _stream_of("moe_gate's gradient", logits, gw)
         if T:
             l, stride = _rows(logits)
-            check("mi_moe_gate_grad", lib().mi_moe_gate_grad(_ptr(l), _DTYPES[l.dtype], stride, _ptr(idx), _ptr(gw), T, E, k,
-                                                             scores, norm, scaling, _ptr(dl), stream))
-        return (dl,) + nothing
+            check("mi_moe_gate_grad", lib().mi_moe_gate_grad(l.data_ptr(), _DTYPES[l.dtype], stride, idx.data_ptr(),
+                                                             gw.data_ptr(), T, E, k, scores, norm, scaling, dl.data_ptr(), stream))
+        return dl, None
 
 
 def moe_gate(logits, k, scores="sigmoid", bias=None, n_group=1, topk_group=1, group_top=2, norm_topk=True, scaling=1.0):
@@ -106,5 +107,5 @@ def moe_gate(logits, k, scores="sigmoid", bias=None, n_group=1, topk_group=1, gr
         raise ValueError("moe_gate: a group counts by its 1 or 2 largest choices, got %r" % (group_top,))
     args = (bias, int(k), kind, int(n_group), int(topk_group), int(group_top), 1 if norm_topk else 0, float(scaling))
     if logits.requires_grad and torch.is_grad_enabled():
-        return _Gate.apply(logits, *args)
-    return _gate(logits, *args)
+        return _Gate.apply(logits, args)
+    return _gate(logits, args)

@@ -44,15 +44,18 @@ def _checked(x, weight, eps, residual, who):
         raise ValueError("%s: eps must be a number from 0 to 1e30, got %r" % (who, eps))
 
 
-def _launch(x, weight, eps, residual, y, stream, rstd, q, s, who):
+def _like(x):
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _launch(x, weight, eps, residual, y, stream, rstd, q, s, hip):
     D = weight.numel()
-    hip = _stream_of(who, x, weight, residual, y, stream, q, s)
     x, x_stride = _rows_of(x, D)
     r_stride = 0
     if residual is not None:
         residual, r_stride = _rows_of(residual, D)
     w = _aligned(weight)
-    check("mi_rms_norm", lib().mi_rms_norm(_ptr(x), _DTYPES[x.dtype], x_stride, _ptr(residual), r_stride, _ptr(w),
+    check("mi_rms_norm", lib().mi_rms_norm(x.data_ptr(), _DTYPES[x.dtype], x_stride, _ptr(residual), r_stride, w.data_ptr(),
                                            _DTYPES[w.dtype], x.numel() // D, D, eps, _ptr(y), _ptr(stream), _ptr(rstd),
                                            _ptr(q), _ptr(s), hip))
 
@@ -60,11 +63,12 @@ def _launch(x, weight, eps, residual, y, stream, rstd, q, s, who):
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        stream = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+        hip = _stream_of("rms_norm", x, weight, residual)
+        y = _like(x)
+        stream = None if residual is None else _like(x)
         rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
         if x.numel():
-            _launch(x, weight, eps, residual, y, stream, rstd, None, None, "rms_norm")
+            _launch(x, weight, eps, residual, y, stream, rstd, None, None, hip)
         ctx.save_for_backward(x if stream is None else stream, weight, rstd)
         ctx.set_materialize_grads(False)
         return y if stream is None else (y, stream)
@@ -110,11 +114,12 @@ def rms_norm(x, weight, eps=1e-5, residual=None, y=None, stream=None):
         return _RmsNorm.apply(x, residual, weight, eps)
     if residual is None and stream is not None:
         raise ValueError("rms_norm: a stream output needs a residual")
-    y = _out(y, x.shape, x.dtype, "rms_norm", x.device)
+    hip = _stream_of("rms_norm", x, weight, residual, y, stream)
+    y = _like(x) if y is None else _out(y, x.shape, x.dtype, "rms_norm", x.device)
     if residual is not None:
-        stream = _out(stream, x.shape, x.dtype, "rms_norm", x.device)
+        stream = _like(x) if stream is None else _out(stream, x.shape, x.dtype, "rms_norm", x.device)
     if x.numel():
-        _launch(x, weight, eps, residual, y, stream, None, None, None, "rms_norm")
+        _launch(x, weight, eps, residual, y, stream, None, None, None, hip)
     return y if residual is None else (y, stream)
 
 
@@ -128,12 +133,13 @@ def fp8_rms_norm(x, weight, eps=1e-5, residual=None, want_y=False, q=None, s=Non
     if residual is None and stream is not None:
         raise ValueError("fp8_rms_norm: a stream output needs a residual")
     D = x.shape[-1]
+    hip = _stream_of("fp8_rms_norm", x, weight, residual, q, s, y, stream)
     q = _out(q, x.shape, FP8, "fp8_rms_norm", x.device)
     s = _out(s, x.shape[:-1] + (_blocks(D),), torch.float32, "fp8_rms_norm", x.device)
     if want_y or y is not None:
         y = _out(y, x.shape, x.dtype, "fp8_rms_norm", x.device)
     if residual is not None:
-        stream = _out(stream, x.shape, x.dtype, "fp8_rms_norm", x.device)
+        stream = _like(x) if stream is None else _out(stream, x.shape, x.dtype, "fp8_rms_norm", x.device)
     if x.numel():
-        _launch(x, weight, eps, residual, y, stream, None, q, s, "fp8_rms_norm")
+        _launch(x, weight, eps, residual, y, stream, None, q, s, hip)
     return (q, s), stream, y
