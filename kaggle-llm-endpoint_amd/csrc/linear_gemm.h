@@ -231,8 +231,7 @@ struct LinOperand {
     uint32_t voff[N];
     int kat;                    // first contraction index of load 0 within the stage
     int frag;                   // byte of this lane's part of fragment 0
-    uint32_t touch_at;          // the line this lane reads ahead, and its contraction index within the stage
-    int touch_k;
+    uint32_t touch_at;          // the line that this lane reads ahead
 
     __device__ __forceinline__ void init(const uint16_t *m, long long ld, int first, int count, int wave, int lane,
                                          int tile0) {
@@ -268,19 +267,17 @@ struct LinOperand {
             __builtin_amdgcn_make_buffer_rsrc((void *)(base + g * advance), (short)0, 0x7fffffff, kLinWord3);
         lin_lds_load(r, lds + 64 * (j * W + wave), voff[j] | (g * kLinCols + kat + (SLOW ? j * (512 * W / T) : 0) >= k ? kLinOut : 0u));
     }
-    // Reading ahead: this lane takes line n of the T of a stage (128 bytes each), if n is below T.
+    // Reading ahead (of a fast operand): this lane takes row n's line of a stage, 128 bytes, if n is below T.
     __device__ __forceinline__ void touch_init(long long ld, int first, int count, int n) {
-        constexpr int L = SLOW ? T / 64 : 1;     // lines of a row
-        const int row = n / L, col = 64 * (n % L);
-        touch_k = SLOW ? row : 0;
-        touch_at = n < T && first + (SLOW ? col : row) < count ? (uint32_t)(2 * (row * ld + col)) : kLinOut;
+        static_assert(!SLOW, "");
+        touch_at = n < T && first + n < count ? (uint32_t)(2 * n * ld) : kLinOut;
     }
+    // both halves of the line, as far as the row reaches (k: the first column behind it)
     __device__ __forceinline__ void touch(uint4 *lds, int g, int k) const {
         const __amdgpu_buffer_rsrc_t r =
             __builtin_amdgcn_make_buffer_rsrc((void *)(base + g * advance), (short)0, 0x7fffffff, kLinWord3);
-        const int at = (int)(touch_at | (g * kLinCols + (SLOW ? touch_k : 0) >= k ? kLinOut : 0u));
-        lin_lds_touch<0>(r, lds, at);
-        lin_lds_touch<64>(r, lds, at);
+        lin_lds_touch<0>(r, lds, (int)(touch_at | (g * kLinCols >= k ? kLinOut : 0u)));
+        lin_lds_touch<64>(r, lds, (int)(touch_at | (g * kLinCols + kLinCols / 2 >= k ? kLinOut : 0u)));
     }
     // fragment of the 16 rows (columns) tile0 + 16 r, contraction indexes 32 half + 8 q .. + 7
     __device__ __forceinline__ lin_bf16x8 read(const uint4 *lds, int r, int half) const {
