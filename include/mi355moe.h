@@ -502,8 +502,8 @@ int mi_moe_combine_grad(const void *dout, const void *y, int32_t dtype, int32_t 
                         float *dw, void *stream);
 
 /*
- * Root-mean-square norm of T rows of D values (bf16 or f32, dtype; D % 8 == 0, D <= 32768, T <= 2^22), with the residual's
- * addition before it (the norms around the blocks whose products are above):
+ * Root-mean-square norm of T rows of D values (bf16 or f32, dtype; D % 8 == 0, D <= 32768, T <= 2^22, below it where D is
+ * past 8192), with the residual's addition before it (the norms around the blocks whose products are above):
  *   s = x + residual, rounded to dtype (s = x where residual is NULL; else written to stream_out, if that is given)
  *   r = f32(1 / sqrt(mean(s^2) + eps)), the squares added in 64 bits, 0 <= eps <= 1e30
  *   y = (s * r) * w, each product rounded to f32

@@ -313,6 +313,7 @@ extern "C" int mi_rms_norm(const void *x, int32_t dtype, int64_t x_stride, const
     const NormFwd p = {x, residual, w, w_dtype == MI_X_F32, x_stride, residual_stride, T, D, eps, y, stream_out, rstd, q, qs};
     return norm_shape(D, [&](auto lanes, auto nv) {
         constexpr int L = decltype(lanes)::value, N = decltype(nv)::value, ROWS = L < 256 ? 256 / L : 1;
+        if (L >= 256 && (long long)T * L >= (1ll << 32)) return (int)MI_ERR_TOKENS;      // a grid's threads
         auto kern = dtype == MI_X_BF16 ? rms_norm_kernel<MI_X_BF16, L, N> : rms_norm_kernel<MI_X_F32, L, N>;
         hipLaunchKernelGGL(kern, dim3((T + ROWS - 1) / ROWS), dim3(L < 256 ? 256 : L), 0, (hipStream_t)stream, p);
         return hipGetLastError() == hipSuccess ? (int)MI_OK : (int)MI_ERR_LAUNCH;

@@ -45,6 +45,7 @@ def test_rms_norm(abi):
         abi("mi_rms_norm", NORM, "ARG", **{name: 2})
     for T in (0, -1, (1 << 22) + 1):
         abi("mi_rms_norm", NORM, "TOKENS", T=T)
+    abi("mi_rms_norm", NORM, "TOKENS", T=1 << 22, D=8200, x_stride=8200, residual_stride=8200)     # 2^32 threads
     for d in (0, -8, 63, 32776):
         abi("mi_rms_norm", NORM, "SHAPE", D=d, x_stride=1 << 16, residual_stride=1 << 16)
     abi("mi_rms_norm", NORM, "SHAPE", D=56, q=A, qs=B)
