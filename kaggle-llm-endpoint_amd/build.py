@@ -6,8 +6,8 @@ The library is a plain C-ABI shared object (include/mi355moe.h) that the package
 measurement-only library, ``libmi355probe.so`` (the streaming-read probe the benchmark times), is built beside it
 from csrc/probe.hip and is not part of the operator's ABI.  The grouped
 kernels are compiled once per (mode, format) from k_grouped.hip, the persistent CB3 kernels once per (mode, token
-class) from k_pstream.hip, the CU-balanced ones once per mode from k_custream.hip and the prefill GEMMs once per
-(mode, rounding form) from k_prefill.hip; all units compile in parallel, then link.
+class) from k_pstream.hip, the CU-balanced ones once per mode from k_custream.hip, the prefill GEMMs once per
+(mode, rounding form) from k_prefill.hip and the bf16 product's tiles from k_linear.hip; all units compile in parallel, then link.
 """
 import hashlib
 import os
@@ -41,6 +41,8 @@ UNITS = [("moe_decode.hip", [], "moe_decode"), ("int8_project.hip", [], "int8_pr
          ("linear.hip", [], "linear")]
 UNITS += [("k_grouped.hip", ["-DMI_KMODE=%d" % m, "-DMI_KQT=%d" % q], "k_grouped_%d_%d" % (m, q))
           for m in (0, 1, 2) for q in (1, 2, 3, 4, 5, 6)]
+# the bf16 product's tiles (weight rows * 1000 + rows)
+UNITS += [("k_linear.hip", ["-DMI_LIN_TILE=%d" % t], "k_linear_%d" % t) for t in (256256, 192256, 256128, 128128, 128064)]
 UNITS += [("k_fused.hip", [], "k_fused")]
 UNITS += [("k_pstream.hip", ["-DMI_PMODE=%d" % m, "-DMI_PTC=%d" % tc], "k_pstream_%d_%d" % (m, tc))
           for m in (0, 1) for tc in (8, 16)]

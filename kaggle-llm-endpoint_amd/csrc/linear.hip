@@ -107,22 +107,6 @@ static size_t lin_up(size_t n) { return (n + 255) & ~(size_t)255; }
 static bool lin_aligned(const void *a, int n) { return ((uintptr_t)a & (n - 1)) == 0; }
 static int lin_ok() { return hipGetLastError() == hipSuccess ? MI_OK : MI_ERR_LAUNCH; }
 
-// FAST: for a product of two fast operands only.
-template <int TW, int TT, int WM, int WN, int NST, bool FAST = false>
-static int lin_launch_tile(LinGemm p, bool slow_a, bool slow_b, hipStream_t st) {
-    p.nw = (p.R + TW - 1) / TW;
-    p.nb = (p.rows + TT - 1) / TT;
-    const long long total = (long long)p.nw * p.nb * p.S, grid = (total + 7) / 8 * 8;
-    if (grid >= (1ll << 31) / (64 * WM * WN)) return MI_ERR_TOKENS;
-    auto kern = lin_gemm_kernel<TW, TT, WM, WN, NST, false, false>;
-    if constexpr (!FAST) {
-        if (slow_b) kern = lin_gemm_kernel<TW, TT, WM, WN, NST, true, true>;
-        else if (slow_a) kern = lin_gemm_kernel<TW, TT, WM, WN, NST, true, false>;
-    }
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * WM * WN), 0, st, p);
-    return lin_ok();
-}
-
 struct LinPlan {
     int tw, tt, S;
 };
@@ -174,11 +158,11 @@ static int lin_launch(LinGemm p, bool slow_a, bool slow_b, float *part, hipStrea
     p.S = pl.S;
     p.part = part;
     int rc;
-    if (pl.tw == 192) rc = lin_launch_tile<192, 256, 2, 4, 2, true>(p, slow_a, slow_b, st);
-    else if (pl.tt == 256) rc = lin_launch_tile<256, 256, 2, 4, 2>(p, slow_a, slow_b, st);
-    else if (pl.tw == 256) rc = lin_launch_tile<256, 128, 4, 2, 3>(p, slow_a, slow_b, st);
-    else if (pl.tt == 128) rc = lin_launch_tile<128, 128, 2, 4, 4>(p, slow_a, slow_b, st);
-    else rc = lin_launch_tile<128, 64, 2, 2, 3>(p, slow_a, slow_b, st);
+    if (pl.tw == 192) rc = lin_launch_192_256(p, slow_a, slow_b, st);
+    else if (pl.tt == 256) rc = lin_launch_256_256(p, slow_a, slow_b, st);
+    else if (pl.tw == 256) rc = lin_launch_256_128(p, slow_a, slow_b, st);
+    else if (pl.tt == 128) rc = lin_launch_128_128(p, slow_a, slow_b, st);
+    else rc = lin_launch_128_64(p, slow_a, slow_b, st);
     if (rc != MI_OK || p.S == 1) return rc;
     const long long n = (long long)p.rows * ((p.R + 3) / 4);
     hipLaunchKernelGGL(lin_reduce_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p);

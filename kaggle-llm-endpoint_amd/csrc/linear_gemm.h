@@ -168,17 +168,22 @@ __device__ __forceinline__ void lin_out_quads(const LinGemm &p, int row, const i
     }
 }
 
-// The same for four outputs of a row, value by value.
-template <int ACT>
-__device__ __forceinline__ void lin_out_single(const LinGemm &p, int row, int o, f32x4 v) {
+// The same for four outputs of a row, value by value, before and after the activation.
+__device__ __forceinline__ void lin_single_before(const LinGemm &p, int row, int o, f32x4 &v) {
     if (row >= p.rows) return;
-    const size_t at = (size_t)row * p.R + o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (o + j >= p.R) continue;
         if (p.bias) v[j] += bf16_to_f32(p.bias[o + j]);
         if (p.z) p.z[(size_t)row * p.ldz + o + j] = v[j];
-        v[j] = lin_act<ACT>(v[j]);
+    }
+}
+__device__ __forceinline__ void lin_single_after(const LinGemm &p, int row, int o, f32x4 v) {
+    if (row >= p.rows) return;
+    const size_t at = (size_t)row * p.R + o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (o + j >= p.R) continue;
         if (p.f32) {
             if (p.res) v[j] += ((const float *)p.res)[at + j];
             ((float *)p.y)[at + j] = v[j];
@@ -192,17 +197,21 @@ __device__ __forceinline__ void lin_out_single(const LinGemm &p, int row, int o,
 // Outputs o .. o + 3 of one row.
 __device__ __forceinline__ void lin_out(const LinGemm &p, int row, int o, f32x4 v) {
     if (o >= p.R) return;
-    lin_with_act(p.act, [&](auto act) __attribute__((always_inline)) {
-        constexpr int ACT = decltype(act)::value;
-        if (lin_quads(p)) {
+    if (lin_quads(p)) {
+        lin_with_act(p.act, [&](auto act) __attribute__((always_inline)) {
             const int at[1] = {o};
             const uint2 bias[1] = {p.bias ? *(const uint2 *)(p.bias + o) : make_uint2(0, 0)};
             f32x4 w[1] = {v};
-            lin_out_quads<ACT, 1>(p, row, at, bias, w);
-        } else {
-            lin_out_single<ACT>(p, row, o, v);
-        }
+            lin_out_quads<decltype(act)::value, 1>(p, row, at, bias, w);
+        });
+        return;
+    }
+    lin_single_before(p, row, o, v);
+    lin_with_act(p.act, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = lin_act<decltype(act)::value>(v[j]);
     });
+    lin_single_after(p, row, o, v);
 }
 
 // ------------------------------------------------------------------------------------------------ tiled product
@@ -446,12 +455,22 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(Lin
         return;
     }
     if (!lin_quads(p)) {
-        lin_with_act(p.act, [&](auto act) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) lin_single_before(p, row_of(t), out_of(r), acc[r][t]);
+        if constexpr (!SLOWA) lin_with_act(p.act, [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < CT; ++t)
 #pragma unroll
-                for (int r = 0; r < RT; ++r) lin_out_single<decltype(act)::value>(p, row_of(t), out_of(r), acc[r][t]);
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[r][t][j] = lin_act<decltype(act)::value>(acc[r][t][j]);
         });
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) lin_single_after(p, row_of(t), out_of(r), acc[r][t]);
         return;
     }
     int o[RT];
@@ -461,7 +480,8 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(Lin
         o[r] = out_of(r);
         bias[r] = p.bias ? *(const uint2 *)(p.bias + min(o[r], p.R - 4)) : make_uint2(0, 0);
     }
-    lin_with_act(SLOWA ? MI_ACT_NONE : p.act, [&](auto act) __attribute__((always_inline)) {
+    // (of the gradients' products nothing but y: the struct's other members are not set)
+    auto out = [&](auto act) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             f32x4 v[RT];
@@ -469,8 +489,17 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(Lin
             for (int r = 0; r < RT; ++r) v[r] = acc[r][t];
             lin_out_quads<decltype(act)::value, RT>(p, row_of(t), o, bias, v);
         }
-    });
+    };
+    if constexpr (SLOWA) out(std::integral_constant<int, MI_ACT_NONE>{});
+    else lin_with_act(p.act, out);
 }
+
+// The tiles (k_linear.hip, one unit each): launches a product of them.
+int lin_launch_128_64(LinGemm p, bool slow_a, bool slow_b, hipStream_t st);
+int lin_launch_128_128(LinGemm p, bool slow_a, bool slow_b, hipStream_t st);
+int lin_launch_256_128(LinGemm p, bool slow_a, bool slow_b, hipStream_t st);
+int lin_launch_256_256(LinGemm p, bool slow_a, bool slow_b, hipStream_t st);
+int lin_launch_192_256(LinGemm p, bool slow_a, bool slow_b, hipStream_t st);     // two fast operands only
 
 // ------------------------------------------------------------------------------------------------ few rows
 // Up to 16 rows: the weights are streamed once, from memory into the matrix instructions' registers.  A workgroup takes 16
