@@ -550,7 +550,8 @@ int mi_moe_gate_grad(const void *logits, int32_t dtype, int64_t stride, const in
  *   z = x W + bias in f32 (bf16 products, exact; f32 sums), y = act(z) + residual, rounded once to y_dtype
  * x bf16 [B, n_in], row stride x_stride elements (a multiple of 8, up to 2^20); wT bf16 [n_out, n_in] (the reference's leaf
  * transposed once, as for mi_bf16_project); bias bf16 [n_out] or NULL; residual [B, n_out] of y_dtype (MI_X_BF16 or
- * MI_X_F32) or NULL; act MI_ACT_*: silu z sigmoid(z), gelu z Phi(z), its tanh form, relu.  z (may be NULL): z in f32, rows
+ * MI_X_F32) or NULL; act MI_ACT_*: silu z sigmoid(z), gelu z Phi(z), its tanh form, relu, each
+ * right relative to its own size (besides what rounds the argument of its exponential).  z (may be NULL): z in f32, rows
  * of n_out rounded up to 8 columns, for the gradient.  1 <= B <= 2^20, n_in % 8 == 0, n_in and n_out <= 2^16.  x, wT, z and
  * the workspace 16-byte aligned.  Workspace: mi_bf16_linear_workspace bytes, no initialisation; its size serves every smaller B.
  * Calls of few rows that stream the weights need none (the size is 0, as for a shape that the call refuses).
