@@ -7,7 +7,7 @@
 Products of bf16 values are exact and summed in f32; bias, activation and residual follow in f32, and the result is rounded
 once.  Gradients of x, the weight, the bias and the residual are recorded, first order and reverse mode only (a forward-mode
 tangent is refused); for an activation the forward pass keeps the values before it, in f32 (rounded to bf16
-they would cost the gradients another such rounding).  Sums in a fixed order,
+they would cost the gradients another such rounding), unless the residual's gradient is the only one asked for.  Sums in a fixed order,
 without atomics.  A captured backward pass needs leaves of its own (``x.detach().requires_grad_()`` inside the capture): an
 eager graph that still holds the same leaves has bound their gradients to another stream.  Everything runs on the current
 torch (HIP) stream of the current device; outputs and workspaces must not overlap the inputs or each other.
@@ -51,7 +51,9 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, wT, bias, residual, act, dtype):
         B, R = x.shape[0], wT.shape[0]
         y = torch.empty((B, R), dtype=dtype, device=x.device)
-        z = torch.empty((B, -(-R // 8) * 8), dtype=torch.float32, device=x.device) if act else None
+        # (the residual's gradient is dy: z serves the others only)
+        keep = act and any(ctx.needs_input_grad[:3])
+        z = torch.empty((B, -(-R // 8) * 8), dtype=torch.float32, device=x.device) if keep else None
         if B:
             _linear(x, wT, bias, act, residual, dtype, y, z, None)
         ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, wT if ctx.needs_input_grad[0] else None, z)
