@@ -140,9 +140,10 @@ static LinPlan lin_plan(int rows, int R, int K, bool fast) {
     for (const Tile &c : tiles) {
         if ((c.tw == 192 && !fast) || (tw && c.tw != tw) || (tt && c.tt != tt)) continue;
         const long long n = (long long)((R + c.tw - 1) / c.tw) * ((rows + c.tt - 1) / c.tt);
-        for (int S = 1; S <= std::min(kLinMaxSplits, steps); ++S) {
-            if (S > 1 && (n * S > c.slots || (size_t)S * rows * lin_part_ld(R) > lin_split_floats(R))) break;
-            if (fs && S != fs) continue;
+        // a forced count of splits is taken as far as the columns, the slots and the workspace hold it: the tile stays
+        int most = std::max(std::min(fs ? std::min(fs, kLinMaxSplits) : kLinMaxSplits, steps), 1);
+        while (most > 1 && (n * most > c.slots || (size_t)most * rows * lin_part_ld(R) > lin_split_floats(R))) --most;
+        for (int S = fs ? most : 1; S <= most; ++S) {
             const long long wgs = n * S;
             const float step = wgs <= kLinCus ? c.one : (float)((wgs + c.slots - 1) / c.slots) * c.more;
             const float us = step * ((steps + S - 1) / S + c.ends) +
