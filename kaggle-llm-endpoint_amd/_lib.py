@@ -26,6 +26,7 @@ I8_CTR_BYTES = 2 * 1024 * 128   # counters at the start of every int8 / bf16 str
 MI_W_BF16 = 3                # mi_mlp_many: bf16 weights
 MI_I8_COL_AFTER = 2          # s [n_out] applied after the dot (the int8 lm_head)
 MI_I8_TILED = 0x100          # OR'ed into scale_axis: qT in the tiled layout of mi_int8_tile
+INT_MAX = (1 << 31) - 1      # a larger count is passed as this one, which the entry refuses: ctypes would drop its high bits
 MI_GATE_SIGMOID = 0          # mi_moe_gate's scores
 MI_GATE_SOFTMAX = 1
 MI_ACT_NONE = 0              # mi_bf16_linear's activations

@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import INT_MAX, check, lib
 from .fp8 import _DTYPES, _no_tangent, _stream_of
 from .resident import _ptr
 
@@ -36,8 +36,8 @@ def _gate(logits, args):
     w = torch.empty((T, k), dtype=torch.float32, device=dev)
     if T:
         l, stride = _rows(logits)
-        check("mi_moe_gate", lib().mi_moe_gate(l.data_ptr(), _DTYPES[l.dtype], stride, _ptr(bias), T, E, k, scores, n_group,
-                                               topk_group, group_top, norm, scaling, idx.data_ptr(), w.data_ptr(), stream))
+        check("mi_moe_gate", lib().mi_moe_gate(l.data_ptr(), _DTYPES[l.dtype], stride, _ptr(bias), min(T, INT_MAX), E, k, scores,
+                                               n_group, topk_group, group_top, norm, scaling, idx.data_ptr(), w.data_ptr(), stream))
     return idx, w
 
 

@@ -6,8 +6,8 @@
 
 Products of bf16 values are exact and summed in f32; bias, activation and residual follow in f32, and the result is rounded
 once.  Gradients of x, the weight, the bias and the residual are recorded, first order and reverse mode only (a forward-mode
-tangent is refused); for an activation the forward pass keeps the values before it, in f32 (rounded to bf16
-they would cost the gradients another such rounding), unless the residual's gradient is the only one asked for.  Sums in a fixed order,
+tangent is refused); for an activation the forward pass keeps the values before it, in f32 (rounded to bf16 they would cost
+the gradients another such rounding), unless the residual's gradient is the only one asked for.  Sums in a fixed order,
 without atomics.  A captured backward pass needs leaves of its own (``x.detach().requires_grad_()`` inside the capture): an
 eager graph that still holds the same leaves has bound their gradients to another stream.  Everything runs on the current
 torch (HIP) stream of the current device; outputs and workspaces must not overlap the inputs or each other.
@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import check, lib
+from ._lib import INT_MAX, check, lib
 from .fp8 import _DTYPES, _aligned, _no_tangent, _out, _stream_of, _workspace
 from .resident import Bf16Leaf, _ptr
 
@@ -34,8 +34,7 @@ def _rows_of(x):
 
 
 def _linear(x, wT, bias, act, residual, dtype, y, z, workspace):
-    B, K = x.shape
-    R = wT.shape[0]
+    B, K, R = min(x.shape[0], INT_MAX), min(x.shape[1], INT_MAX), min(wT.shape[0], INT_MAX)
     stream = _stream_of("bf16_linear", x, wT, bias, residual, y, z, workspace)
     x, stride = _rows_of(x)
     wT = _aligned(wT)

@@ -16,7 +16,7 @@ overlap the inputs or each other.
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._lib import check, lib
+from ._lib import INT_MAX, check, lib
 from .fp8 import _DTYPES, FP8, _aligned, _blocks, _no_grad, _no_tangent, _out, _stream_of
 from .resident import _ptr
 
@@ -56,8 +56,8 @@ def _launch(x, weight, eps, residual, y, stream, rstd, q, s, hip):
         residual, r_stride = _rows_of(residual, D)
     w = _aligned(weight)
     check("mi_rms_norm", lib().mi_rms_norm(x.data_ptr(), _DTYPES[x.dtype], x_stride, _ptr(residual), r_stride, w.data_ptr(),
-                                           _DTYPES[w.dtype], x.numel() // D, D, eps, _ptr(y), _ptr(stream), _ptr(rstd),
-                                           _ptr(q), _ptr(s), hip))
+                                           _DTYPES[w.dtype], min(x.numel() // D, INT_MAX), min(D, INT_MAX), eps, _ptr(y),
+                                           _ptr(stream), _ptr(rstd), _ptr(q), _ptr(s), hip))
 
 
 class _RmsNorm(torch.autograd.Function):
