@@ -546,8 +546,9 @@ int mi_moe_gate_grad(const void *logits, int32_t dtype, int64_t stride, const in
                      int32_t E, int32_t k, int32_t scores, int32_t norm_topk, float scaling, void *dlogits, void *stream);
 
 /*
- * Product over bf16 weights for any number of rows, with bias, activation and residual, and its gradients:
+ * Product over bf16 weights for one row to many, with bias, activation and residual, and its gradients:
  *   z = x W + bias in f32 (bf16 products, exact; f32 sums), y = act(z) + residual, rounded once to y_dtype
+ * (Without atomics: equal calls give equal bits.  The order of a row's sums depends on B and on the row's place.)
  * x bf16 [B, n_in], row stride x_stride elements (a multiple of 8, up to 2^20); wT bf16 [n_out, n_in] (the reference's leaf
  * transposed once, as for mi_bf16_project); bias bf16 [n_out] or NULL; residual [B, n_out] of y_dtype (MI_X_BF16 or
  * MI_X_F32) or NULL; act MI_ACT_*: silu z sigmoid(z), gelu z Phi(z), its tanh form, relu, each
@@ -583,8 +584,8 @@ size_t mi_bf16_linear_grad_workspace(int32_t B, int32_t n_in, int32_t n_out);
  * CS1, CS2 with _RTW; MGMAX), launch-family switches (CUSTREAM, CUMULTI, PERSIST_ABOVE, FUSE_SWIGLU, CU_FORM_H), the
  * one-launch decode's poll limit (SPIN_LIMIT), the int8 split plan (I8S, I8_WAVES, I8_FUSE) and the many-token MLP's
  * splits and token tile (DG_S1, DG_S2, DG_NT), the prefill's wide blocks (PF_WIDE), the dense fp8 product's tile and
- * splits (F8_TW, F8_TT, F8_S) and the fp8 routed layer's streaming limit and rows per block (F8_STREAM, F8_TM), the tile and splits of the bf16 product with an
- * epilogue and its streaming limit (LIN_TW, LIN_TT, LIN_S, LIN_STREAM).
+ * splits (F8_TW, F8_TT, F8_S) and the fp8 routed layer's streaming limit and rows per block (F8_STREAM, F8_TM), the
+ * tile and splits of the bf16 product with an epilogue and its streaming limit (LIN_TW, LIN_TT, LIN_S, LIN_STREAM).
  * Overrides change launch shapes and summation orders, never the result beyond f32 rounding (of the fp8 MLP and routed
  * layer: beyond what that moves of h when it is rounded to e4m3, and F8_TM or F8_TT above 128 takes gate and up from f32
  * sums to the fp8 instruction's); workspace sizes follow them, so set them before sizing a workspace.  Not synchronised with calls running on other host threads.

@@ -1,4 +1,4 @@
-// Products over bf16 weights with bias, activation and residual, for any number of rows, and their gradients
+// Products over bf16 weights with bias, activation and residual, for one row to many, and their gradients
 // (linear_gemm.h), behind the C ABI.
 #include <algorithm>
 
@@ -28,8 +28,10 @@ __global__ void __launch_bounds__(256) lin_reduce_kernel(LinGemm p) {
     lin_out(p, row, 4 * (int)(at - (long long)row * quads), v);
 }
 
-// dz = dy act'(z), rounded to bf16 for the products (2^-9 of each term), in rows of ldz columns whose last ones are zeros,
-// and each workgroup's sums of dz (before their rounding) over its rows, for the bias.  A workgroup takes 256 columns, 32
+// dz = dy act'(z), rounded to bf16 for the products, whose matrix instructions take bf16 (each term off by at most 2^-8 of
+// itself; dx and dW of 2048 x 6144 x 6144 behind gelu come out 0.00233 of their 2-norm off instead of the 0.00166 of their own
+// rounding; a second product with what the rounding leaves would double their time), in rows of ldz columns whose last ones
+// are zeros, and each workgroup's sums of dz (before their rounding) over its rows, for the bias.  A workgroup takes 256 columns, 32
 // lanes of 8, and rows blockIdx.y * 8 + .., 8 at a time.
 struct LinDz {
     const void *dy;             // [B, N]
@@ -122,8 +124,9 @@ static size_t lin_split_floats(int R) {
 // The tile and the splits of the contraction: the pair of least estimated time.  A stage of 64 columns of a tile takes `one`
 // us in a launch of at most one workgroup per CU, `more` in each round of `slots` workgroups otherwise, its start and epilogue
 // as much as `ends` stages; a split adds a launch and a pass over its sums.  The times are those of operands from memory:
-// 6144 x 6144, 37 / 48 / 128 / 256 / 517 / 2048 / 4096 rows take 18 (of 2051 outputs), 23, 29, 40, 53, 135 and 260 us with
-// the tiles that this chooses; all with 256 x 256 would take 140 to 158 up to 2048 rows and 284.
+// 6144 x 6144, 37 / 48 / 128 / 256 / 517 / 2048 / 4096 rows take 15 (of 2051 outputs), 22.5, 29, 42, 50, 130 and 258 us with
+// the tiles that this chooses; all with 256 x 256 would take 140 to 158 up to 2048 rows and 285.  3000 / 4096 / 6000 rows take
+// 225 / 258 / 394 with 256 x 128 (chosen for the first two) and 246 / 255 / 379 with 192 x 256 (for the last).
 static LinPlan lin_plan(int rows, int R, int K, bool fast) {
     struct Tile {
         int tw, tt, slots;

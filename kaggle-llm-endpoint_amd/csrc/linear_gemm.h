@@ -313,6 +313,10 @@ struct LinOperand {
 // that do not fill the last round, and the ends (7 to 9 stages' time).  8192^3 in 790 us (1.39 PFLOP/s), its gradients' products in
 // 810 and 800; a library's product, without an epilogue, takes 740, 820 and 940.  4096 x 6144 x 6144 260, 265, 285 (290, 325, 350).
 //
+// The tiles of 192 x 256 and 256 x 256 hold 96 and 128 sums a lane and spill: 207, and 480 / 152 / 121 (forward, dx, dW) registers,
+// almost all of them in the epilogue, which has every activation, whole accesses and the value-by-value form in one kernel; the
+// loop has one reload, of the dW form.
+//
 // Measured and not kept: 4 wavefronts of 128 x 128 (the accumulators and two sets of fragments do not fit), 2 x 2 wavefronts for
 // 256 x 128 (20 % slower), 128 x 128 with 2 stages and 2 workgroups a CU (10 to 40 % slower than with 4 stages and one), or
 // with 4 wavefronts instead of 8 (517 x 6144 x 6144 57 us instead of 50).
@@ -358,7 +362,8 @@ __global__ void __launch_bounds__(64 * WM * WN, WM * WN / 4) lin_gemm_kernel(Lin
     };
     // A stage's loads have a step to come back, less than memory takes.  So 3 stages ahead of its use a stage's lines are
     // brought into L2, each by one of the workgroups that share them, both 64-byte halves (one word of a line brings half of it).
-    // 253 us instead of 295 of 4096 x 6144 x 6144, 135 instead of 150 of 2048.  Tiles of 256 x 256 have no registers for it.
+    // 253 us instead of 295 of 4096 x 6144 x 6144 in these tiles (where 256 x 128 without it take 258, and are chosen), 135 instead
+    // of 150 of 2048.  Tiles of 256 x 256 have no registers for it.
     if constexpr (AHEAD) {
         const int line = wave * 64 + lane;
         const bool mine = ((line ^ (int)(blockIdx.x >> 3)) & (kLinNear - 1)) == 0;

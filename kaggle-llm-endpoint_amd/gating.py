@@ -75,7 +75,7 @@ def moe_gate(logits, k, scores="sigmoid", bias=None, n_group=1, topk_group=1, gr
     c = s + bias (f32 [E]); with ``n_group`` > 1 (a power of two, up to 32) the E / n_group consecutive experts of a group
     stay if it is one of the ``topk_group`` with the largest sum of their ``group_top`` (1 or 2) largest choices; idx = the k
     largest choices (equal ones: the lower id), w = s[idx], divided by their sum + 1e-20 with ``norm_topk``, times
-    ``scaling``.  E up to 1024, k up to 32.
+    ``scaling``.  E up to 1024, k up to 32, T up to 2^22.
 
     An expert whose logit is -inf is out of service.  A slot that no expert is left for has id -1 and weight 0, which
     ragged_plan, fp8_moe and moe_combine take as nothing.  Choices are compared in 64 bits (within 2^-42 of each other's size

@@ -7,10 +7,13 @@
 Products of bf16 values are exact and summed in f32; bias, activation and residual follow in f32, and the result is rounded
 once.  Gradients of x, the weight, the bias and the residual are recorded, first order and reverse mode only (a forward-mode
 tangent is refused); for an activation the forward pass keeps the values before it, in f32 (rounded to bf16 they would cost
-the gradients another such rounding), unless the residual's gradient is the only one asked for.  Sums in a fixed order,
-without atomics.  A captured backward pass needs leaves of its own (``x.detach().requires_grad_()`` inside the capture): an
-eager graph that still holds the same leaves has bound their gradients to another stream.  Everything runs on the current
-torch (HIP) stream of the current device; outputs and workspaces must not overlap the inputs or each other.
+the gradients another such rounding), unless the residual's gradient is the only one asked for.  Sums without atomics, in an
+order that the call's sizes and a row's place in it decide: equal calls give equal bits, but a row's last bits may change
+with the number of rows, or between equal rows of one call.  For the products of the gradients act'(z) dy is rounded to bf16
+(where it is not dy itself, in bf16).  A captured backward pass needs leaves of its own (``x.detach().requires_grad_()``
+inside the capture): an eager graph that still holds the same leaves has bound their gradients to another stream.
+Everything runs on the current torch (HIP) stream of the current device; outputs and workspaces must not overlap the inputs
+or each other.
 """
 import torch
 from torch.autograd.function import once_differentiable
@@ -91,9 +94,10 @@ class _Linear(torch.autograd.Function):
 
 
 def bf16_linear(x, w, bias=None, act=None, residual=None, dtype=torch.bfloat16, y=None, workspace=None):
-    """y = act(x W + bias) + residual: x bf16 [B, n_in] (any B, n_in a multiple of 8; rows may be strided), w a Bf16Leaf
-    (any n_out) or the reference's W bf16 [n_in, n_out], transposed in the call; bias bf16 [n_out]; act None, "silu", "gelu",
-    "gelu_tanh" or "relu"; residual [B, n_out] of ``dtype`` -> y [B, n_out] of ``dtype`` (bf16 or f32).  ``y`` and
+    """y = act(x W + bias) + residual: x bf16 [B, n_in] (B up to 2^20, n_in a multiple of 8 up to 65536; rows may be
+    strided), w a Bf16Leaf (n_out up to 65536; bf16_project takes a wider vocabulary) or the reference's W bf16 [n_in, n_out],
+    transposed in the call; bias bf16 [n_out]; act None, "silu", "gelu", "gelu_tanh" or "relu"; residual [B, n_out] of
+    ``dtype`` -> y [B, n_out] of ``dtype`` (bf16 or f32).  ``y`` and
     ``workspace`` (uint8, mi_bf16_linear_workspace bytes, needs no initialisation) make the call allocation-free; gradients
     are recorded without them only."""
     if x.dtype != torch.bfloat16 or x.dim() != 2:

@@ -101,7 +101,7 @@ class _RmsNorm(torch.autograd.Function):
 
 def rms_norm(x, weight, eps=1e-5, residual=None, y=None, stream=None):
     """y = s / sqrt(mean(s^2) + eps) * weight over the last dimension: x bf16 or f32 [..., D] (D a multiple of 8, up to
-    32768), weight bf16 or f32 [D] -> y as x.  With ``residual`` (as x) s = x + residual, rounded to their type, and the
+    32768; up to 2^22 rows, one less where D is past 8192), weight bf16 or f32 [D] -> y as x.  With ``residual`` (as x) s = x + residual, rounded to their type, and the
     result is (y, s): s is the stream that goes on, and y the norm of what it holds.  Rows may be strided.  ``y`` and
     ``stream``: outputs to write into.  Records the gradients of x, residual (the same one) and weight; not into
     preallocated outputs."""
